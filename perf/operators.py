@@ -74,10 +74,13 @@ _device = None
 
 
 def device():
-    """The process's one handle, on torch's stream."""
+    """The process's one handle.  It shares the stream that torch works on from then on: one of its own, since a handle takes
+    the default stream for its own."""
     global _device
     if _device is None:
         from ferrum_b200 import surface
+        torch.cuda.synchronize()
+        torch.cuda.set_stream(torch.cuda.Stream())
         _device = surface.Device(0)
     return _device
 
@@ -98,6 +101,8 @@ def _matrix(gen, rows, cols):
 
 
 def prepare(case, seed):
+    if own:
+        device()
     gen = torch.Generator(device="cuda")
     gen.manual_seed(int(seed) * 1000003 + 29)
     randn = lambda *shape: torch.randn(shape, device="cuda", generator=gen)
