@@ -13,7 +13,7 @@ LIB_PATH = os.path.join(HERE, "libferrum_b200.so")
 
 OK, ERR_SHAPE, ERR_RANGE, ERR_DEVICE, ERR_ALIAS, ERR_WEIGHT, ERR_SYNC, ERR_TIMEOUT, ERR_CUDA, ERR_PARAM, \
     ERR_UNSUPPORTED, ERR_GGUF = range(12)
-Q8_0, Q4_K, Q5_K, Q6_K, IQ4_NL, IQ4_XS = 8, 12, 13, 14, 20, 23
+Q8_0, Q4_K, Q5_K, Q6_K, IQ4_NL, IQ4_XS, I8 = 8, 12, 13, 14, 20, 23, 24
 F32, BF16 = 0, 30
 
 
@@ -104,6 +104,14 @@ SIGNATURES = {
     "fq_rmsnorm_project_many": (_I, [_P, C.POINTER(_P), _Z, _P, _P, C.c_float, _Z, _Z, _P, C.POINTER(_P)]),
     "fq_argmax": (_I, [_P, _P, _U32, _U32, _P]),
     "fq_topk_blocks": (_I, [_P, _P, _U32, _U32, _P]),
+    "fq_quantize_i8": (_I, [_P, _P, _I, _U32, _U32, _P, _P]),
+    "fq_rmsnorm_i8": (_I, [_P, _P, _I, _P, _U32, C.c_float, _U32, _P, _P]),
+    "fq_add_rmsnorm_i8": (_I, [_P, _P, _P, _I, _P, _U32, C.c_float, _U32, _P, _P, _P]),
+    "fq_glu_i8": (_I, [_P, _P, _P, _I, _U32, _U32, _P, _P]),
+    "fq_matrix_create_i8": (_I, [_P, _U64, _U64, _P, _P, C.POINTER(_P)]),
+    "fq_project_i8": (_I, [_P, _P, _P, _Z, _P, _Z, _P, _I, _Z]),
+    "fq_project_many_i8": (_I, [_P, C.POINTER(_P), _Z, _P, _Z, _P, _Z, C.POINTER(_P), _I]),
+    "fq_token_logprobs": (_I, [_P, _P, _I, _U32, _Z, _U32, _P, _U32, _P, _P, _P, _P, _P]),
     "fq_project_id": (_I, [_P, _P, _P, _Z, _P, _Z, _Z, _P, _Z]),
     "fq_project_mm_id": (_I, [_P, _P, _P, _I, _Z, _P, _P, _Z, _Z, _P, _I, _Z]),
     "fq_get_rows": (_I, [_P, _P, _P, _Z, _P, _I, _Z]),

@@ -711,6 +711,19 @@ static int check_dtype(fq_device *dev, int dt) {
     return (dt == FQ_F32 || dt == FQ_BF16) ? FQ_OK : fq_fail(dev, FQ_ERR_UNSUPPORTED, "element type %d", dt);
 }
 
+// Matrices of plain 8-bit integers take 8-bit rows with scales and have entry points of their own (gemm_i8.cu).
+static int check_format(fq_device *dev, const fq_matrix *w) {
+    if (w->format == FQ_I8) return fq_fail(dev, FQ_ERR_UNSUPPORTED, "a matrix of 8-bit integers is multiplied by fq_project_i8");
+    return FQ_OK;
+}
+
+// A matrix of this handle in one of the GGUF block formats.
+static int check_matrix(fq_device *dev, const fq_matrix *w) {
+    if (!w) return fq_fail(dev, FQ_ERR_PARAM, "null matrix");
+    if (w->dev != dev) return fq_fail(dev, FQ_ERR_DEVICE, "matrix belongs to another device handle");
+    return check_format(dev, w);
+}
+
 static bool is_iq4(uint32_t format) { return format == FQ_IQ4_NL || format == FQ_IQ4_XS; }
 
 // Small IQ4 matrices of more rows than k_nt packs into an MMA tile: its preparation launch and its ring cost more than the
@@ -742,8 +755,7 @@ static int launch_decode(fq_device *dev, const ProjectArgs *a, uint32_t count) {
 extern "C" int fq_project(fq_device *dev, const fq_matrix *w, const void *x, int x_dtype, size_t x_elems, size_t m,
                           void *y, int y_dtype, size_t y_elems) {
     if (int rc = fq_begin_enqueue(dev)) return rc;
-    if (!w) return fq_fail(dev, FQ_ERR_PARAM, "null matrix");
-    if (w->dev != dev) return fq_fail(dev, FQ_ERR_DEVICE, "matrix belongs to another device handle");
+    if (int rc = check_matrix(dev, w)) return rc;
     if (int rc = check_dtype(dev, x_dtype)) return rc;
     if (int rc = check_dtype(dev, y_dtype)) return rc;
     if (m == 0 || x_elems != m * w->cols || y_elems != m * w->rows)
@@ -777,8 +789,7 @@ extern "C" int fq_project_many(fq_device *dev, const fq_matrix *const *w, size_t
     if (count > MAX) return fq_fail(dev, FQ_ERR_PARAM, "at most %zu projections share an input", MAX);
     ProjectArgs args[MAX];
     for (size_t i = 0; i < count; i++) {
-        if (!w[i]) return fq_fail(dev, FQ_ERR_PARAM, "null matrix");
-        if (w[i]->dev != dev) return fq_fail(dev, FQ_ERR_DEVICE, "matrix belongs to another device handle");
+        if (int rc = check_matrix(dev, w[i])) return rc;
         if (m == 0 || x_elems != m * w[i]->cols)
             return fq_fail(dev, FQ_ERR_SHAPE, "projection [%zu, %llu] from %zu values", m, (unsigned long long)w[i]->cols, x_elems);
         const size_t xb = x_elems * fq_dtype_size(x_dtype), yb = m * w[i]->rows * fq_dtype_size(y_dtype);
@@ -812,6 +823,9 @@ extern "C" int fq_rmsnorm_project_many(fq_device *dev, const fq_matrix *const *w
     if (m == 0 || x_elems != m * cols || cols % 4) return fq_fail(dev, FQ_ERR_SHAPE, "normalised projection [%zu, %zu] from %zu values", m, cols, x_elems);
     if (int rc = fq_check_binding(dev, x, x_elems * 4, "x")) return rc;
     if (int rc = fq_check_binding(dev, norm_w, cols * 4, "norm_w")) return rc;
+    for (size_t i = 0; i < count; i++)
+        if (w[i])
+            if (int rc = check_format(dev, w[i])) return rc;
     bool fused = !dev->exact && m <= (size_t)FQ_GEMV_MAX_M && count <= 4;
     ProjectArgs args[4];
     for (size_t i = 0; i < count && fused; i++) {
@@ -854,6 +868,7 @@ extern "C" int fq_project_many_gather(fq_device *dev, fq_comm *comm, size_t regi
     size_t covered = 0;
     for (size_t i = 0; i < count; i++) {
         if (!w[i]) return fq_fail(dev, FQ_ERR_PARAM, "null matrix");
+        if (int rc = check_format(dev, w[i])) return rc;
         if ((const uint8_t *)y[i] != mine + covered)
             return fq_fail(dev, FQ_ERR_RANGE, "output %zu does not follow the output before it from the start of this rank's slice", i);
         covered += m * w[i]->rows * 4;
@@ -877,8 +892,7 @@ extern "C" int fq_project_many_gather(fq_device *dev, fq_comm *comm, size_t regi
 extern "C" int fq_project_id(fq_device *dev, const fq_matrix *w, const float *x, size_t x_elems, const uint32_t *ids,
                              size_t routes, size_t x_div, float *y, size_t y_elems) {
     if (int rc = fq_begin_enqueue(dev)) return rc;
-    if (!w) return fq_fail(dev, FQ_ERR_PARAM, "null matrix");
-    if (w->dev != dev) return fq_fail(dev, FQ_ERR_DEVICE, "matrix belongs to another device handle");
+    if (int rc = check_matrix(dev, w)) return rc;
     const size_t rows_e = w->expert_rows();
     if (routes == 0 || x_div == 0 || y_elems != routes * rows_e || x_elems * x_div != routes * w->cols)
         return fq_fail(dev, FQ_ERR_SHAPE, "expert projection geometry");
@@ -923,8 +937,7 @@ extern "C" int fq_project_mm_id(fq_device *dev, const fq_matrix *w, const void *
                                 const uint32_t *offsets, const uint32_t *slots, size_t groups, size_t max_rows,
                                 void *y, int y_dtype, size_t y_elems) {
     if (int rc = fq_begin_enqueue(dev)) return rc;
-    if (!w) return fq_fail(dev, FQ_ERR_PARAM, "null matrix");
-    if (w->dev != dev) return fq_fail(dev, FQ_ERR_DEVICE, "matrix belongs to another device handle");
+    if (int rc = check_matrix(dev, w)) return rc;
     if (int rc = check_dtype(dev, x_dtype)) return rc;
     if (int rc = check_dtype(dev, y_dtype)) return rc;
     const size_t rows_e = w->expert_rows();
@@ -959,8 +972,7 @@ extern "C" int fq_project_mm_id(fq_device *dev, const fq_matrix *w, const void *
 extern "C" int fq_get_rows(fq_device *dev, const fq_matrix *w, const uint32_t *ids, size_t tokens, void *y, int y_dtype,
                            size_t y_elems) {
     if (int rc = fq_begin_enqueue(dev)) return rc;
-    if (!w) return fq_fail(dev, FQ_ERR_PARAM, "null matrix");
-    if (w->dev != dev) return fq_fail(dev, FQ_ERR_DEVICE, "matrix belongs to another device handle");
+    if (int rc = check_matrix(dev, w)) return rc;
     if (int rc = check_dtype(dev, y_dtype)) return rc;
     if (tokens == 0 || y_elems != tokens * w->cols) return fq_fail(dev, FQ_ERR_SHAPE, "embedding lookup geometry");
     if (int rc = fq_check_binding(dev, ids, tokens * 4, "ids")) return rc;
@@ -1100,6 +1112,8 @@ static int project_id_pair(fq_device *dev, const fq_matrix *w0, const fq_matrix 
 extern "C" int fq_dense_ffn(fq_device *dev, const fq_matrix *gate, const fq_matrix *up, const fq_matrix *down,
                             const float *x, size_t m, float *scratch, size_t scratch_elems, float *out) {
     if (!dev || !gate || !up || !down) return fq_fail(dev, FQ_ERR_PARAM, "null matrix");
+    for (const fq_matrix *w : {gate, up, down})
+        if (int rc = check_matrix(dev, w)) return rc;
     const size_t width = gate->rows;
     if (up->rows != width || up->cols != gate->cols || down->cols != width)
         return fq_fail(dev, FQ_ERR_SHAPE, "feed-forward matrices do not chain");
@@ -1186,7 +1200,7 @@ extern "C" int fq_moe_ffn(fq_device *dev, const fq_moe_ffn_desc *f, const float 
         f->down_exps->cols != ef || f->shared_gate->rows != f->shared_ffn || f->shared_down->rows != hidden)
         return fq_fail(dev, FQ_ERR_SHAPE, "MoE matrices do not match the description");
     for (const fq_matrix *w : {f->router, f->gate_exps, f->up_exps, f->down_exps, f->shared_gate, f->shared_up, f->shared_down})
-        if (w->dev != dev) return fq_fail(dev, FQ_ERR_DEVICE, "matrix belongs to another device handle");
+        if (int rc = check_matrix(dev, w)) return rc;
     MoeScratch s = moe_layout(f, m, scratch);
     if (scratch_elems < s.total) return fq_fail(dev, FQ_ERR_SHAPE, "MoE scratch holds %zu of %zu floats", scratch_elems, s.total);
     const size_t routes = m * used;
@@ -1271,6 +1285,8 @@ extern "C" int fq_moe_ffn_ep(fq_device *dev, fq_comm *comm, size_t region_offset
         f->down_exps->expert_rows() != hidden || f->down_exps->cols != ef || f->shared_gate->rows != f->shared_ffn ||
         f->shared_down->rows != hidden || local * (size_t)world != experts || expert_first != (size_t)rank * local)
         return fq_fail(dev, FQ_ERR_SHAPE, "MoE matrices do not match the description or the expert split");
+    for (const fq_matrix *w : {f->router, f->gate_exps, f->up_exps, f->down_exps, f->shared_gate, f->shared_up, f->shared_down})
+        if (int rc = check_format(dev, w)) return rc;
     MoeScratch s = moe_layout(f, m, scratch);
     if (scratch_elems < s.total) return fq_fail(dev, FQ_ERR_SHAPE, "MoE scratch holds %zu of %zu floats", scratch_elems, s.total);
     const size_t routes = m * used;

@@ -95,6 +95,7 @@ struct fq_matrix {
     uint64_t pitch = 0; // bytes between rows of the device layout (see fq_row_pitch)
     uint32_t block_elems = 0, block_bytes = 0;
     uint8_t *data = nullptr; // device copy of the blocks in the device layout
+    float *scales = nullptr; // FQ_I8: one per row, in the allocation of `data`
     uint64_t expert_rows() const { return rows / experts; }
 };
 

@@ -16,7 +16,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import BF16, F32, Q4_K, Q6_K, Q8_0  # noqa: F401  (re-exported)
+from ._lib import BF16, F32, I8, Q4_K, Q6_K, Q8_0  # noqa: F401  (re-exported)
 
 
 class FerrumError(RuntimeError):
@@ -386,6 +386,19 @@ class Matrix:
         device.check(device._L.fq_matrix_from_gguf(device.handle, file.handle, name.encode(), experts, rows, cols, int(q3k_as_q6k), C.byref(h)))
         return cls(device, h)
 
+    @classmethod
+    def from_i8(cls, device: Device, values, scales) -> "Matrix":
+        """A matrix of 8-bit integers ``values`` [rows, cols] with one fp32 scale per row, for ``project_i8``.  Both are
+        tensors on the CPU or the handle's device, or arrays."""
+        values, scales = (t if isinstance(t, torch.Tensor) else torch.from_numpy(np.ascontiguousarray(t)) for t in (values, scales))
+        if values.dtype != torch.int8 or scales.dtype != torch.float32:
+            raise Unsupported(f"8-bit matrix of {values.dtype} with scales of {scales.dtype}")
+        if values.dim() != 2 or scales.numel() != values.shape[0] or not values.is_contiguous() or not scales.is_contiguous():
+            raise ShapeError(f"8-bit matrix {tuple(values.shape)} with {scales.numel()} scales")
+        h = C.c_void_p()
+        device.check(device._L.fq_matrix_create_i8(device.handle, values.shape[0], values.shape[1], _ptr(values), _ptr(scales), C.byref(h)))
+        return cls(device, h)
+
     def byte_size(self) -> int:
         return self._byte_size
 
@@ -480,6 +493,101 @@ def topk_blocks(d: Device, x: torch.Tensor, n: int, rows: int, out: torch.Tensor
     """``h_topk_blocks``: per 1024-value block the 32 largest (value, index) pairs, descending."""
     _need(d, x, out)
     d.check(d._L.fq_topk_blocks(d.handle, _ptr(x), n, rows, _ptr(out)))
+
+
+def _want(t: Optional[torch.Tensor], dtype: torch.dtype, count: int, name: str) -> None:
+    if t is None:
+        return
+    if t.dtype != dtype:
+        raise Unsupported(f"{name} of {t.dtype}")
+    if t.numel() != count:
+        raise ShapeError(f"{name} of {t.numel()} values for {count}")
+
+
+def _rows_i8(x: torch.Tensor, rows: int, q: torch.Tensor, scales: torch.Tensor) -> int:
+    """Checks the outputs of ``rows`` rows in 8 bits; the length of a row."""
+    n = x.numel() // rows if rows > 0 else 0
+    if rows <= 0 or n * rows != x.numel():
+        raise ShapeError(f"{x.numel()} values as {rows} rows")
+    _want(q, torch.int8, x.numel(), "q")
+    _want(scales, torch.float32, rows, "scales")
+    return n
+
+
+def quantize_i8(d: Device, x: torch.Tensor, rows: int, q: torch.Tensor, scales: torch.Tensor) -> None:
+    """``rows`` rows of F32 or BF16 values as 8-bit integers with a scale per row."""
+    _need(d, x, q, scales)
+    n = _rows_i8(x, rows, q, scales)
+    d.check(d._L.fq_quantize_i8(d.handle, _ptr(x), _dtype_id(x), n, rows, _ptr(q), _ptr(scales)))
+
+
+def rmsnorm_i8(d: Device, x: torch.Tensor, w: torch.Tensor, eps: float, rows: int, q: torch.Tensor, scales: torch.Tensor) -> None:
+    """``rmsnorm`` with its rows in 8 bits: q * scale = rmsnorm(x) * w."""
+    _need(d, x, w, q, scales)
+    n = _rows_i8(x, rows, q, scales)
+    _want(w, torch.float32, n, "w")
+    d.check(d._L.fq_rmsnorm_i8(d.handle, _ptr(x), _dtype_id(x), _ptr(w), n, eps, rows, _ptr(q), _ptr(scales)))
+
+
+def add_rmsnorm_i8(d: Device, x: torch.Tensor, r: torch.Tensor, w: torch.Tensor, eps: float, rows: int, h: torch.Tensor, q: torch.Tensor,
+                   scales: torch.Tensor) -> None:
+    """``add_rmsnorm`` with its rows in 8 bits: h = x + r, q * scale = rmsnorm(h) * w."""
+    _need(d, x, r, w, h, q, scales)
+    n = _rows_i8(x, rows, q, scales)
+    _want(r, x.dtype, x.numel(), "r")
+    _want(h, x.dtype, x.numel(), "h")
+    _want(w, torch.float32, n, "w")
+    d.check(d._L.fq_add_rmsnorm_i8(d.handle, _ptr(x), _ptr(r), _dtype_id(x), _ptr(w), n, eps, rows, _ptr(h), _ptr(q), _ptr(scales)))
+
+
+def glu_i8(d: Device, gate: torch.Tensor, up: torch.Tensor, rows: int, q: torch.Tensor, scales: torch.Tensor) -> None:
+    """``glu`` with its rows in 8 bits: q * scale = silu(gate) * up."""
+    _need(d, gate, up, q, scales)
+    n = _rows_i8(gate, rows, q, scales)
+    _want(up, gate.dtype, gate.numel(), "up")
+    d.check(d._L.fq_glu_i8(d.handle, _ptr(gate), _ptr(up), _dtype_id(gate), n, rows, _ptr(q), _ptr(scales)))
+
+
+def project_i8(d: Device, w: Matrix, x: torch.Tensor, x_scales: torch.Tensor, m: int, y: torch.Tensor) -> None:
+    """y[m, rows] = (x[m, cols] . W^T) * x_scales * the scales of W's rows, x and W in 8-bit integers (``Matrix.from_i8``)."""
+    _need(d, x, x_scales, y)
+    _want(x, torch.int8, x.numel(), "x")
+    _want(x_scales, torch.float32, m, "x_scales")
+    d.check(d._L.fq_project_i8(d.handle, w.handle, _ptr(x), x.numel(), _ptr(x_scales), m, _ptr(y), _dtype_id(y), y.numel()))
+
+
+def project_many_i8(d: Device, ws: Sequence[Matrix], x: torch.Tensor, x_scales: torch.Tensor, m: int, ys: Sequence[torch.Tensor]) -> None:
+    """``project_i8`` by up to eight matrices of one width that share x (q|k|v, gate|up), in one launch."""
+    _need(d, x, x_scales, *ys)
+    n = len(ws)
+    if n == 0 or len(ys) != n:
+        raise ParameterError(f"{n} matrices for {len(ys)} outputs")
+    _want(x, torch.int8, x.numel(), "x")
+    _want(x_scales, torch.float32, m, "x_scales")
+    for w, y in zip(ws, ys):
+        _want(y, ys[0].dtype, m * w.rows, "output")
+    wa = (C.c_void_p * n)(*[w.handle.value for w in ws])
+    ya = (C.c_void_p * n)(*[y.data_ptr() for y in ys])
+    d.check(d._L.fq_project_many_i8(d.handle, wa, n, _ptr(x), x.numel(), _ptr(x_scales), m, ya, _dtype_id(ys[0])))
+
+
+def token_logprobs(d: Device, logits: torch.Tensor, n: int, rows: int, ids: Optional[torch.Tensor], logprobs: Optional[torch.Tensor],
+                   ranks: Optional[torch.Tensor], entropy: Optional[torch.Tensor], k: int = 0, top_logprobs: Optional[torch.Tensor] = None,
+                   top_ids: Optional[torch.Tensor] = None, stride: Optional[int] = None) -> None:
+    """Log probability and rank of the token ``ids[r]`` under row r of ``rows`` rows of n logits (``stride`` values apart, n by
+    default), the rows' entropy, and their k most likely tokens.  Outputs that are None are not computed."""
+    _need(d, logits, ids, logprobs, ranks, entropy, top_logprobs, top_ids)
+    stride = n if stride is None else stride
+    if n <= 0 or rows <= 0 or stride < n or logits.numel() < (rows - 1) * stride + n:
+        raise ShapeError(f"{logits.numel()} values as {rows} rows of {n} logits, {stride} apart")
+    if k < 0:
+        raise ParameterError(f"{k} alternatives")
+    for t, dtype, count, name in ((ids, torch.int32, rows, "ids"), (logprobs, torch.float32, rows, "logprobs"), (ranks, torch.int32, rows, "ranks"),
+                                  (entropy, torch.float32, rows, "entropy"), (top_logprobs, torch.float32, rows * k, "top_logprobs"),
+                                  (top_ids, torch.int32, rows * k, "top_ids")):
+        _want(t, dtype, count, name)
+    d.check(d._L.fq_token_logprobs(d.handle, _ptr(logits), _dtype_id(logits), n, stride, rows, _ptr(ids), k, _ptr(logprobs), _ptr(ranks),
+                                   _ptr(entropy), _ptr(top_logprobs), _ptr(top_ids)))
 
 
 def project_id(d: Device, w: Matrix, x: torch.Tensor, ids: torch.Tensor, routes: int, x_div: int, y: torch.Tensor) -> None:

@@ -52,8 +52,9 @@ typedef enum fq_status {
  * 1..16 rows, and grouped ones of up to 48 rows per expert and 2304 columns, run on the integer tensor path with
  * activations rounded to 31 bits of the largest of their 256 values, which loses less than fp32 sums do; per-route
  * expert projections of up to 16384 columns round them to 16 bits of the largest of their 32; everything else runs on
- * the exact fp32 kernels. */
-typedef enum fq_format { FQ_Q8_0 = 8, FQ_Q4_K = 12, FQ_Q5_K = 13, FQ_Q6_K = 14, FQ_IQ4_NL = 20, FQ_IQ4_XS = 23 } fq_format;
+ * the exact fp32 kernels.  I8 (plain 8-bit integers, one scale per row) is the format of `fq_matrix_create_i8` and of the
+ * 8-bit entry points only: every other one refuses such a matrix with FQ_ERR_UNSUPPORTED. */
+typedef enum fq_format { FQ_Q8_0 = 8, FQ_Q4_K = 12, FQ_Q5_K = 13, FQ_Q6_K = 14, FQ_IQ4_NL = 20, FQ_IQ4_XS = 23, FQ_I8 = 24 } fq_format;
 
 /* Activation / output element types (GGML ids of F32 and BF16). */
 typedef enum fq_dtype { FQ_F32 = 0, FQ_BF16 = 30 } fq_dtype;
@@ -246,6 +247,56 @@ int fq_argmax(fq_device *dev, const float *x, uint32_t n, uint32_t rows, uint32_
  * pairs in descending order, ties to the lower index; out[(r * ceil(n / 1024) + block) * 32 + k] = {value, index
  * as the bits of a float}. */
 int fq_topk_blocks(fq_device *dev, const float *x, uint32_t n, uint32_t rows, float *out);
+
+/* ---- 8-bit activations and weights (no counterpart in the reference) --------------------------- */
+
+/* Rows of activations as 8-bit integers with one scale per row: q[r][i] = round(127 v[i] / max|v|), to the nearest whole
+ * number and ties to even of the exact quotient (every value that goes into it is taken in 64 bits where that decides), and
+ * scales[r] so that q * scale is the row.
+ *   fq_quantize_i8      v = x
+ *   fq_rmsnorm_i8       v = x * rsqrt(mean(x^2) + eps) * w
+ *   fq_add_rmsnorm_i8   h = x + r (written to h, rounded to its type, which is x's), v = h * rsqrt(mean(h^2) + eps) * w;
+ *                       h may be x or r itself
+ *   fq_glu_i8           v = silu(gate) * up
+ * The row inputs are F32 or BF16, `rows` rows of n values (a multiple of 4); w is F32.  A row of zeros has scale 0.  A row
+ * with an infinity or a NaN among its inputs or its v (for the norms: among h * w) has scale NaN and q = 0, which makes NaN of everything
+ * projected from it and of nothing else. */
+int fq_quantize_i8(fq_device *dev, const void *x, int x_dtype, uint32_t n, uint32_t rows, int8_t *q, float *scales);
+int fq_rmsnorm_i8(fq_device *dev, const void *x, int x_dtype, const float *w, uint32_t n, float eps, uint32_t rows, int8_t *q, float *scales);
+int fq_add_rmsnorm_i8(fq_device *dev, const void *x, const void *r, int x_dtype, const float *w, uint32_t n, float eps, uint32_t rows, void *h,
+                      int8_t *q, float *scales);
+int fq_glu_i8(fq_device *dev, const void *gate, const void *up, int dtype, uint32_t n, uint32_t rows, int8_t *q, float *scales);
+/* A matrix of 8-bit integers, [rows][cols], with a scale for each row; cols is a multiple of 16 and at most 65536.  `values`
+ * and `scales` may be host memory or memory of the handle's device (read in the order of the handle's stream; the call waits
+ * for the copy), e.g. what `fq_quantize_i8` makes of a matrix of floats.  Scales must be finite (FQ_ERR_WEIGHT).
+ * `fq_matrix_destroy` and `fq_matrix_get_info` as for the other formats (byte_size = rows * (cols + 4)). */
+int fq_matrix_create_i8(fq_device *dev, uint64_t rows, uint64_t cols, const int8_t *values, const float *scales, fq_matrix **out);
+/* y[t][o] = (sum_k x[t][k] w[o][k]) * x_scales[t] * w_scale[o] for m rows of 8-bit integers.  The sum is exact at every
+ * width; it is rounded to fp32 once, multiplied by the token's scale, then by the row's, and stored as F32 or BF16 (RNE).
+ * x_elems must be m * cols and y_elems m * rows.  `fq_project_many_i8` is up to eight matrices of one width that share x
+ * (q|k|v, gate|up) in one launch; y[i] receives m * rows_i values. */
+int fq_project_i8(fq_device *dev, const fq_matrix *w, const int8_t *x, size_t x_elems, const float *x_scales, size_t m, void *y, int y_dtype,
+                  size_t y_elems);
+int fq_project_many_i8(fq_device *dev, const fq_matrix *const *w, size_t count, const int8_t *x, size_t x_elems, const float *x_scales, size_t m,
+                       void *const *y, int y_dtype);
+
+/* ---- scores of tokens (no counterpart in the reference) ------------------------------------------ */
+
+/* What the output head's logits l say of a row's token ids[r], and of the row: with z = log sum_j exp(l_j),
+ *   logprobs[r]  l_id - z            ranks[r]    1 + the number of logits above l_id
+ *   entropy[r]   z - sum_j exp(l_j - z) l_j
+ *   top_ids / top_logprobs [r][k]    the k (0..32, at most n) most likely tokens in descending order, ties to the lower id.
+ * Logits are F32 or BF16: `rows` rows of n, the first of each `stride` values (at least n) after the one before; what lies
+ * between the rows is not read.  An output that is not wanted is NULL (top_ids and top_logprobs are when k = 0), and so is `ids`
+ * when neither logprobs nor ranks are wanted.
+ * A logit of -infinity is a token of probability 0: it adds nothing, and its own log probability is -infinity.  A row with a
+ * NaN, with +infinity, or with nothing above -infinity has no distribution: its log probabilities and entropy are NaN; ranks
+ * and top_ids still follow the order of the logits, a NaN below everything.  An id that is not below n names no token (a row
+ * of padding): log probability NaN, rank 0.  Logits may start at any element and the other arrays at any 4 bytes. */
+int fq_token_logprobs(fq_device *dev, const void *logits, int dtype, uint32_t n, size_t stride, uint32_t rows, const uint32_t *ids, uint32_t k,
+                      float *logprobs, uint32_t *ranks, float *entropy, float *top_logprobs, uint32_t *top_ids);
+
+/* ---- experts ------------------------------------------------------------------------------------ */
 
 /* `HybridModel::project_id(d, w, x, ids, routes, x_div, y)` (src/hybrid/engine.rs:3114-3147):
  * route r multiplies activation row r / x_div by the rows of expert ids[r]; F32 in and out. */

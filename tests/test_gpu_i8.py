@@ -1,0 +1,399 @@
+"""Rows in 8 bits and their projections against the same in 64 bits.  The 8-bit values and the projections' sums are exact, so
+they are compared bit for bit; a scale is one fp32 number rounded from 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+EPS = 1e-6
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def S():
+    from ferrum_b200 import surface
+    return surface
+
+
+def gpu(a, dtype=F32):
+    return torch.as_tensor(np.ascontiguousarray(a)).to(dtype).cuda()
+
+
+def f64(t):
+    return t.detach().cpu().double().numpy()
+
+
+def rows_to_8_bits(v, factor):
+    """The definition on 64-bit rows: whole numbers (ties to even) and scales."""
+    a = np.abs(v).max(axis=1, keepdims=True)
+    q = np.rint(v * 127 / np.where(a > 0, a, 1))
+    return q, (a * factor / 127)[:, 0]
+
+
+def values_of(op, x, r, w):
+    """(v, factor, h) of the operators' definition in 64 bits from tensors as they are passed."""
+    if op == "quantize":
+        return f64(x), 1.0, None
+    if op == "glu":
+        g, u = f64(x), f64(r)
+        with np.errstate(over="ignore"):
+            return g / (1 + np.exp(-g)) * u, 1.0, None
+    h = x if op == "rmsnorm" else (x.float().cpu() + r.float().cpu()).to(x.dtype)
+    v = f64(h)
+    return v * f64(w), 1 / np.sqrt((v * v).mean(axis=1, keepdims=True) + np.float64(np.float32(EPS))), h
+
+
+def run_op(d, op, x, r, w, rows, h=None):
+    n = x.numel() // rows
+    q, s = torch.full((rows + 1, n), 99, dtype=torch.int8, device="cuda"), torch.full((rows + 4,), -7.0, device="cuda")
+    qq, ss = q[:rows], s[:rows]
+    if op == "quantize":
+        S().quantize_i8(d, x, rows, qq, ss)
+    elif op == "rmsnorm":
+        S().rmsnorm_i8(d, x, w, EPS, rows, qq, ss)
+    elif op == "add":
+        S().add_rmsnorm_i8(d, x, r, w, EPS, rows, h, qq, ss)
+    else:
+        S().glu_i8(d, x, r, rows, qq, ss)
+    d.synchronize()
+    assert torch.all(q[rows:] == 99) and torch.all(s[rows:] == -7), "nothing behind the last row is written"
+    return qq.cpu().numpy(), ss.cpu().numpy()
+
+
+def check_rows(op, x, r, w, q, s):
+    v, factor, _ = values_of(op, x, r, w)
+    want_q, want_s = rows_to_8_bits(v, factor)
+    assert np.array_equal(q, want_q), np.argwhere(q != want_q)[:5]
+    # Half an fp32 step, and the few 2^-53 of the sum of squares; scales below 2^-126 have steps of 2^-149.
+    assert np.all(np.abs(s - want_s) <= want_s * 2.0 ** -24 * (1 + 1e-6) + 2.0 ** -149)
+
+
+OPS = ["quantize", "rmsnorm", "add", "glu"]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows", [1, 3, 310])
+@pytest.mark.parametrize("n", [4, 12, 128, 132, 516, 1024, 2048, 2052, 4100, 5120, 8200, 17408, 70004])
+@pytest.mark.parametrize("op", OPS)
+def test_rows_of_every_length(device, op, n, rows, dtype):
+    if n > 20000 and rows > 3:
+        rows = 150
+    rng = np.random.default_rng(n + rows)
+    x = gpu(rng.standard_normal((rows, n)) * (1 + 30 * (rng.random(n) < 0.01)), dtype)
+    r, w = gpu(rng.standard_normal((rows, n)), dtype), gpu(1 + 0.1 * rng.standard_normal(n))
+    h = torch.zeros_like(x)
+    q, s = run_op(device, op, x, r, w, rows, h)
+    check_rows(op, x, r, w, q, s)
+    if op == "add":
+        assert torch.equal(h.cpu(), values_of(op, x, r, w)[2])
+        for place in (x.clone(), r.clone()):  # the sum in place of either input
+            first = place if torch.equal(place, x) else x
+            second = r if first is place else place
+            assert np.array_equal(run_op(device, op, first, second, w, rows, place)[0], q) and torch.equal(place, h)
+
+
+@pytest.mark.parametrize("op", ["rmsnorm", "glu"])
+def test_values_next_to_a_border_fall_on_its_right_side(device, op):
+    """Inputs for which the same formula in 32 bits rounds some values to the wrong whole number."""
+    rows, n = 512, 8192
+    rng = np.random.default_rng(5)
+    x, r, w = gpu(rng.standard_normal((rows, n))), gpu(rng.standard_normal((rows, n))), gpu(1 + 0.1 * rng.standard_normal(n))
+    v, factor, _ = values_of(op, x, r, w)
+    a, b, c = (t.cpu().numpy() for t in (x, r, w))
+    v32 = a * c if op == "rmsnorm" else a / (1 + np.exp(-a)) * b  # all of it in 32 bits
+    v32 = v32 * (np.float32(127) / np.abs(v32).max(axis=1, keepdims=True))
+    assert v32.dtype == np.float32
+    assert np.any(np.rint(v32) != rows_to_8_bits(v, factor)[0]), "the inputs hold no such value"
+    check_rows(op, x, r, w, *run_op(device, op, x, r, w, rows))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_ties_go_to_the_even_number(device, dtype):
+    v = np.concatenate([[127.0], np.arange(-126.5, 127, 1.0), [0.5, 1.5, -0.5, 2.5]])
+    v = np.concatenate([v, np.zeros(-len(v) % 4)])[None]
+    for scale in (1.0, 2.0 ** -40, 2.0 ** 60):
+        x = gpu(v * scale, dtype)
+        check_rows("quantize", x, None, None, *run_op(device, "quantize", x, None, None, 1))
+        ones = torch.ones(v.shape[1], device="cuda")
+        check_rows("rmsnorm", x, None, ones, *run_op(device, "rmsnorm", x, None, ones, 1))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [64, 5120])
+@pytest.mark.parametrize("op", OPS)
+def test_rows_of_extreme_values(device, op, n, dtype):
+    rng = np.random.default_rng(n)
+    x = rng.standard_normal((12, n))
+    x[0] = 0
+    x[1] *= 1e-30
+    x[2] *= 2.0 ** -130   # subnormal in fp32
+    x[3] *= 1e37 / np.abs(x[3]).max()
+    x[4], x[5, :-1] = 0, 0
+    x[4, n // 2] = -3.0
+    x[5, -1] = 1e-38
+    x[6] = -100.0 + x[6]  # a gate that closes: silu of -100
+    r = rng.standard_normal((12, n))
+    r[3] *= 1e-3
+    r[0] = 0 if op != "glu" else r[0]
+    if op == "glu":
+        r[7] = 0
+    x, r, w = gpu(x, dtype), gpu(r, dtype), gpu(1 + 0.1 * rng.standard_normal(n))
+    q, s = run_op(device, op, x, r, w, 12, torch.zeros_like(x))
+    check_rows(op, x, r, w, q, s)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [64, 5120])
+@pytest.mark.parametrize("op", OPS)
+def test_a_row_that_is_not_finite_spoils_itself_only(device, op, n, dtype):
+    rng = np.random.default_rng(n + 1)
+    x, r = rng.standard_normal((9, n)), rng.standard_normal((9, n))
+    for row, bad in ((1, np.inf), (3, -np.inf), (5, np.nan)):
+        x[row, rng.integers(n)] = bad
+    if op in ("add", "glu"):
+        r[7, rng.integers(n)] = np.nan
+    x, r, w = gpu(x, dtype), gpu(r, dtype), gpu(1 + 0.1 * rng.standard_normal(n))
+    q, s = run_op(device, op, x, r, w, 9, torch.zeros_like(x))
+    bad = [1, 3, 5] + ([7] if op in ("add", "glu") else [])
+    good = [i for i in range(9) if i not in bad]
+    assert np.all(np.isnan(s[bad])) and not q[bad].any()
+    pick = lambda t: None if t is None else t[good]
+    check_rows(op, pick(x), pick(r), w, q[good], s[good])
+
+
+def matrix(rng, d, rows, cols):
+    wq = rng.integers(-128, 128, (rows, cols), dtype=np.int8)
+    ws = (0.01 + rng.random(rows)).astype(np.float32) * rng.choice([-1, 1], rows).astype(np.float32)
+    return S().Matrix.from_i8(d, wq, ws), wq, ws
+
+
+def expect(xq, xs, wq, ws):
+    """Exact sums (whole numbers in 64 bits), rounded to fp32, times the token's scale, times the row's: fp32 steps."""
+    acc = (torch.from_numpy(xq).double().cuda() @ torch.from_numpy(wq).double().cuda().T).cpu().numpy()
+    return acc.astype(np.float32) * xs[:, None] * ws[None]
+
+
+def project(d, mats, xq, xs, dtype, many):
+    m = len(xq)
+    bufs = [torch.full((m * w.rows + 64,), 5.5, dtype=dtype, device="cuda") for w in mats]
+    ys = [b[:m * w.rows] for b, w in zip(bufs, mats)]
+    x, scales = torch.from_numpy(xq).cuda(), torch.from_numpy(xs).cuda()
+    if many:
+        S().project_many_i8(d, mats, x, scales, m, ys)
+    else:
+        for w, y in zip(mats, ys):
+            S().project_i8(d, w, x, scales, m, y)
+    d.synchronize()
+    assert all(torch.all(b[m * w.rows:] == 5.5) for b, w in zip(bufs, mats)), "nothing behind the last row is written"
+    return [y.view(m, w.rows) for y, w in zip(ys, mats)]
+
+
+def same(y, want):
+    return torch.equal(y.cpu(), torch.from_numpy(want).to(y.dtype))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("m", [1, 2, 7, 16, 17, 33, 64, 65, 128, 130, 256, 257, 300, 513])
+@pytest.mark.parametrize("rows,cols", [(1, 16), (100, 48), (128, 128), (129, 144), (300, 1040), (1000, 2048), (2500, 4096), (5121, 528)])
+def test_projections_of_every_shape(device, rows, cols, m, dtype):
+    rng = np.random.default_rng(rows + m)
+    w, wq, ws = matrix(rng, device, rows, cols)
+    xq, xs = rng.integers(-128, 128, (m, cols), dtype=np.int8), rng.random(m).astype(np.float32)
+    assert same(project(device, [w], xq, xs, dtype, False)[0], expect(xq, xs, wq, ws))
+
+
+@pytest.mark.parametrize("m", [1, 16, 260])
+def test_the_largest_sums(device, m):
+    """65536 products of 2^14: 2^30 fits, and so does its negative."""
+    wq, ws = np.full((130, 65536), -128, np.int8), np.ones(130, np.float32)
+    w = S().Matrix.from_i8(device, wq, ws)
+    xq, xs = np.full((m, 65536), -128, np.int8), np.ones(m, np.float32)
+    xq[m // 2] = 127
+    assert same(project(device, [w], xq, xs, F32, False)[0], expect(xq, xs, wq, ws))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("m", [1, 5, 40, 200, 700])
+@pytest.mark.parametrize("shapes", [(6144, 1024, 1024), (257, 1), (130, 1000, 3, 64, 128, 129, 7, 640)])
+def test_several_matrices_in_one_launch(device, shapes, m, dtype):
+    rng = np.random.default_rng(m)
+    cols = 1296
+    mats = [matrix(rng, device, r, cols) for r in shapes]
+    xq, xs = rng.integers(-127, 128, (m, cols), dtype=np.int8), rng.random(m).astype(np.float32)
+    ys = project(device, [w for w, _, _ in mats], xq, xs, dtype, True)
+    for y, (_, wq, ws) in zip(ys, mats):
+        assert same(y, expect(xq, xs, wq, ws))
+    again = project(device, [mats[0][0]] * 2, xq, xs, dtype, True)  # the same matrix twice
+    assert torch.equal(again[0], ys[0]) and torch.equal(again[1], ys[0])
+
+
+def test_a_matrix_made_on_the_device_or_the_host(device):
+    rng = np.random.default_rng(0)
+    x = gpu(rng.standard_normal((300, 272)))
+    q, s = torch.zeros(300, 272, dtype=torch.int8, device="cuda"), torch.zeros(300, device="cuda")
+    S().quantize_i8(device, x, 300, q, s)  # weights of floats, quantised where they are
+    mats = [S().Matrix.from_i8(device, q, s), S().Matrix.from_i8(device, q.cpu(), s.cpu()), S().Matrix.from_i8(device, q.cpu().numpy(), s)]
+    assert (mats[0].rows, mats[0].cols, mats[0].experts, mats[0].format, mats[0].byte_size()) == (300, 272, 1, S().I8, 300 * 276)
+    xq, xs = rng.integers(-127, 128, (3, 272), dtype=np.int8), np.ones(3, np.float32)
+    ys = project(device, mats, xq, xs, F32, True)
+    assert same(ys[0], expect(xq, xs, q.cpu().numpy(), s.cpu().numpy())) and torch.equal(ys[0], ys[1]) and torch.equal(ys[0], ys[2])
+
+
+def test_scales_that_are_not_finite_spoil_their_row_only(device):
+    rng = np.random.default_rng(3)
+    w, wq, ws = matrix(rng, device, 200, 160)
+    xq, xs = rng.integers(-127, 128, (6, 160), dtype=np.int8), rng.random(6).astype(np.float32)
+    want = expect(xq, xs, wq, ws)
+    xs[2] = np.nan
+    y = project(device, [w], xq, xs, F32, False)[0].cpu().numpy()
+    assert np.all(np.isnan(y[2])) and np.array_equal(np.delete(y, 2, 0), np.delete(want, 2, 0))
+
+
+def test_refused_calls(device):
+    s, d = S(), device
+    x, w = torch.zeros(4, 64, device="cuda"), torch.ones(64, device="cuda")
+    q, sc = torch.zeros(4, 64, dtype=torch.int8, device="cuda"), torch.zeros(4, device="cuda")
+    before = d.counters().dispatches
+    with pytest.raises(s.ShapeError):
+        s.quantize_i8(d, x, 3, q, sc)
+    with pytest.raises(s.ShapeError):  # rows of 6 values
+        s.quantize_i8(d, x.view(-1)[:24], 4, q.view(-1)[:24], sc)
+    with pytest.raises(s.Unsupported):
+        s.quantize_i8(d, x.half(), 4, q, sc)
+    with pytest.raises(s.Unsupported):
+        s.quantize_i8(d, x, 4, q.view(torch.uint8), sc)
+    with pytest.raises(s.AliasError):
+        s.quantize_i8(d, x, 4, x.view(torch.int8).view(-1)[:256].view(4, 64), sc)
+    with pytest.raises(s.AliasError):
+        s.rmsnorm_i8(d, x, w, EPS, 4, q, w[:4])
+    with pytest.raises(s.RangeError):
+        s.rmsnorm_i8(d, x.view(-1)[1:253 - 188], w[:16], EPS, 4, q.view(-1)[:64], sc)
+    with pytest.raises(s.AliasError):  # h over part of x
+        s.add_rmsnorm_i8(d, x[:2], x[2:], w, EPS, 2, x[1:3], q[:2], sc[:2])
+    with pytest.raises(s.Unsupported):
+        s.add_rmsnorm_i8(d, x, x.bfloat16(), w, EPS, 4, x.clone(), q, sc)
+    with pytest.raises(s.Unsupported):
+        s.glu_i8(d, x, x.bfloat16(), 4, q, sc)
+    with pytest.raises(s.ShapeError):
+        s.glu_i8(d, x, x[:2], 4, q, sc)
+    with pytest.raises(s.DeviceMismatch):
+        s.glu_i8(d, x, x.cpu(), 4, q, sc)
+    ok = s.Matrix.from_i8(d, np.ones((32, 64), np.int8), np.ones(32, np.float32))
+    for bad, error in (((np.ones((32, 24), np.int8), np.ones(32, np.float32)), s.ShapeError), ((np.ones((32, 65552), np.int8), np.ones(32, np.float32)), s.ShapeError),
+                       ((np.ones((32, 64), np.int8), np.ones(31, np.float32)), s.ShapeError), ((np.ones((32, 64), np.uint8), np.ones(32, np.float32)), s.Unsupported),
+                       ((np.ones((32, 64), np.int8), np.full(32, np.inf, np.float32)), s.WeightError)):
+        with pytest.raises(error):
+            s.Matrix.from_i8(d, *bad)
+    y = torch.zeros(4, 32, device="cuda")
+    with pytest.raises(s.ShapeError):
+        s.project_i8(d, ok, q, sc, 4, y[:3])
+    with pytest.raises(s.ShapeError):
+        s.project_i8(d, ok, q[:3], sc, 4, y)
+    with pytest.raises(s.ShapeError):
+        s.project_i8(d, ok, q, sc[:3], 4, y)
+    with pytest.raises(s.Unsupported):
+        s.project_i8(d, ok, q, sc, 4, y.half())
+    with pytest.raises(s.Unsupported):
+        s.project_i8(d, ok, x, sc, 4, y)
+    with pytest.raises(s.AliasError):
+        s.project_many_i8(d, [ok, ok], q, sc, 4, [y, y])
+    with pytest.raises(s.ParameterError):
+        s.project_many_i8(d, [ok] * 9, q, sc, 4, [torch.zeros(4, 32, device="cuda") for _ in range(9)])
+    with pytest.raises(s.ParameterError):
+        s.project_many_i8(d, [], q, sc, 4, [])
+    other = s.Device(0)
+    with pytest.raises(s.DeviceMismatch):
+        s.project_i8(other, ok, q, sc, 4, y)
+    from oracle import ref
+    packed = s.Matrix.from_packed(d, 32, 64, 1, s.Q8_0, ref.random_matrix(ref.Q8_0, 32, 64, seed=0))
+    with pytest.raises(s.Unsupported):
+        s.project_i8(d, packed, q, sc, 4, y)
+    ids = torch.zeros(4, dtype=torch.int32, device="cuda")
+    for call in (lambda: s.project(d, ok, x, 4, y), lambda: s.project_many(d, [packed, ok], x, 4, [y, y.clone()]),
+                 lambda: s.rmsnorm_project_many(d, [packed, ok], x, w, EPS, 4, [y, y.clone()], torch.zeros_like(x)),
+                 lambda: s.project_id(d, ok, x, ids, 4, 1, y), lambda: s.project_mm_id(d, ok, x, torch.tensor([0, 4], dtype=torch.int32, device="cuda"), 4, y),
+                 lambda: s.get_rows(d, ok, ids, x.clone()), lambda: s.dense_ffn(d, packed, packed, ok, x, 4, torch.zeros(4 * 96, device="cuda"), x.clone())):
+        with pytest.raises(s.Unsupported):
+            call()
+    assert d.counters().dispatches == before, "a refused call enqueues nothing"
+
+
+def test_a_layer_on_8_bits_captured_and_replayed():
+    """norm -> gate | up -> gated unit -> down -> norm -> output head -> scores on the handle's own stream: eagerly, then as a
+    graph that is replayed on other inputs, beside a second graph of the same handle."""
+    s = S()
+    d = s.Device(0, use_torch_stream=False)
+    rng = np.random.default_rng(11)
+    hidden, ffn, vocab = 256, 688, 1003
+    mats = {n: matrix(rng, d, r, c) for n, (r, c) in {"gate": (ffn, hidden), "up": (ffn, hidden), "down": (hidden, ffn), "head": (vocab, hidden)}.items()}
+    w1, w2 = gpu(1 + 0.1 * rng.standard_normal(hidden)), gpu(1 + 0.1 * rng.standard_normal(hidden))
+
+    def state(m):
+        new = lambda *shape, dtype=F32: torch.zeros(shape, dtype=dtype, device="cuda")
+        return {"m": m, "x": new(m, hidden), "r": new(m, hidden), "h": new(m, hidden), "q": new(m, hidden, dtype=torch.int8), "s": new(m),
+                "g": new(m, ffn), "u": new(m, ffn), "a": new(m, ffn, dtype=torch.int8), "as": new(m), "d": new(m, hidden), "h2": new(m, hidden),
+                "l": new(m, vocab), "ids": torch.arange(m, dtype=torch.int32, device="cuda"), "lp": new(m), "rk": new(m, dtype=torch.int32),
+                "en": new(m), "tp": new(m, 4), "ti": new(m, 4, dtype=torch.int32)}
+
+    def step(t):
+        m = t["m"]
+        s.add_rmsnorm_i8(d, t["x"], t["r"], w1, EPS, m, t["h"], t["q"], t["s"])
+        s.project_many_i8(d, [mats["gate"][0], mats["up"][0]], t["q"], t["s"], m, [t["g"], t["u"]])
+        s.glu_i8(d, t["g"], t["u"], m, t["a"], t["as"])
+        s.project_i8(d, mats["down"][0], t["a"], t["as"], m, t["d"])
+        s.add_rmsnorm_i8(d, t["h"], t["d"], w2, EPS, m, t["h2"], t["q"], t["s"])
+        s.project_i8(d, mats["head"][0], t["q"], t["s"], m, t["l"])
+        s.token_logprobs(d, t["l"], vocab, m, t["ids"], t["lp"], t["rk"], t["en"], 4, t["tp"], t["ti"])
+
+    def fill(t, seed):
+        g = torch.Generator().manual_seed(seed)
+        t["x"].copy_(torch.randn(t["m"], hidden, generator=g))
+        t["r"].copy_(torch.randn(t["m"], hidden, generator=g))
+        torch.cuda.synchronize()
+
+    def check(t):
+        x, r = t["x"], t["r"]
+        v, factor, h = values_of("add", x, r, w1)
+        q, sc = rows_to_8_bits(v, factor)
+        sc = sc.astype(np.float32)
+        proj = lambda n, q, sc: expect(q.astype(np.int8), sc, mats[n][1], mats[n][2])
+        assert torch.equal(t["h"].cpu(), h)
+        # The scale is the kernel's (half a step from 64 bits at most); everything behind it is bit for bit from there.
+        g, u = t["g"].cpu(), t["u"].cpu()
+        close = lambda a, b: np.all(np.abs(a - b) <= np.abs(b) * 2.0 ** -22)
+        assert close(g.numpy(), proj("gate", q, sc)) and close(u.numpy(), proj("up", q, sc))
+        v, factor, _ = values_of("glu", g, u, None)
+        a, asc = rows_to_8_bits(v, factor)
+        assert np.array_equal(t["a"].cpu().numpy(), a)
+        assert close(t["d"].cpu().numpy(), proj("down", a, asc.astype(np.float32)))
+        v, factor, h2 = values_of("add", t["h"], t["d"], w2)
+        q, sc = rows_to_8_bits(v, factor)
+        assert np.array_equal(t["q"].cpu().numpy(), q) and torch.equal(t["h2"].cpu(), h2)
+        l = f64(t["l"])
+        assert close(l, proj("head", q, sc.astype(np.float32)))
+        z = np.log(np.exp(l - l.max(1, keepdims=True)).sum(1)) + l.max(1)
+        got = l[np.arange(t["m"]), np.arange(t["m"])]
+        # These logits reach thousands, where one fp32 rounding of the result is 2^-24 of it; 1e-4 is for the sums.
+        assert np.all(np.abs(t["lp"].cpu().numpy() - (got - z)) <= np.abs(got - z) * 2.0 ** -23 + 1e-4)
+        assert np.array_equal(t["rk"].cpu().numpy(), 1 + (l > got[:, None]).sum(1))
+        assert np.array_equal(t["ti"].cpu().numpy(), np.argsort(-l, axis=1, kind="stable")[:, :4])
+
+    a, b = state(3), state(40)
+    fill(a, 1), fill(b, 2)
+    step(a), step(b)
+    d.synchronize()
+    check(a), check(b)
+    graphs = []
+    for t in (a, b):
+        d.capture_begin()
+        step(t)
+        graphs.append(d.capture_end())
+    fill(a, 3), fill(b, 4)
+    for _ in range(2):
+        for g in graphs:
+            g.launch()
+    d.synchronize()
+    check(a), check(b)
+    for g in graphs:
+        g.close()
+    d.close()

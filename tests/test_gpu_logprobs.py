@@ -1,0 +1,232 @@
+"""Scores of tokens against the same in 64 bits: log probabilities, ranks, entropy and the most likely tokens, at the row
+lengths, strides, masks and ties where a kernel that reads a row once, in pieces, can go wrong."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def S():
+    from ferrum_b200 import surface
+    return surface
+
+
+def run(d, l, n, ids, k, stride=None):
+    """`l`: a flat CUDA tensor of logits.  Outputs with a guard behind them."""
+    rows = len(ids)
+    new = lambda count, dtype, fill: torch.full((count + 4,), fill, dtype=dtype, device="cuda")
+    lp, rk, en = new(rows, F32, 9.5), new(rows, torch.int32, -9), new(rows, F32, 9.5)
+    tp, ti = new(rows * k, F32, 9.5), new(rows * k, torch.int32, -9)
+    S().token_logprobs(d, l, n, rows, torch.from_numpy(np.asarray(ids, np.int64).astype(np.uint32).view(np.int32)).cuda(), lp[:rows], rk[:rows], en[:rows], k,
+                       tp[:rows * k] if k else None, ti[:rows * k] if k else None, stride)
+    d.synchronize()
+    for t, count in ((lp, rows), (rk, rows), (en, rows), (tp, rows * k), (ti, rows * k)):
+        assert torch.all(t[count:] == (9.5 if t.dtype == F32 else -9))
+    out = [t[:c].cpu().numpy() for t, c in ((lp, rows), (rk, rows), (en, rows), (tp, rows * k), (ti, rows * k))]
+    return out[:3] + [o.reshape(rows, k) for o in out[3:]]
+
+
+def check(l, ids, k, got):
+    """`l`: [rows, n] float64 of exactly the logits that were passed."""
+    lp, rk, en, tp, ti = got
+    rows, n = l.shape
+    with np.errstate(all="ignore"):
+        mx = l.max(axis=1)
+        e = np.exp(l - mx[:, None])
+        s = e.sum(axis=1)
+        z = mx + np.log(s)
+        p = e / s[:, None]
+        entropy = -np.where(p > 0, p * (l - z[:, None]), 0).sum(axis=1)
+        z, entropy = np.where(np.isfinite(mx), z, np.nan), np.where(np.isfinite(mx), entropy, np.nan)
+        inside = np.asarray(ids) < n
+        given = np.where(inside, l[np.arange(rows), np.where(inside, ids, 0)], np.nan)
+        want = given - z
+        rank = np.where(inside, 1 + (l > given[:, None]).sum(axis=1), 0)
+    order = np.argsort(np.where(np.isnan(l), np.inf, -l), axis=1, kind="stable")
+    # NaN goes behind -infinity, which the key above cannot say: only rows without NaN are compared by it.
+    clean = ~np.isnan(l).any(axis=1)
+    # Sums: a term exp(d) carries the roundings of d (|d| * 2^-24 twice), 2^-22 of the exponential, and the additions of a
+    # thread's share (n / 256 at the most) and of a tree; far terms weigh nothing, so |d| is taken at 100.  The entropy's
+    # second sum has one rounding more in terms of at most |d| times the first's.
+    sums = (2 * 100 + 4 + n / 256 + 24) * 2.0 ** -24
+    off = lambda v: np.abs(v) * 2.0 ** -23 + sums
+    def near(a, b, off):
+        with np.errstate(all="ignore"):
+            return np.array_equal(np.isnan(a), np.isnan(b)) and np.all((a == b) | np.isnan(b) | (np.abs(a - b) <= off))
+    assert near(lp, want, off(want)), (lp, want)
+    span = np.log(n) + 1
+    assert near(en, entropy, off(entropy) * (1 + span)), (en, entropy)
+    assert np.array_equal(rk, rank), (rk, rank)
+    if k:
+        assert np.array_equal(ti[clean], order[clean, :k])
+        top = l[np.arange(rows)[:, None], ti]
+        with np.errstate(all="ignore"):
+            want = top - z[:, None]
+        assert near(tp, want, off(want))
+
+
+def logits(rng, rows, n):
+    l = 2.5 * rng.standard_normal((rows, n))
+    l[np.arange(rows), rng.integers(0, n, rows)] += 12
+    return l
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows", [1, 5, 130, 700])
+@pytest.mark.parametrize("n", [1, 2, 3, 7, 31, 33, 128, 1000, 4099, 32000, 50257, 151936])
+def test_rows_of_every_length(device, n, rows, dtype):
+    if n > 40000 and rows > 130:
+        rows = 300
+    rng = np.random.default_rng(n + rows)
+    l = torch.from_numpy(logits(rng, rows, n)).to(dtype)
+    ids = rng.integers(0, n, rows)
+    ids[::2] = l.float().argmax(1).numpy()[::2]
+    for k in {0, 1, min(n, 5), min(n, 32)}:
+        check(l.double().numpy(), ids, k, run(device, l.cuda().view(-1), n, ids, k))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows", [1, 9, 200])
+@pytest.mark.parametrize("n", [20, 777, 33000])
+def test_masked_rows(device, n, rows, dtype):
+    """Masks of -infinity and of the type's lowest value, at random, all but one token, the first part, everything."""
+    rng = np.random.default_rng(n + rows)
+    low = torch.finfo(dtype).min
+    for kind in range(6):
+        l = torch.from_numpy(logits(rng, rows, n)).to(dtype)
+        mask = torch.from_numpy(rng.random((rows, n)) < 0.5)
+        keep = rng.integers(0, n, rows)
+        if kind in (1, 4):
+            mask[:] = True
+            mask[np.arange(rows), keep] = False
+        if kind == 2:
+            mask[:] = False
+            mask[:, :n - n // 8] = True
+        if kind == 5:
+            mask[:] = True
+        l = l.masked_fill(mask, -float("inf") if kind in (0, 1, 2, 5) else low)
+        ids = rng.integers(0, n, rows)
+        ids[::2] = keep[::2]
+        check(l.double().numpy(), ids, min(n, 32), run(device, l.cuda().view(-1), n, ids, min(n, 32)))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows", [1, 40])
+def test_ties_and_orders(device, rows, dtype):
+    """Equal logits (the two zeros among them), rising and falling rows, a few values in all: ties go to the lower id."""
+    n = 20011
+    rng = np.random.default_rng(rows)
+    for row in (np.zeros(n), np.full(n, -3.25), np.where(rng.random(n) < 0.5, 0.0, -0.0), np.arange(n) / 1024.0, -np.arange(n) / 1024.0,
+                rng.integers(0, 3, n), rng.integers(0, 40, n), np.full(n, -np.inf)):
+        l = torch.from_numpy(np.tile(np.asarray(row, np.float64), (rows, 1))).to(dtype)
+        ids = rng.integers(0, n, rows)
+        check(l.double().numpy(), ids, 32, run(device, l.cuda().view(-1), n, ids, 32))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_large_offsets_and_peaks(device, dtype):
+    """Rows shifted far from zero, one token that takes nearly everything, values that grow towards the end of the row."""
+    n, rng = 9000, np.random.default_rng(1)
+    rows = []
+    for shift in (0, 1000, -1000, 3e4):
+        rows.append(np.round(rng.standard_normal(n) * 4) + shift)
+    peak = rng.standard_normal(n)
+    peak[4567] = 60
+    late = rng.standard_normal(n) - 200
+    late[-5:] = 150
+    l = torch.from_numpy(np.stack(rows + [peak, late, np.linspace(-300, 300, n)])).to(dtype)
+    ids = np.array([0, 5, 8999, 17, 4567, 8996, 3])
+    check(l.double().numpy(), ids, 32, run(device, l.cuda().view(-1), n, ids, 32))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_rows_without_a_distribution(device, dtype):
+    n, rng = 3000, np.random.default_rng(2)
+    for n in (17, 3000, 40000):
+        l = logits(rng, 8, n)
+        l[1, n // 3] = np.nan
+        l[3, 0] = np.inf
+        l[4, n - 1] = np.inf
+        l[4, n // 2] = np.nan
+        l[6, :] = np.nan
+        t = torch.from_numpy(l).to(dtype)
+        ids = rng.integers(0, n, 8)
+        got = run(device, t.cuda().view(-1), n, ids, 8)
+        x = t.double().numpy()
+        ordered = np.where(np.isnan(x), -1e300, np.where(np.isinf(x), 1e300, x))  # no -infinity here: NaN is below everything
+        assert np.array_equal(got[4], np.argsort(-ordered, axis=1, kind="stable")[:, :8])
+        for row in (1, 3, 4, 6):
+            assert np.isnan(got[0][row]) and np.isnan(got[2][row]) and np.all(np.isnan(got[3][row]))
+        with np.errstate(all="ignore"):
+            assert np.array_equal(got[1], 1 + (x > x[np.arange(8), ids][:, None]).sum(1))
+        good = [0, 2, 5, 7]
+        check(x[good], ids[good], 8, [g[good] for g in got])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,stride,first", [(1000, 1024, 0), (1001, 1001, 1), (1001, 1003, 3), (997, 1003, 5), (33000, 33007, 7), (151936, 151943, 1)])
+def test_padded_and_unaligned_rows(device, n, stride, first, dtype):
+    """Rows apart, and a buffer that begins anywhere; what lies between the rows is NaN and infinity and is not read."""
+    rng, rows = np.random.default_rng(n), 6
+    l = torch.from_numpy(logits(rng, rows, n)).to(dtype)
+    whole = torch.full((first + rows * stride + 64,), float("nan"), dtype=dtype)
+    whole[::2] = float("inf")
+    for r in range(rows):
+        whole[first + r * stride:first + r * stride + n] = l[r]
+    buf = whole.cuda()[first:first + (rows - 1) * stride + n]
+    ids = rng.integers(0, n, rows)
+    check(l.double().numpy(), ids, 16, run(device, buf, n, ids, 16, stride))
+
+
+def test_padding_rows_and_unwanted_outputs(device):
+    """Ids that name no token, the same id in every row, and each output alone with the same values."""
+    s, rng, n = S(), np.random.default_rng(4), 5000
+    l = torch.from_numpy(logits(rng, 6, n)).float()
+    ids = np.array([7, 0xFFFFFFFF, 4999, 5000, 7, 7])
+    got = run(device, l.cuda().view(-1), n, ids, 3)
+    assert np.isnan(got[0][[1, 3]]).all() and not got[1][[1, 3]].any()
+    check(l.double().numpy(), ids, 3, got)
+    x, new = l.cuda(), lambda dtype, *shape: torch.zeros(shape, dtype=dtype, device="cuda")
+    dev_ids = torch.from_numpy(ids.astype(np.uint32).view(np.int32)).cuda()
+    lp, rk, en, tp, ti = new(F32, 6), new(torch.int32, 6), new(F32, 6), new(F32, 6, 3), new(torch.int32, 6, 3)
+    s.token_logprobs(device, x, n, 6, dev_ids, lp, None, None)
+    s.token_logprobs(device, x, n, 6, dev_ids, None, rk, None)
+    s.token_logprobs(device, x, n, 6, None, None, None, en)
+    s.token_logprobs(device, x, n, 6, None, None, None, None, 3, tp, ti)
+    device.synchronize()
+    for a, b in zip((lp, rk, en, tp, ti), got):
+        assert np.array_equal(a.cpu().numpy(), b, equal_nan=a.dtype == F32)
+
+
+def test_repeated_calls_give_the_same_bits(device):
+    rng = np.random.default_rng(6)
+    for rows, n in ((1, 151936), (17, 50001), (400, 3001)):
+        l = torch.from_numpy(logits(rng, rows, n)).float().cuda().view(-1)
+        ids = rng.integers(0, n, rows)
+        first = run(device, l, n, ids, 32)
+        for _ in range(3):
+            assert all(np.array_equal(a, b) for a, b in zip(first, run(device, l, n, ids, 32)))
+
+
+def test_refused_calls(device):
+    s, d = S(), device
+    l, ids = torch.zeros(4, 100, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda")
+    lp, rk, en = torch.zeros(4, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda"), torch.zeros(4, device="cuda")
+    tp, ti = torch.zeros(4, 33, device="cuda"), torch.zeros(4, 33, dtype=torch.int32, device="cuda")
+    before = d.counters().dispatches
+    for call, error in ((lambda: s.token_logprobs(d, l, 101, 4, ids, lp, rk, en), s.ShapeError), (lambda: s.token_logprobs(d, l, 100, 4, ids, lp, rk, en, stride=99), s.ShapeError),
+                        (lambda: s.token_logprobs(d, l, 100, 4, ids[:3], lp, rk, en), s.ShapeError), (lambda: s.token_logprobs(d, l, 100, 4, ids, lp[:3], rk, en), s.ShapeError),
+                        (lambda: s.token_logprobs(d, l.half(), 100, 4, ids, lp, rk, en), s.Unsupported), (lambda: s.token_logprobs(d, l, 100, 4, ids.long(), lp, rk, en), s.Unsupported),
+                        (lambda: s.token_logprobs(d, l, 100, 4, None, lp, None, en), s.ParameterError), (lambda: s.token_logprobs(d, l, 100, 4, ids, None, None, None), s.ParameterError),
+                        (lambda: s.token_logprobs(d, l, 100, 4, ids, lp, rk, en, 33, tp, ti), s.ParameterError),
+                        (lambda: s.token_logprobs(d, l, 4, 4, ids, lp, rk, en, 5, tp.view(-1)[:20], ti.view(-1)[:20]), s.ParameterError),
+                        (lambda: s.token_logprobs(d, l, 100, 4, ids, lp, rk, en, 2, None, ti.view(-1)[:8]), s.RangeError),
+                        (lambda: s.token_logprobs(d, l, 100, 4, ids, lp, rk, lp), s.AliasError), (lambda: s.token_logprobs(d, l, 100, 4, ids, lp, ids, en), s.AliasError),
+                        (lambda: s.token_logprobs(d, l, 100, 4, ids, l.view(-1)[:4], rk, en), s.AliasError),
+                        (lambda: s.token_logprobs(d, l.cpu(), 100, 4, ids, lp, rk, en), s.DeviceMismatch)):
+        with pytest.raises(error):
+            call()
+    assert d.counters().dispatches == before, "a refused call enqueues nothing"
