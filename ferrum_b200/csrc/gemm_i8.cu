@@ -1,56 +1,374 @@
-// Projections of 8-bit rows by 8-bit matrices:
+// Projections of 8-bit rows by 8-bit matrices on the fifth-generation tensor cores (kind::i8, sums in tensor memory):
 //
 //   y[t][o] = (sum_k x[t][k] w[o][k]) * x_scale[t] * w_scale[o]
 //
-// The sum is a whole number of at most 2^14 * 65536 < 2^31 and exact; it is converted to fp32 once (rounded past 2^24), multiplied by the
-// token's scale and then by the row's, and rounded to the output's type.
+// The sum is a whole number of at most 2^14 * 65536 < 2^31 and exact at every width and however it is cut; it is converted to
+// fp32 once, multiplied by the token's scale and then by the row's, and rounded to the output's type.
+//
+// Weights sit on the MMA's M side (128 rows), tokens on its N side (16..256), so one kernel serves one token and a prompt.
+// `fq_matrix_create_i8` lays the matrix out in tiles of 128 rows x 128 bytes of K, each stored in the 128-byte-swizzled order
+// in which the MMA reads shared memory, one after the other along K: a tile is one contiguous copy of 16 KB without a tensor
+// map, and a block's share of the weights is one run of memory.
+//
+//   warp 0       one thread copies the weight tiles (cp.async.bulk) and, by TMA, the tokens' 128 bytes of K beside them;
+//   warp 1       one thread issues tcgen05.mma (M = 128, N = the token tile, K = 32, four per stage);
+//   warps 2..5   read the accumulator, scale and store.  The accumulator is double: the next tile's MMAs run meanwhile.
+//
+// Blocks walk (row tile, token tile) items.  Where there are fewer items than blocks the machine holds, a cluster of up to
+// eight blocks cuts an item's K and adds the partial sums (whole numbers, so in any order) through distributed shared memory:
+// block r of the cluster collects and stores the tokens of its share.  All waits are bounded (tcgen05.cuh).
+#include <algorithm>
 #include <cmath>
 #include <vector>
 
 #include "gemv_common.cuh"
 #include "internal.h"
+#include "tcgen05.cuh"
 
 namespace {
+using namespace fqtc;
+using fqk::pdl_trigger;
+using fqk::pdl_wait;
 
-constexpr uint32_t TILE = 64;
+constexpr uint32_t BM = 128;              // weight rows of a tile (MMA M)
+constexpr uint32_t BK = 128;              // bytes of K of a stage: one swizzle row
+constexpr uint32_t TILE_BYTES = BM * BK;
+constexpr uint32_t MAX_STAGES = 12;
+constexpr uint32_t MAX_MANY = 8, MAX_SLICES = 8;
+constexpr uint32_t EPILOGUE_WARPS = 4, THREADS = (2 + EPILOGUE_WARPS) * 32;
+constexpr uint32_t SMEM_MAX = 227 * 1024;
 
-// 64 weight rows x 64 tokens a block, 4 x 4 outputs a thread, 64 bytes of K at a time through shared memory.
-template <typename YT>
-__global__ void __launch_bounds__(256)
-k_project_i8(const int8_t *__restrict__ w, const float *__restrict__ ws, uint32_t rows, uint32_t cols, const int8_t *__restrict__ x,
-             const float *__restrict__ xs, uint32_t m, YT *__restrict__ y) {
-    __shared__ int a[TILE][17], b[TILE][17];
-    const uint32_t tid = threadIdx.x, r0 = blockIdx.x * TILE, t0 = blockIdx.y * TILE;
-    int acc[4][4] = {};
-    for (uint32_t k0 = 0; k0 < cols; k0 += 64) {
-        for (uint32_t i = tid; i < TILE * 16; i += 256) {
-            const uint32_t row = i / 16, k = k0 + 4 * (i % 16);
-            a[row][i % 16] = r0 + row < rows && k < cols ? *(const int *)(w + (size_t)(r0 + row) * cols + k) : 0;
-            b[row][i % 16] = t0 + row < m && k < cols ? *(const int *)(x + (size_t)(t0 + row) * cols + k) : 0;
-        }
-        __syncthreads();
-        for (uint32_t k = 0; k < 16; k++)
-            for (uint32_t i = 0; i < 4; i++)
-                for (uint32_t j = 0; j < 4; j++) acc[i][j] = __dp4a(a[(tid & 15) + 16 * i][k], b[(tid >> 4) + 16 * j][k], acc[i][j]);
-        __syncthreads();
-    }
-    for (uint32_t i = 0; i < 4; i++)
-        for (uint32_t j = 0; j < 4; j++) {
-            const uint32_t row = r0 + (tid & 15) + 16 * i, t = t0 + (tid >> 4) + 16 * j;
-            if (row >= rows || t >= m) continue;
-            const float v = (float)acc[i][j] * xs[t] * ws[row];
-            if constexpr (sizeof(YT) == 2) y[(size_t)t * rows + row] = __float2bfloat16_rn(v);
-            else y[(size_t)t * rows + row] = v;
-        }
+struct Target {
+    const uint8_t *w; // tiles
+    const float *scales;
+    void *y;
+    uint32_t rows;
+    uint32_t tile_end; // row tiles up to and including this matrix
+};
+struct Job {
+    Target t[MAX_MANY];
+    const float *x_scales;
+    uint32_t count, m;
+    uint32_t k_blocks;           // of the whole K
+    uint32_t bn, token_tiles;    // tokens of a tile (a multiple of 16) and how many tiles cover m
+    uint32_t items;              // row tiles of all matrices * token_tiles
+    uint32_t slices, per;        // blocks of a cluster, k-blocks each
+    uint32_t stages, box_bytes;  // of the ring; bytes of one TMA box of tokens
+    uint32_t tmem_cols;
+    int bf16;
+};
+
+struct Ctl {
+    uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc_full[2], acc_empty[2], drained;
+    uint32_t tmem_base, abort_flag;
+};
+
+// kind::i8: D = s32, A = B = s8, both K-major.
+__device__ __forceinline__ uint32_t idesc_i8(uint32_t n) { return (2u << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((BM >> 4) << 24); }
+__device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}"
+                 ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, int (&v)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+                   "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                 : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_address(uint32_t saddr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void store_cluster(uint32_t addr, int v) { asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
-int launch_one(fq_device *dev, const fq_matrix *w, const int8_t *x, const float *xs, uint32_t m, void *y, int y_dtype) {
-    const uint32_t rows = (uint32_t)w->rows, cols = (uint32_t)w->cols;
-    const dim3 grid((rows + TILE - 1) / TILE, (m + TILE - 1) / TILE);
-    if (y_dtype == FQ_BF16)
-        k_project_i8<<<grid, 256, 0, dev->stream>>>((const int8_t *)w->data, w->scales, rows, cols, x, xs, m, (__nv_bfloat16 *)y);
-    else k_project_i8<<<grid, 256, 0, dev->stream>>>((const int8_t *)w->data, w->scales, rows, cols, x, xs, m, (float *)y);
-    return FQ_OK;
+// Where an item lies: its matrix, row tile and token tile.  Token tiles run fastest, so that blocks that run together share
+// weight tiles in L2.
+struct Place {
+    uint32_t which, tile, m0;
+};
+__device__ __forceinline__ Place place_of(const Job &J, uint32_t item) {
+    Place p;
+    uint32_t tile = item / J.token_tiles, first = 0;
+    p.m0 = (item - tile * J.token_tiles) * J.bn;
+    p.which = 0;
+    for (uint32_t i = 0; i + 1 < J.count; i++)
+        if (tile >= J.t[i].tile_end) {
+            p.which = i + 1;
+            first = J.t[i].tile_end;
+        }
+    p.tile = tile - first;
+    return p;
+}
+
+__device__ __forceinline__ void store_value(const Job &J, const Target &T, uint32_t token, uint32_t row, int acc, float xs, float ws) {
+    const float v = (float)acc * xs * ws;
+    const size_t at = (size_t)token * T.rows + row;
+    if (J.bf16) static_cast<__nv_bfloat16 *>(T.y)[at] = __float2bfloat16_rn(v);
+    else static_cast<float *>(T.y)[at] = v;
+}
+
+template <bool SLICED>
+__global__ void __launch_bounds__(THREADS)
+k_gemm_i8(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ Job J, int *status) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ Ctl ctl;
+    uint8_t *ring = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, stage_bytes = TILE_BYTES + J.bn * BK;
+    const uint32_t slice = SLICED ? blockIdx.x % J.slices : 0, unit = SLICED ? blockIdx.x / J.slices : blockIdx.x, units = SLICED ? gridDim.x / J.slices : gridDim.x;
+    const uint32_t k_first = slice * J.per, k_iters = min(J.per, J.k_blocks - k_first);
+    pdl_trigger();
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < J.stages; s++) {
+            mbar_init(&ctl.full[s], 1);
+            mbar_init(&ctl.empty[s], 1);
+        }
+        for (int b = 0; b < 2; b++) {
+            mbar_init(&ctl.acc_full[b], 1);
+            mbar_init(&ctl.acc_empty[b], EPILOGUE_WARPS * 32);
+        }
+        mbar_init(&ctl.drained, 1);
+        ctl.abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&xmap) : "memory");
+    }
+    if (warp == 1) {
+        __syncwarp();
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl.tmem_base)), "r"(J.tmem_cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *(volatile uint32_t *)&ctl.tmem_base;
+
+    if (warp == 0) {
+        if (elect_one()) {
+            auto weights = [&](const Place &p, uint32_t it) {
+                return J.t[p.which].w + ((size_t)p.tile * J.k_blocks + k_first + it) * TILE_BYTES;
+            };
+            // The weights are nobody's output: the first ones are under way before the kernel ahead has finished.
+            const uint32_t primed = unit < J.items ? min(J.stages, k_iters) : 0;
+            for (uint32_t it = 0; it < primed; it++) {
+                mbar_expect_tx(&ctl.full[it], TILE_BYTES + J.box_bytes);
+                bulk_load(ring + it * stage_bytes, weights(place_of(J, unit), it), TILE_BYTES, &ctl.full[it]);
+            }
+            pdl_wait();
+            uint32_t s = 0, phase = 0, issued = 0;
+            bool ok = true;
+            for (uint32_t item = unit; item < J.items && ok; item += units) {
+                const Place p = place_of(J, item);
+                for (uint32_t it = 0; it < k_iters; it++) {
+                    if (issued >= primed) {
+                        if (!(ok = mbar_wait(&ctl.empty[s], phase ^ 1, &ctl, status))) break;
+                        mbar_expect_tx(&ctl.full[s], TILE_BYTES + J.box_bytes);
+                        bulk_load(ring + s * stage_bytes, weights(p, it), TILE_BYTES, &ctl.full[s]);
+                    }
+                    tma_load_2d(ring + s * stage_bytes + TILE_BYTES, &xmap, (int)((k_first + it) * BK), (int)p.m0, &ctl.full[s]);
+                    issued++;
+                    if (++s == J.stages) s = 0, phase ^= 1;
+                }
+            }
+            // After an abort the copies under way still land: wait for them (bounded) before the shared memory goes away.
+            if (*(volatile uint32_t *)&ctl.abort_flag)
+                for (uint32_t ib = issued > J.stages ? issued - J.stages : 0; ib < issued; ib++)
+                    for (uint32_t i = 0; i < WAIT_LIMIT && !mbar_try(&ctl.full[ib % J.stages], (ib / J.stages) & 1); i++) {}
+        }
+    } else if (warp == 1) {
+        if (elect_one()) {
+            pdl_wait(); // the clock of the bounded waits starts when there is something to wait for
+            const uint32_t idesc = idesc_i8(J.bn);
+            uint32_t s = 0, phase = 0, buf = 0, buf_phase = 0;
+            bool ok = true;
+            for (uint32_t item = unit; item < J.items && ok; item += units) {
+                if (!mbar_wait(&ctl.acc_empty[buf], buf_phase ^ 1, &ctl, status)) break;
+                const uint32_t acc = tmem + buf * J.bn;
+                for (uint32_t it = 0; it < k_iters; it++) {
+                    if (!(ok = mbar_wait(&ctl.full[s], phase, &ctl, status))) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t at = smem_u32(ring + s * stage_bytes);
+                    const uint64_t a = umma_desc(at), b = umma_desc(at + TILE_BYTES);
+#pragma unroll
+                    for (uint32_t k = 0; k < BK / 32; k++) umma_i8(acc, a + 2 * k, b + 2 * k, idesc, (it | k) != 0);
+                    umma_commit(&ctl.empty[s]);
+                    if (++s == J.stages) s = 0, phase ^= 1;
+                }
+                if (ok) umma_commit(&ctl.acc_full[buf]);
+                if (++buf == 2) buf = 0, buf_phase ^= 1;
+            }
+            // Everything this thread issued has finished (after an abort too) before the accumulators are released.
+            umma_commit(&ctl.drained);
+            for (uint32_t i = 0; i < WAIT_LIMIT && !mbar_try(&ctl.drained, 0, WAIT_HINT_NS); i++) {}
+        }
+    } else {
+        pdl_wait(); // x_scales may be, and what y held may still be in use by, the kernel ahead
+    }
+
+    const uint32_t quarter = warp & 3; // the tensor-memory lanes a warp may read
+    if constexpr (!SLICED) {
+        if (warp >= 2) {
+            uint32_t buf = 0, buf_phase = 0;
+            for (uint32_t item = unit; item < J.items; item += units) {
+                const Place p = place_of(J, item);
+                const Target &T = J.t[p.which];
+                const uint32_t row = p.tile * BM + 32 * quarter + lane, live = min(J.bn, J.m - p.m0);
+                const float ws = row < T.rows ? T.scales[row] : 0.f;
+                if (!__all_sync(0xffffffffu, mbar_wait(&ctl.acc_full[buf], buf_phase, &ctl, status))) break; // the warp agrees
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t acc = tmem + buf * J.bn + ((32 * quarter) << 16);
+                for (uint32_t c0 = 0; c0 < live; c0 += 16) {
+                    const uint32_t mine = c0 + (lane & 15);
+                    const float xs = mine < live ? __ldcg(J.x_scales + p.m0 + mine) : 0.f;
+                    int v[16];
+                    tmem_ld16(acc + c0, v);
+#pragma unroll
+                    for (uint32_t c = 0; c < 16; c++) {
+                        const float f = __shfl_sync(0xffffffffu, xs, c);
+                        if (row < T.rows && c0 + c < live) store_value(J, T, p.m0 + c0 + c, row, v[c], f, ws);
+                    }
+                }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                mbar_arrive(&ctl.acc_empty[buf]);
+                if (++buf == 2) buf = 0, buf_phase ^= 1;
+            }
+        }
+    } else { // one item per cluster; every thread passes both barriers whatever happened
+        const Place p = place_of(J, unit);
+        const Target &T = J.t[p.which];
+        const uint32_t live = min(J.bn, J.m - p.m0), share = (live + J.slices - 1) / J.slices;
+        const uint32_t mine = slice * share, mine_end = min(live, mine + share), acc = tmem + ((32 * quarter) << 16);
+        if (warp >= 2 && mbar_wait(&ctl.acc_full[0], 0, &ctl, status)) asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        __syncthreads();
+        cluster_sync(); // every block's MMAs have read their ring (or given up): it takes the partial sums now
+        if (warp >= 2 && *(volatile uint32_t *)&ctl.abort_flag == 0) {
+            for (uint32_t c0 = 0; c0 < live; c0 += 16) {
+                int v[16];
+                tmem_ld16(acc + c0, v);
+#pragma unroll
+                for (uint32_t c = 0; c < 16; c++) {
+                    const uint32_t col = c0 + c, owner = col / share;
+                    if (col >= live || owner == slice) continue;
+                    const uint32_t from = slice < owner ? slice : slice - 1;
+                    store_cluster(cluster_address(smem_u32(ring), owner) + ((from * share + col - owner * share) * BM + 32 * quarter + lane) * 4, v[c]);
+                }
+            }
+        }
+        __syncwarp();
+        cluster_sync();
+        if (warp >= 2 && *(volatile uint32_t *)&ctl.abort_flag == 0) {
+            const uint32_t row = p.tile * BM + 32 * quarter + lane;
+            const float ws = row < T.rows ? T.scales[row] : 0.f;
+            const int *part = reinterpret_cast<const int *>(ring) + 32 * quarter + lane;
+            for (uint32_t c0 = mine & ~15u; c0 < mine_end; c0 += 16) {
+                int v[16];
+                tmem_ld16(acc + c0, v);
+#pragma unroll
+                for (uint32_t c = 0; c < 16; c++) {
+                    const uint32_t col = c0 + c;
+                    if (col < mine || col >= mine_end) continue;
+                    int sum = v[c];
+                    for (uint32_t from = 0; from + 1 < J.slices; from++) sum += part[(from * share + col - mine) * BM];
+                    if (row < T.rows) store_value(J, T, p.m0 + col, row, sum, __ldcg(J.x_scales + p.m0 + col), ws);
+                }
+            }
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(J.tmem_cols) : "memory");
+}
+
+// A matrix of rows of `cols` bytes as swizzled tiles: 16 bytes a thread, zero past the matrix's end.
+__global__ void __launch_bounds__(256) k_tile_i8(const uint8_t *__restrict__ src, uint64_t rows, uint64_t cols, uint32_t k_blocks,
+                                                        uint8_t *__restrict__ dst) {
+    const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; // 1024 chunks a tile, eight a row; four blocks a tile
+    const uint64_t tile = i >> 10, row = (tile / k_blocks) * BM + ((i >> 3) & 127), k = (tile % k_blocks) * BK + (i & 7) * 16;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (row < rows && k < cols) v = *reinterpret_cast<const uint4 *>(src + row * cols + k);
+    const uint32_t r = (uint32_t)(i >> 3) & 127, chunk = (uint32_t)(i & 7) ^ (r & 7);
+    *reinterpret_cast<uint4 *>(dst + (tile << 14) + r * 128 + chunk * 16) = v;
+}
+
+// How a product is cut: tokens of a tile, and the blocks among which an item's K is shared.
+struct Plan {
+    uint32_t bn, token_tiles, slices, per, stages, per_sm;
+};
+Plan plan(uint32_t row_tiles, uint32_t k_blocks, uint32_t m, uint32_t sms) {
+    Plan p{};
+    p.token_tiles = (m + 255) / 256;
+    p.bn = ((m + p.token_tiles - 1) / p.token_tiles + 15) / 16 * 16;
+    p.token_tiles = (m + p.bn - 1) / p.bn;
+    p.per_sm = p.bn <= 64 ? 2 : 1;
+    const uint32_t items = row_tiles * p.token_tiles, slots = sms * p.per_sm;
+    p.slices = std::max(1u, std::min({slots / items, MAX_SLICES, k_blocks}));
+    p.per = (k_blocks + p.slices - 1) / p.slices;
+    p.slices = (k_blocks + p.per - 1) / p.per; // no slice is left without work
+    p.stages = std::min((SMEM_MAX / p.per_sm - 3072) / (TILE_BYTES + p.bn * BK), MAX_STAGES);
+    return p;
+}
+
+// Once per handle's device: the kernels may use all of an SM's shared memory.
+cudaError_t allow_shared_memory() {
+    cudaError_t e = cudaFuncSetAttribute(k_gemm_i8<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(SMEM_MAX - 2048));
+    return e != cudaSuccess ? e : cudaFuncSetAttribute(k_gemm_i8<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(SMEM_MAX - 2048));
+}
+
+int launch(fq_device *dev, const fq_matrix *const *w, uint32_t count, const int8_t *x, const float *x_scales, uint32_t m, void *const *y, int y_dtype) {
+    const uint32_t cols = (uint32_t)w[0]->cols, k_blocks = (cols + BK - 1) / BK;
+    Job J{};
+    uint32_t tiles = 0;
+    for (uint32_t i = 0; i < count; i++) {
+        tiles += (uint32_t)((w[i]->rows + BM - 1) / BM);
+        J.t[i] = {w[i]->data, w[i]->scales, y[i], (uint32_t)w[i]->rows, tiles};
+    }
+    const Plan p = plan(tiles, k_blocks, m, (uint32_t)dev->sm_count);
+    J.x_scales = x_scales;
+    J.count = count;
+    J.m = m;
+    J.k_blocks = k_blocks;
+    J.bn = p.bn;
+    J.token_tiles = p.token_tiles;
+    J.items = tiles * p.token_tiles;
+    J.slices = p.slices;
+    J.per = p.per;
+    J.stages = p.stages;
+    J.bf16 = y_dtype == FQ_BF16;
+    for (J.tmem_cols = 32; J.tmem_cols < 2 * p.bn;) J.tmem_cols *= 2;
+    EncodeTiled encode = encode_fn();
+    if (!encode) return fq_fail(dev, FQ_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
+    CUtensorMap map;
+    const uint32_t box_rows = std::min(m, p.bn);
+    const cuuint64_t dims[2] = {cols, m}, strides[1] = {cols};
+    const cuuint32_t box[2] = {BK, box_rows}, step[2] = {1, 1};
+    const CUresult r = encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t *>(x), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fq_fail(dev, FQ_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    J.box_bytes = box_rows * BK;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(p.slices > 1 ? J.items * p.slices : std::min(J.items, (uint32_t)dev->sm_count * p.per_sm));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = 1024 + p.stages * (TILE_BYTES + p.bn * BK);
+    cfg.stream = dev->stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = p.slices;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = p.slices > 1 ? 2 : 1;
+    const cudaError_t e = p.slices > 1 ? cudaLaunchKernelEx(&cfg, k_gemm_i8<true>, map, J, dev->status_dev) : cudaLaunchKernelEx(&cfg, k_gemm_i8<false>, map, J, dev->status_dev);
+    return fq_check_cuda(dev, e, "8-bit projection launch");
 }
 
 } // namespace
@@ -64,10 +382,12 @@ extern "C" int fq_matrix_create_i8(fq_device *dev, uint64_t rows, uint64_t cols,
     if (cols > FQ_MAX_COLS || rows > 0x7fffffffull / 128) return fq_fail(dev, FQ_ERR_SHAPE, "matrix geometry is out of range");
     if (dev->capturing) return fq_fail(dev, FQ_ERR_PARAM, "a matrix cannot be created inside a graph capture");
     if (int rc = fq_check_cuda(dev, cudaSetDevice(dev->ordinal), "cudaSetDevice")) return rc;
-    for (const void *p : {(const void *)values, (const void *)scales}) {
+    bool on_device = false;
+    for (const void *p : {(const void *)scales, (const void *)values}) {
         cudaPointerAttributes attr{};
         if (int rc = fq_check_cuda(dev, cudaPointerGetAttributes(&attr, p), "payload")) return rc;
         if (attr.type == cudaMemoryTypeDevice && attr.device != dev->ordinal) return fq_fail(dev, FQ_ERR_DEVICE, "the payload is on device %d", attr.device);
+        on_device = attr.type == cudaMemoryTypeDevice;
     }
     std::vector<float> host(rows);
     cudaError_t e = cudaMemcpyAsync(host.data(), scales, rows * 4, cudaMemcpyDefault, dev->stream);
@@ -83,12 +403,27 @@ extern "C" int fq_matrix_create_i8(fq_device *dev, uint64_t rows, uint64_t cols,
     w->row_bytes = w->pitch = cols;
     w->byte_size = rows * (cols + 4);
     w->block_elems = w->block_bytes = 1;
-    const size_t len = rows * cols;
-    e = cudaMalloc((void **)&w->data, len + rows * 4);
+    const uint32_t k_blocks = (uint32_t)((cols + BK - 1) / BK);
+    const uint64_t tiles = (rows + BM - 1) / BM * k_blocks;
+    const size_t len = tiles * TILE_BYTES;
+    // The tiles are laid out on the device; rows in host memory (or off their 16 bytes) go through a copy of their own.
+    uint8_t *staged = nullptr;
+    const uint8_t *src = (const uint8_t *)values;
+    e = allow_shared_memory();
+    if (e == cudaSuccess) e = cudaMalloc((void **)&w->data, len + rows * 4);
     w->scales = (float *)(w->data + len);
-    if (e == cudaSuccess) e = cudaMemcpyAsync(w->data, values, len, cudaMemcpyDefault, dev->stream);
+    if (e == cudaSuccess && (!on_device || ((uintptr_t)values & 15))) {
+        e = cudaMalloc((void **)&staged, rows * cols);
+        if (e == cudaSuccess) e = cudaMemcpyAsync(staged, values, rows * cols, cudaMemcpyDefault, dev->stream);
+        src = staged;
+    }
+    if (e == cudaSuccess) {
+        k_tile_i8<<<(unsigned)(tiles * 4), 256, 0, dev->stream>>>(src, rows, cols, k_blocks, w->data);
+        e = cudaGetLastError();
+    }
     if (e == cudaSuccess) e = cudaMemcpyAsync(w->scales, host.data(), rows * 4, cudaMemcpyHostToDevice, dev->stream);
     if (e == cudaSuccess) e = cudaStreamSynchronize(dev->stream);
+    if (staged) cudaFree(staged);
     if (e != cudaSuccess) {
         if (w->data) cudaFree(w->data);
         delete w;
@@ -102,7 +437,7 @@ extern "C" int fq_matrix_create_i8(fq_device *dev, uint64_t rows, uint64_t cols,
 extern "C" int fq_project_many_i8(fq_device *dev, const fq_matrix *const *w, size_t count, const int8_t *x, size_t x_elems, const float *x_scales,
                                   size_t m, void *const *y, int y_dtype) {
     if (int rc = fq_begin_enqueue(dev)) return rc;
-    constexpr size_t MAX = 8;
+    constexpr size_t MAX = MAX_MANY;
     if (!w || !y || count == 0) return fq_fail(dev, FQ_ERR_PARAM, "projection list");
     if (count > MAX) return fq_fail(dev, FQ_ERR_PARAM, "at most %zu projections share an input", MAX);
     if (y_dtype != FQ_F32 && y_dtype != FQ_BF16) return fq_fail(dev, FQ_ERR_UNSUPPORTED, "element type %d", y_dtype);
@@ -122,8 +457,8 @@ extern "C" int fq_project_many_i8(fq_device *dev, const fq_matrix *const *w, siz
         for (size_t j = 0; j < i; j++)
             if (int rc = fq_check_no_alias(dev, y[i], yb, y[j], m * w[j]->rows * fq_dtype_size(y_dtype), "y")) return rc;
     }
-    for (size_t i = 0; i < count; i++) launch_one(dev, w[i], x, x_scales, (uint32_t)m, y[i], y_dtype);
-    return fq_end_enqueue(dev, "project_i8", (int)count);
+    if (int rc = launch(dev, w, (uint32_t)count, x, x_scales, (uint32_t)m, y, y_dtype)) return rc;
+    return fq_end_enqueue(dev, "project_i8", 1);
 }
 
 extern "C" int fq_project_i8(fq_device *dev, const fq_matrix *w, const int8_t *x, size_t x_elems, const float *x_scales, size_t m, void *y,
