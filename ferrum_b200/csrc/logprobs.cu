@@ -6,10 +6,14 @@
 // A logit of -infinity is a token of probability 0 and adds nothing anywhere.  A row with a NaN, with +infinity or with nothing
 // above -infinity has no distribution: its numbers are NaN.
 //
-// A row is read once, by a block or by a cluster of up to eight (each a contiguous part; block 0 collects through distributed
-// shared memory).  Per thread: S = sum exp(l - p) and T = sum exp(l - p)(l - p) with a pivot p, the largest logit of what the
-// block reads first, moved only when a logit is more than 20 above it (S grows to e^20 per term at most, far from fp32's end;
-// a running maximum would rescale every few values).  log S and T / S at the end give z = p + log S and the entropy log S - T / S.
+// A row is read once, by a block or by a cluster of blocks (each a contiguous part; block 0 collects through distributed shared
+// memory).  In powers of two, with b = log2(e) as fp32 has it and a pivot c:
+//
+//   S = sum 2^(b l - c)     T = sum 2^(b l - c) (b l - c)     z = (c + log2 S) / b     entropy = ln 2 (log2 S - T / S)
+//
+// b l - c is one FMA with one rounding; c is the largest b l of what the block reads first and moves only when a logit is more
+// than 20 / b above it (a term is 2^20 at most, far from fp32's end; a running maximum would rescale every few values).  Dividing by b as
+// it is keeps its own rounding out of z.
 //
 // The most likely tokens: every warp keeps its best 32 as a sorted list, one (value, index) key per lane, and puts a value in
 // only if it can still matter: above a bound that k values of the block are known to reach.  The bound starts with what is read
@@ -26,6 +30,12 @@ using namespace fqk;
 
 constexpr uint32_t MAX_TOP = 32, MAX_CLUSTER = 8;
 constexpr int UNROLL = 4; // 16-byte loads of a thread in flight
+constexpr float LOG2E = 1.44269502f; // b: log2(e) rounded to fp32
+constexpr float SLACK = 20.f;        // how far b l may be above the pivot
+// Beyond a million the rounding of c is no longer small: a row whose largest logit lies there is summed in 64 bits (sum_64).
+constexpr float MOST = 1048576.f;
+// Lower logits, -infinity among them, count as this: a power of two, so that b LEAST is exact, and a bf16 number.
+constexpr float LEAST = -0x1p126f;
 
 // Numbers in their order as unsigned integers: NaN below everything, the two zeros equal.
 __device__ __forceinline__ uint32_t order_of(float v) {
@@ -40,52 +50,85 @@ __device__ __forceinline__ float just_below(uint32_t least) {
 }
 __device__ __forceinline__ uint64_t key_of(uint32_t order, uint32_t i) { return (uint64_t)order << 32 | (uint32_t)~i; }
 
+__device__ __forceinline__ float exp2_fast(float d) { // within 2^-22 of itself; 0 below 2^-126
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+    return r;
+}
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
-__device__ __forceinline__ float exp_fast(float d) { // 2^-22 of itself; 0 below 2^-126
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d * 1.44269504f));
+__device__ __forceinline__ uint32_t max_nan_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
+__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ float low_half(uint32_t u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float high_half(uint32_t u) { return __uint_as_float(u & 0xFFFF0000u); }
+
+// Pairs of fp32 in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
 
 template <typename T> constexpr int PER_LOAD = 16 / (int)sizeof(T);
-__device__ __forceinline__ void unpack(const uint4 &u, float (&v)[4]) {
-    v[0] = __uint_as_float(u.x), v[1] = __uint_as_float(u.y), v[2] = __uint_as_float(u.z), v[3] = __uint_as_float(u.w);
-}
-__device__ __forceinline__ void unpack(const uint4 &u, float (&v)[8]) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        v[2 * i] = __uint_as_float(w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+__device__ __forceinline__ uint32_t word(const uint4 &u, int i) { return i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w; }
+// The largest of a 16-byte piece; NaN if one is.
+template <typename T> __device__ __forceinline__ float piece_max(const uint4 &u) {
+    if constexpr (sizeof(T) == 2) {
+        const uint32_t m = max_nan_bf16x2(max_nan_bf16x2(u.x, u.y), max_nan_bf16x2(u.z, u.w));
+        return max_nan(low_half(m), high_half(m));
+    } else {
+        return max_nan(max_nan(__uint_as_float(u.x), __uint_as_float(u.y)), max_nan(__uint_as_float(u.z), __uint_as_float(u.w)));
     }
+}
+// Values 2 i and 2 i + 1 of a piece.
+template <typename T> __device__ __forceinline__ float2 pair_of(const uint4 &u, int i) {
+    if constexpr (sizeof(T) == 2) return make_float2(low_half(word(u, i)), high_half(word(u, i)));
+    else return make_float2(__uint_as_float(word(u, 2 * i)), __uint_as_float(word(u, 2 * i + 1)));
+}
+// The same, not below LEAST (and without NaN).
+template <typename T> __device__ __forceinline__ float2 pair_from_least(const uint4 &u, int i) {
+    if constexpr (sizeof(T) == 2) {
+        const uint32_t w = max_bf16x2(word(u, i), 0xFE80FE80u); // LEAST
+        return make_float2(low_half(w), high_half(w));
+    } else {
+        return make_float2(fmaxf(__uint_as_float(word(u, 2 * i)), LEAST), fmaxf(__uint_as_float(word(u, 2 * i + 1)), LEAST));
+    }
+}
+template <typename T> __device__ __forceinline__ float load1(const T *l, uint32_t i) {
+    if constexpr (sizeof(T) == 2) return low_half(__ldcg(reinterpret_cast<const unsigned short *>(l) + i));
+    else return __ldcg(l + i);
 }
 
 struct Sums {
-    float p, s, t; // pivot, sum exp(l - p), sum exp(l - p)(l - p)
+    float c, s, t; // pivot, sum 2^(b l - c), sum 2^(b l - c) (b l - c)
 };
+constexpr float NO_PIVOT = LEAST * LOG2E;
 // The sums about another pivot.
-__device__ __forceinline__ void move_pivot(Sums &a, float p) {
-    const float f = exp_fast(a.p - p);
-    // f = 0: nothing is left of them (and a.p - p may be -infinity)
-    a.t = f > 0.f ? f * fmaf(a.p - p, a.s, a.t) : 0.f;
-    a.s = f * a.s;
-    a.p = p;
+__device__ __forceinline__ void move_pivot(Sums &a, float c) {
+    const float f = exp2_fast(a.c - c);
+    a.t = f > 0.f ? f * fmaf(a.c - c, a.s, a.t) : 0.f; // f = 0: nothing is left of them, whatever they were
+    a.s = f > 0.f ? f * a.s : 0.f;
+    a.c = c;
 }
 __device__ __forceinline__ void join(Sums &a, Sums b) {
-    const float p = fmaxf(a.p, b.p);
-    if (a.p != p) move_pivot(a, p);
-    if (b.p != p) move_pivot(b, p);
+    const float c = fmaxf(a.c, b.c);
+    if (a.c != c) move_pivot(a, c);
+    if (b.c != c) move_pivot(b, c);
     a.s += b.s;
     a.t += b.t;
 }
 __device__ __forceinline__ Sums join_warp(Sums a) {
-#pragma unroll
+#pragma unroll 1
     for (int off = 16; off > 0; off >>= 1) {
-        const Sums b{__shfl_xor_sync(0xffffffffu, a.p, off), __shfl_xor_sync(0xffffffffu, a.s, off), __shfl_xor_sync(0xffffffffu, a.t, off)};
+        const Sums b{__shfl_xor_sync(0xffffffffu, a.c, off), __shfl_xor_sync(0xffffffffu, a.s, off), __shfl_xor_sync(0xffffffffu, a.t, off)};
         join(a, b);
     }
     return a;
@@ -94,12 +137,27 @@ __device__ __forceinline__ Sums join_warp(Sums a) {
 __device__ __forceinline__ uint64_t merge_lists(uint64_t a, const uint64_t *b, uint32_t lane) {
     const uint64_t o = b[31 - lane];
     uint64_t c = a > o ? a : o;
-#pragma unroll
+#pragma unroll 1
     for (int off = 16; off > 0; off >>= 1) {
         const uint64_t other = __shfl_xor_sync(0xffffffffu, c, off);
         if ((other > c) == ((lane & off) == 0)) c = other;
     }
     return c;
+}
+
+// A row of logits around numbers beyond MOST: by one warp, in 64 bits about its largest.
+template <typename T> __device__ __noinline__ void sum_64(const T *l, uint32_t n, uint32_t lane, double &z, double &entropy) {
+    double mx = -INFINITY, s = 0.0, t = 0.0;
+    for (uint32_t i = lane; i < n; i += 32) mx = fmax(mx, (double)load1(l, i));
+    for (int off = 16; off > 0; off >>= 1) mx = fmax(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+    for (uint32_t i = lane; i < n; i += 32) {
+        const double d = fmax((double)load1(l, i) - mx, -1000.0), e = exp(d);
+        s += e;
+        t = fma(d, e, t);
+    }
+    for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off), t += __shfl_xor_sync(0xffffffffu, t, off);
+    z = mx + log(s);
+    entropy = log(s) - t / s;
 }
 
 struct Outputs {
@@ -114,6 +172,7 @@ __device__ __forceinline__ uint32_t cluster_address(const void *p, uint32_t rank
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
     return r;
 }
+__device__ __forceinline__ void store_cluster(uint32_t to, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to), "r"(v) : "memory"); }
 
 // Block `rank` of the `parts` of row blockIdx.x / parts.
 template <typename T, int NT, bool TOP>
@@ -141,171 +200,175 @@ k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids
     const uint32_t pieces = (uint32_t)(((uint64_t)skip + n + V - 1) / V), per = (pieces + parts - 1) / parts;
     const uint32_t begin = min(rank * per, pieces), end = min(begin + per, pieces);
     const uint32_t id = ids ? __ldcg(ids + row) : n;
-    const float none = -INFINITY;
-    auto load = [&](uint32_t j, uint4 &u) {
+    auto load = [&](uint32_t j) {
         const uint32_t first = j * V - skip; // wraps in the piece that begins before the row
-        if (first <= n && n - first >= (uint32_t)V) {
-            u = __ldcg(reinterpret_cast<const uint4 *>(aligned) + j);
-        } else { // the row's ends: elements one at a time, -infinity outside
-            T e[V];
+        if (first <= n && n - first >= (uint32_t)V) return __ldcg(reinterpret_cast<const uint4 *>(aligned) + j);
+        uint32_t w[4]; // the row's ends: elements one at a time, -infinity outside
 #pragma unroll
-            for (int i = 0; i < V; i++) {
+        for (int i = 0; i < 4; i++) {
+            if constexpr (sizeof(T) == 2) {
+                const uint32_t a = first + 2 * i, b = a + 1;
+                const uint32_t lo = a < n ? __ldcg(reinterpret_cast<const unsigned short *>(l) + a) : 0xFF80u, hi = b < n ? __ldcg(reinterpret_cast<const unsigned short *>(l) + b) : 0xFF80u;
+                w[i] = lo | hi << 16;
+            } else {
                 const uint32_t at = first + i;
-                if constexpr (sizeof(T) == 2) e[i] = __ushort_as_bfloat16(at < n ? __ldcg(reinterpret_cast<const unsigned short *>(l) + at) : 0xFF80u);
-                else e[i] = at < n ? __ldcg(l + at) : none;
+                w[i] = at < n ? __float_as_uint(__ldcg(l + at)) : 0xFF800000u;
             }
-            u = *reinterpret_cast<const uint4 *>(e);
         }
+        return make_uint4(w[0], w[1], w[2], w[3]);
     };
     uint4 next[UNROLL];
     auto fetch = [&](uint32_t j0) {
 #pragma unroll
-        for (int u = 0; u < UNROLL; u++)
-            if (j0 + u * NT < end) load(j0 + u * NT, next[u]);
+        for (int u = 0; u < UNROLL; u++) {
+            const uint32_t j = j0 + u * NT;
+            next[u] = make_uint4(0xFF800000u, 0xFF800000u, 0xFF800000u, 0xFF800000u); // nothing: -infinity, or in bf16 -infinity and 0
+            if constexpr (sizeof(T) == 2) next[u] = make_uint4(0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u);
+            if (j < end) next[u] = load(j);
+        }
     };
     fetch(begin + tid);
-    const float given = id < n ? (sizeof(T) == 2 ? __uint_as_float((uint32_t)__ldcg(reinterpret_cast<const unsigned short *>(l) + id) << 16)
-                                                 : __ldcg(reinterpret_cast<const float *>(l) + id))
-                               : __int_as_float(0x7fc00000);
+    const float given = id < n ? load1(l, id) : __int_as_float(0x7fc00000);
 
     // What is read first gives the pivot and a bound that k values of the block reach.
     uint32_t best = 0;
 #pragma unroll
     for (int u = 0; u < UNROLL; u++)
-        if (begin + tid + u * NT < end) {
-            float v[V];
-            unpack(next[u], v);
-#pragma unroll
-            for (int i = 0; i < V; i++) best = max(best, order_of(v[i]));
-        }
+        if (begin + tid + u * NT < end) best = max(best, order_of(piece_max<T>(next[u]))); // (a piece with a NaN does not count)
     const uint32_t warps = min((uint32_t)W, (end - begin + 31) / 32); // with something to read
     uint32_t high = __reduce_max_sync(0xffffffffu, best);
     if (lane == 0) first_max[warp] = high;
     if constexpr (TOP) {
         const uint32_t m = warps ? (k + warps - 1) / warps : 1; // this warp's m-th largest maximum
-        uint32_t mine = best;
+#pragma unroll 1
         for (uint32_t i = 1; i < m; i++) {
-            const uint32_t holders = __ballot_sync(0xffffffffu, mine == high && mine != 0);
-            if (holders && lane == (uint32_t)__ffs(holders) - 1) mine = 0;
-            high = __reduce_max_sync(0xffffffffu, mine);
+            const uint32_t holders = __ballot_sync(0xffffffffu, best == high && best != 0);
+            if (holders && lane == (uint32_t)__ffs(holders) - 1) best = 0;
+            high = __reduce_max_sync(0xffffffffu, best);
         }
         if (lane == 0) first_bound[warp] = high;
     }
     __syncthreads();
-    Sums a{0.f, 0.f, 0.f};
+    const float top = value_of(max(__reduce_max_sync(0xffffffffu, first_max[lane % W]), 1u << 23)); // -infinity where there is nothing (or NaN)
+    Sums a{fmaxf(top, LEAST) * LOG2E, 0.f, 0.f};
+    float limit = fminf(fmaf(SLACK, 1.f / LOG2E, fmaxf(top, LEAST)), MOST); // logits above it move the pivot
     uint32_t least = 0; // values of a lower order do not matter any more; 0: all do
-    {
-        const uint32_t top = __reduce_max_sync(0xffffffffu, first_max[lane < W ? lane : 0]);
-        a.p = top > order_of(-INFINITY) ? value_of(top) : -3.402823466e38f;
-        if constexpr (TOP) least = __reduce_min_sync(0xffffffffu, lane < warps ? first_bound[lane] : 0xFFFFFFFFu);
-    }
-    bool bad = a.p == INFINITY;
-    float limit = a.p + 20.f, below = just_below(least);
+    if constexpr (TOP) least = __reduce_min_sync(0xffffffffu, lane < warps ? first_bound[lane] : 0xFFFFFFFFu);
+    float below = just_below(least);
+    bool bad = false, beyond = false, some = false; // a NaN or +infinity; a logit above MOST; one above -infinity
     uint32_t count = 0;
     uint64_t list = 0;
+    float2 s2 = make_float2(0.f, 0.f), t2 = make_float2(0.f, 0.f);
 
-    auto take = [&](const uint4 &u, uint32_t j, bool live) {
-        float v[V];
-        unpack(u, v);
-        float mx = v[0];
+#pragma unroll 1
+    for (uint32_t j0 = begin; j0 < end; j0 += UNROLL * NT) {
+        uint4 now[UNROLL];
+        float mx[UNROLL];
 #pragma unroll
-        for (int i = 1; i < V; i++) mx = max_nan(mx, v[i]);
-        if (!live) mx = none;
+        for (int u = 0; u < UNROLL; u++) now[u] = next[u];
+        fetch(j0 + UNROLL * NT + tid);
+#pragma unroll
+        for (int u = 0; u < UNROLL; u++) mx[u] = piece_max<T>(now[u]);
         if constexpr (TOP) {
-            uint32_t vote = __ballot_sync(0xffffffffu, live && !(mx <= below));
-            if (vote) {
-                while (vote) { // values in the order of their indexes
-                    const uint32_t src = __ffs(vote) - 1, at = __shfl_sync(0xffffffffu, j, src) * V - skip;
-                    vote &= vote - 1;
+            uint32_t maybe = 0;
 #pragma unroll
-                    for (int i = 0; i < V; i++) {
-                        const uint32_t order = order_of(__shfl_sync(0xffffffffu, v[i], src));
-                        if (order < least || at + i >= n) continue; // uniform
-                        const uint64_t key = key_of(order, at + i);
-                        const uint32_t pos = __popc(__ballot_sync(0xffffffffu, list > key));
-                        const uint64_t up = __shfl_up_sync(0xffffffffu, list, 1);
-                        if (lane >= pos) list = lane == pos ? key : up;
-                        const uint64_t kth = __shfl_sync(0xffffffffu, list, k - 1);
-                        if (kth) least = max(least, (uint32_t)(kth >> 32) + 1); // later values have higher indexes
+            for (int u = 0; u < UNROLL; u++) maybe |= (uint32_t)!(mx[u] <= below) << u;
+            if (__any_sync(0xffffffffu, maybe)) { // some pieces are looked into, in the order of their indexes
+                least = max(least, *(volatile uint32_t *)&bound);
+#pragma unroll 1
+                for (int u = 0; u < UNROLL; u++) {
+                    uint32_t vote = __ballot_sync(0xffffffffu, (maybe >> u & 1) && j0 + u * NT + tid < end);
+                    while (vote) {
+                        const uint32_t src = __ffs(vote) - 1, j = j0 + u * NT + 32 * warp + src;
+                        vote &= vote - 1;
+                        uint4 piece = u == 0 ? now[0] : u == 1 ? now[1] : u == 2 ? now[2] : now[3];
+                        piece = make_uint4(__shfl_sync(0xffffffffu, piece.x, src), __shfl_sync(0xffffffffu, piece.y, src), __shfl_sync(0xffffffffu, piece.z, src),
+                                           __shfl_sync(0xffffffffu, piece.w, src));
+#pragma unroll 1
+                        for (int i = 0; i < V; i++) {
+                            const uint32_t w = word(piece, sizeof(T) == 2 ? i / 2 : i), at = j * V - skip + i;
+                            const uint32_t order = order_of(sizeof(T) == 4 ? __uint_as_float(w) : (i & 1) ? high_half(w) : low_half(w));
+                            if (order < least || at >= n) continue;
+                            const uint64_t key = key_of(order, at);
+                            const uint32_t pos = __popc(__ballot_sync(0xffffffffu, list > key));
+                            const uint64_t up = __shfl_up_sync(0xffffffffu, list, 1);
+                            if (lane >= pos) list = lane == pos ? key : up;
+                            const uint64_t kth = __shfl_sync(0xffffffffu, list, k - 1);
+                            if (kth) least = max(least, (uint32_t)(kth >> 32) + 1); // later values have higher indexes
+                        }
                     }
                 }
                 if (lane == k - 1 && list) atomicMax(&bound, (uint32_t)(list >> 32));
                 below = just_below(least);
             }
         }
-        if (!live) return;
-        if (!(mx <= given))
+        float highest = mx[0];
 #pragma unroll
-            for (int i = 0; i < V; i++) count += v[i] > given;
-        if (!(mx <= limit)) {
-            float high = none;
+        for (int u = 1; u < UNROLL; u++) highest = max_nan(highest, mx[u]);
+        if (!(highest <= given))
 #pragma unroll
-            for (int i = 0; i < V; i++) {
-                bad |= v[i] != v[i];
-                high = fmaxf(high, v[i]);
-            }
-            bad |= high == INFINITY;
-            if (high > limit && !bad) {
-                move_pivot(a, high);
-                limit = high + 20.f;
-            }
-        }
+            for (int u = 0; u < UNROLL; u++)
 #pragma unroll
-        for (int i = 0; i < V; i++) {
-            const float d = fmaxf(v[i] - a.p, -200.f); // e^-200 is 0, and so is what -infinity adds to T
-            const float e = exp_fast(d);
-            a.s += e;
-            a.t = fmaf(d, e, a.t);
-        }
-    };
-    for (uint32_t j0 = begin; j0 < end; j0 += UNROLL * NT) {
-        uint4 now[UNROLL];
-#pragma unroll
-        for (int u = 0; u < UNROLL; u++) now[u] = next[u];
-        fetch(j0 + UNROLL * NT + tid);
-        if constexpr (TOP) {
-            const uint32_t shared = *(volatile uint32_t *)&bound;
-            if (shared > least) {
-                least = shared;
-                below = just_below(least);
+                for (int i = 0; i < V / 2; i++) {
+                    const float2 v = pair_of<T>(now[u], i);
+                    count += v.x > given;
+                    count += v.y > given;
+                }
+        some |= highest > -INFINITY;
+        if (!(highest <= limit)) {
+            bad |= !(highest < INFINITY);
+            beyond |= highest > MOST;
+            if (!bad && !beyond) {
+                a.s = s2.x + s2.y;
+                a.t = t2.x + t2.y;
+                move_pivot(a, highest * LOG2E);
+                limit = fminf(fmaf(SLACK, 1.f / LOG2E, highest), MOST);
+                s2 = make_float2(a.s, 0.f);
+                t2 = make_float2(a.t, 0.f);
             }
         }
+        const float2 b2 = make_float2(LOG2E, LOG2E), c2 = make_float2(-a.c, -a.c);
 #pragma unroll
-        for (int u = 0; u < UNROLL; u++) take(now[u], j0 + tid + u * NT, j0 + tid + u * NT < end);
+        for (int u = 0; u < UNROLL; u++)
+#pragma unroll
+            for (int i = 0; i < V / 2; i++) {
+                const float2 d = fma2(pair_from_least<T>(now[u], i), b2, c2);
+                const float2 e = make_float2(exp2_fast(d.x), exp2_fast(d.y));
+                s2 = add2(s2, e);
+                t2 = fma2(d, e, t2);
+            }
     }
+    a.s = s2.x + s2.y;
+    a.t = t2.x + t2.y;
 
     // The block's sums and list, then the cluster's.
     a = join_warp(a);
     count = __reduce_add_sync(0xffffffffu, count);
-    bad = __any_sync(0xffffffffu, bad);
+    const uint32_t flags = (__any_sync(0xffffffffu, bad) ? 1 : 0) | (__any_sync(0xffffffffu, beyond) ? 2 : 0) | (__any_sync(0xffffffffu, some) ? 4 : 0);
     if (lane == 0) {
         sums[warp] = a;
         counts[warp] = count;
-        bads[warp] = bad;
+        bads[warp] = flags;
     }
     if constexpr (TOP) {
         lists[warp][lane] = list;
-#pragma unroll
+#pragma unroll 1
         for (int half = W / 2; half > 0; half >>= 1) {
             __syncthreads();
             if (warp < (uint32_t)half) lists[warp][lane] = list = merge_lists(list, lists[warp + half], lane);
         }
     }
     __syncthreads();
+    uint32_t all = 0;
     if (parts > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
     if (warp == 0) {
-        a = join_warp(lane < W ? sums[lane] : Sums{-3.402823466e38f, 0.f, 0.f});
+        a = join_warp(lane < W ? sums[lane] : Sums{NO_PIVOT, 0.f, 0.f});
         count = __reduce_add_sync(0xffffffffu, lane < W ? counts[lane] : 0u);
-        bad = __any_sync(0xffffffffu, lane < W && bads[lane]);
+        all = __reduce_or_sync(0xffffffffu, lane < W ? bads[lane] : 0u);
         if (parts > 1) {
-            if (lane == 0) {
-                const uint32_t to = cluster_address(&all_sums[rank], 0);
-                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(a.p) : "memory");
-                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4), "f"(a.s) : "memory");
-                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 8), "f"(a.t) : "memory");
-                asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_address(&all_counts[rank], 0)), "r"(count) : "memory");
-                asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_address(&all_bads[rank], 0)), "r"((uint32_t)bad) : "memory");
-            }
+            if (lane < 3) store_cluster(cluster_address(&all_sums[rank], 0) + 4 * lane, __float_as_uint(lane == 0 ? a.c : lane == 1 ? a.s : a.t));
+            if (lane == 3) store_cluster(cluster_address(&all_counts[rank], 0), count);
+            if (lane == 4) store_cluster(cluster_address(&all_bads[rank], 0), all);
             if constexpr (TOP) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(cluster_address(&all_lists[rank][lane], 0)), "l"(list) : "memory");
         }
     }
@@ -313,25 +376,31 @@ k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids
         __syncwarp();
         asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
         if (rank != 0 || warp != 0) return;
-        a = join_warp(lane < parts ? all_sums[lane] : Sums{-3.402823466e38f, 0.f, 0.f});
+        a = join_warp(lane < parts ? all_sums[lane] : Sums{NO_PIVOT, 0.f, 0.f});
         count = __reduce_add_sync(0xffffffffu, lane < parts ? all_counts[lane] : 0u);
-        bad = __any_sync(0xffffffffu, lane < parts && all_bads[lane]);
+        all = __reduce_or_sync(0xffffffffu, lane < parts ? all_bads[lane] : 0u);
         if constexpr (TOP)
+#pragma unroll 1
             for (uint32_t i = 1; i < parts; i++) list = merge_lists(list, all_lists[i], lane);
     }
     if (warp != 0) return;
-    bad |= !(a.s > 0.f); // nothing above -infinity
-    const double log_s = bad ? NAN : log((double)a.s);
-    const double p = a.p;
+    double z, entropy;
+    if ((all & 1) || !(all & 4)) z = entropy = NAN;
+    else if ((all & 2) || a.c < -MOST * LOG2E) sum_64(l, n, lane, z, entropy); // (the pivot is the row's largest or near it)
+    else {
+        const double log2_s = log2((double)a.s);
+        z = ((double)a.c + log2_s) / (double)LOG2E;
+        entropy = 0.69314718055994531 * (log2_s - (double)a.t / (double)a.s);
+    }
     if (lane == 0) {
-        if (out.logprobs) out.logprobs[row] = (float)((double)given - p - log_s);
+        if (out.logprobs) out.logprobs[row] = (float)((double)given - z);
         if (out.ranks) out.ranks[row] = id < n ? 1 + count : 0;
-        if (out.entropy) out.entropy[row] = (float)(log_s - (double)a.t / (double)a.s);
+        if (out.entropy) out.entropy[row] = (float)entropy;
     }
     if constexpr (TOP)
         if (lane < k) {
             out.top_ids[(size_t)row * k + lane] = ~(uint32_t)list;
-            out.top_logprobs[(size_t)row * k + lane] = (float)((double)value_of((uint32_t)(list >> 32)) - p - log_s);
+            out.top_logprobs[(size_t)row * k + lane] = (float)((double)value_of((uint32_t)(list >> 32)) - z);
         }
 }
 
@@ -365,7 +434,7 @@ extern "C" int fq_token_logprobs(fq_device *dev, const void *logits, int dtype, 
                                  uint32_t k, float *logprobs, uint32_t *ranks, float *entropy, float *top_logprobs, uint32_t *top_ids) {
     if (int rc = fq_begin_enqueue(dev)) return rc;
     if (dtype != FQ_F32 && dtype != FQ_BF16) return fq_fail(dev, FQ_ERR_UNSUPPORTED, "element type %d", dtype);
-    if (n == 0 || rows == 0 || rows > 0x7fffffffu || stride < n) return fq_fail(dev, FQ_ERR_SHAPE, "%u rows of %u logits, %zu apart", rows, n, stride);
+    if (n == 0 || n > 0x7fffffffu || rows == 0 || rows > 0x7fffffffu / MAX_CLUSTER || stride < n) return fq_fail(dev, FQ_ERR_SHAPE, "%u rows of %u logits, %zu apart", rows, n, stride);
     if (k > MAX_TOP || k > n) return fq_fail(dev, FQ_ERR_PARAM, "%u alternatives of %u tokens (at most %u)", k, n, MAX_TOP);
     const size_t bytes = ((size_t)(rows - 1) * stride + n) * fq_dtype_size(dtype);
     if (int rc = fq_check_binding(dev, logits, bytes, "logits", (uint32_t)fq_dtype_size(dtype))) return rc;

@@ -8,10 +8,12 @@
 // to the nearest whole number, ties to even, of the exact quotient: the 8-bit values do not depend on how a row is spread
 // over threads.
 //
-// A row is read once and stays in registers.  v is computed in 32 bits; the few values that decide are taken again in 64: those
-// that may be the row's largest, and those whose quotient lies within the error of 32 bits of the border between two whole
-// numbers (one in twelve thousand; of a gated unit one in five thousand).  The sum of squares is held in 64 bits: it costs a
-// conversion and an FMA a value, where memory leaves time for some fifty instructions.
+// A row is read from memory once and kept in shared memory, every thread its own values of it.  v is computed in 32 bits; the
+// few values that decide are taken again in 64: those that may be the row's largest, and those whose quotient lies within
+// the error of 32 bits of the border between two whole numbers.  Squares are added by fours in 32 bits and from there in 64.
+// (Held in registers, unrolled over a row, the same took 105 registers and 63 instructions a value, a third of the time
+// waiting for instructions: 2048 x 5120 bf16 45 us.)
+#include <atomic>
 #include <type_traits>
 
 #include "gemv_common.cuh"
@@ -28,241 +30,260 @@ __device__ __forceinline__ float4 load4(const __nv_bfloat16 *p) {
     const uint2 b = __ldcg(reinterpret_cast<const uint2 *>(p));
     return make_float4(__uint_as_float(b.x << 16), __uint_as_float(b.x & 0xFFFF0000u), __uint_as_float(b.y << 16), __uint_as_float(b.y & 0xFFFF0000u));
 }
-// a + b as it is kept.
-__device__ __forceinline__ float4 sum4(const float *, const float4 &a, const float4 &b) { return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); }
-__device__ __forceinline__ float4 sum4(const __nv_bfloat16 *, const float4 &a, const float4 &b) {
-    const float4 s = sum4((const float *)nullptr, a, b);
-    auto keep = [](float v) { return __bfloat162float(__float2bfloat16_rn(v)); };
-    return make_float4(keep(s.x), keep(s.y), keep(s.z), keep(s.w));
-}
-__device__ __forceinline__ void store4(float *p, const float4 &v) { *reinterpret_cast<float4 *>(p) = v; }
-__device__ __forceinline__ void store4(__nv_bfloat16 *p, const float4 &v) { // values that are bf16 already
-    *reinterpret_cast<uint2 *>(p) = make_uint2(__byte_perm(__float_as_uint(v.x), __float_as_uint(v.y), 0x7632), __byte_perm(__float_as_uint(v.z), __float_as_uint(v.w), 0x7632));
-}
 __device__ __forceinline__ float load1(const float *p) { return __ldcg(p); }
-__device__ __forceinline__ float load1(const __nv_bfloat16 *p) { return __bfloat162float(__ushort_as_bfloat16(__ldcg(reinterpret_cast<const unsigned short *>(p)))); }
-__device__ __forceinline__ float part(const float4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+__device__ __forceinline__ float load1(const __nv_bfloat16 *p) { return __uint_as_float((uint32_t)__ldcg(reinterpret_cast<const unsigned short *>(p)) << 16); }
+// a + b, stored as its type keeps it, and as it is kept.
+__device__ __forceinline__ float4 add4(float *p, const float4 &a, const float4 &b) {
+    const float4 s = make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
+    *reinterpret_cast<float4 *>(p) = s;
+    return s;
+}
+__device__ __forceinline__ float4 add4(__nv_bfloat16 *p, const float4 &a, const float4 &b) {
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(a.x + b.x, a.y + b.y), hi = __floats2bfloat162_rn(a.z + b.z, a.w + b.w);
+    const uint2 u = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+    *reinterpret_cast<uint2 *>(p) = u;
+    return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xFFFF0000u));
+}
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; } // ordered as |v|, NaN above infinity
+__device__ __forceinline__ uint32_t magnitude(const float4 &v) { return max(max(magnitude(v.x), magnitude(v.y)), max(magnitude(v.z), magnitude(v.w))); }
 
-// silu(g) u: within 4.5 * 2^-23 of itself (2 steps of the exponential, and four roundings) while e^-g does not overflow, and
-// within 2^-100 of |u| beyond.
-__device__ __forceinline__ float gated(float g, float u) { return g / (1.f + expf(-g)) * u; }
+// silu(g) u.  Relative error: 2 steps (2^-22) of the exponential and as much of the quotient, two roundings: 10 * 2^-24; beyond
+// g = -87, where e^-g leaves the range of the quotient, 0 instead of less than 2^-118 |u|.
+__device__ __forceinline__ float gated(float g, float u) { return __fdividef(g, 1.f + expf(-g)) * u; }
 __device__ __forceinline__ double gated64(double g, double u) { return g / (1.0 + exp(-g)) * u; }
 
-// Where a row leaves these, 64 bits are used throughout: the smallest and largest |v| of a row's maximum, so that what 32 bits
-// lose to underflow is nothing beside it, and for the gated unit the largest |u|, for what `gated` loses of a closed gate.
-constexpr float LEAST = 1e-20f, MOST = 1e37f, MOST_UP = 1048576.f;
-// How far 127 v / a in 32 bits may be from the exact quotient: 127 times 1.5 * 2^-23 of v, 127 / a and their product, and
-// for the gated unit 4 * 2^-23 more.
-template <int OP> constexpr float NEAR = OP == GLU ? 1e-4f : 4e-5f;
-// How many steps of fp32 the exact largest value may be below the largest fp32 one: products are rounded once, which keeps
-// their order; a gated unit is off by 9 half steps, and so is the largest.
-template <int OP> constexpr uint32_t BELOW = OP == GLU ? 12 : 0;
+// The part of a quotient t = 127 v / a that its computation in 32 bits may be off: v as above or (norms) once rounded, a and
+// 127 / a rounded.
+template <int OP> constexpr float OFF = OP == GLU ? 14 * 0x1p-24f : 4 * 0x1p-24f;
+// How many steps of fp32 the exact largest value may lie below the largest fp32 one: single roundings keep their order; a
+// gated unit is off by at most 10 steps, and so is the largest.
+template <int OP> constexpr uint32_t BELOW = OP == GLU ? 24 : 0;
+// Rows that leave these go through 64 bits throughout: the largest |v|, so that what 32 bits lose to underflow is nothing
+// beside it; and of the norms the largest sum of four squares, of the gated unit the largest |u|, for the same reason.
+constexpr float LEAST = 1e-20f, MOST = 1e37f;
+template <int OP> constexpr float LEAST_2 = OP == NORM || OP == ADD_NORM ? 1e-20f : 0.f;
+template <int OP> constexpr float MOST_2 = OP == GLU ? 1048576.f : 1e37f;
 
-// WPR warps per row, a block per row (eight rows with one warp each).  A thread holds CACHED float4s of the row's values; what
-// lies beyond them in longer rows is read again for every step.
-template <int OP, typename T, int WPR, int CACHED>
-__global__ void __launch_bounds__(WPR == 1 ? 256 : WPR * 32)
+// NT threads per row: a block, or one of its eight warps.  STAGED: the row is kept in shared memory (for the norms h, otherwise
+// v); longer rows are computed again from memory for every step.
+template <int OP, typename T, int NT, bool STAGED>
+__global__ void __launch_bounds__(NT == 32 ? 256 : NT)
 k_rows_i8(const T *x, const T *r, const float *w, uint32_t n, float eps, uint32_t rows, T *h, int8_t *q, float *scales) {
-    constexpr bool IS_NORM = OP == NORM || OP == ADD_NORM;
-    __shared__ double part_ss[WPR];
-    __shared__ uint32_t part_max[WPR], part_up[WPR];
-    __shared__ unsigned long long most64;
+    constexpr bool IS_NORM = OP == NORM || OP == ADD_NORM, ONE_WARP = NT == 32;
+    constexpr int W = NT / 32;
+    extern __shared__ float4 stage[];
+    __shared__ double part_ss[W];
+    __shared__ uint32_t part_max[W], part_2[W];
+    __shared__ unsigned long long largest;
     pdl_trigger();
-    const uint32_t lane = threadIdx.x & 31, warp = WPR == 1 ? 0 : threadIdx.x >> 5, tid = 32 * warp + lane;
-    const uint32_t row = WPR == 1 ? blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x, n4 = n / 4;
-    if (WPR > 1 && threadIdx.x == 0) most64 = 0;
+    const uint32_t lane = threadIdx.x & 31, warp = ONE_WARP ? 0 : threadIdx.x >> 5, tid = ONE_WARP ? lane : threadIdx.x;
+    const uint32_t row = ONE_WARP ? blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x, n4 = n / 4;
+    if (!ONE_WARP && tid == 0) largest = 0;
     pdl_wait();
     if (row >= rows) return; // whole warps
-    const size_t base = (size_t)row * n;
-    x += base;
-    if constexpr (OP == ADD_NORM || OP == GLU) r += base;
-    if constexpr (OP == ADD_NORM) h += base;
-    q += base;
-    constexpr uint32_t STEP = WPR * 32;
+    float4 *const kept = stage + (ONE_WARP ? (threadIdx.x >> 5) * n4 : 0);
+    x += (size_t)row * n;
+    if constexpr (OP == ADD_NORM || OP == GLU) r += (size_t)row * n;
+    if constexpr (OP == ADD_NORM) h += (size_t)row * n;
+    uint32_t *const out = reinterpret_cast<uint32_t *>(q + (size_t)row * n);
+    const float4 *const w4 = reinterpret_cast<const float4 *>(w);
 
-    // The row: for the norms h, of which v = h w; otherwise v itself.
-    float4 a[CACHED], b[OP == PLAIN ? 1 : CACHED];
-#pragma unroll
-    for (int j = 0; j < CACHED; j++)
-        if (tid + STEP * j < n4) a[j] = load4(x + 4 * (tid + STEP * j));
-    if constexpr (OP == ADD_NORM || OP == GLU)
-#pragma unroll
-        for (int j = 0; j < CACHED; j++)
-            if (tid + STEP * j < n4) b[j] = load4(r + 4 * (tid + STEP * j));
-    if constexpr (OP == ADD_NORM)
-#pragma unroll
-        for (int j = 0; j < CACHED; j++)
-            if (tid + STEP * j < n4) store4(h + 4 * (tid + STEP * j), a[j] = sum4(x, a[j], b[j]));
-    if constexpr (IS_NORM)
-#pragma unroll
-        for (int j = 0; j < CACHED; j++)
-            if (tid + STEP * j < n4) b[j] = reinterpret_cast<const float4 *>(w)[tid + STEP * j];
-    // One group of four beyond the cached ones; `first`: the sum is still to be written.
-    auto beyond = [&](uint32_t i, float4 &va, float4 &vb, bool first) {
-        va = load4((OP == ADD_NORM && !first ? (const T *)h : x) + 4 * i);
-        if constexpr (OP == ADD_NORM)
-            if (first) store4(h + 4 * i, va = sum4(x, va, load4(r + 4 * i)));
-        if constexpr (OP == GLU) vb = load4(r + 4 * i);
-        if constexpr (IS_NORM) vb = reinterpret_cast<const float4 *>(w)[i];
+    auto values = [&](const float4 &a, const float4 &b) {
+        if constexpr (OP == PLAIN) return a;
+        else if constexpr (OP == GLU) return make_float4(gated(a.x, b.x), gated(a.y, b.y), gated(a.z, b.z), gated(a.w, b.w));
+        else return make_float4(a.x * b.x, a.y * b.y, a.z * b.z, a.w * b.w);
     };
-    auto value = [](float va, float vb) { return OP == PLAIN ? va : OP == GLU ? gated(va, vb) : va * vb; };
-    auto value64 = [](float va, float vb) { return OP == PLAIN ? (double)va : OP == GLU ? gated64(va, vb) : (double)va * (double)vb; };
-    // The exact value of element i of the row (from memory: by now this thread has written h there).
+    // v of group i of four, after the row has been read once.
+    auto again = [&](uint32_t i) {
+        if constexpr (STAGED) return IS_NORM ? values(kept[i], w4[i]) : kept[i];
+        else if constexpr (OP == ADD_NORM) return values(load4((const T *)h + 4 * i), w4[i]);
+        else if constexpr (OP == NORM) return values(load4(x + 4 * i), w4[i]);
+        else if constexpr (OP == GLU) return values(load4(x + 4 * i), load4(r + 4 * i));
+        else return load4(x + 4 * i);
+    };
+    // Value i in 64 bits, from memory (of h this thread has written its own values there).
     auto exact = [&](uint32_t i) {
-        const float va = load1(OP == ADD_NORM ? (const T *)h + i : x + i);
-        return value64(va, OP == GLU ? load1(r + i) : IS_NORM ? w[i] : 0.f);
+        const float a = load1(OP == ADD_NORM ? (const T *)h + i : x + i);
+        if constexpr (OP == PLAIN) return (double)a;
+        else if constexpr (OP == GLU) return gated64((double)a, (double)load1(r + i));
+        else return (double)a * (double)w[i];
     };
 
     double ss = 0.0;
-    uint32_t most = 0, up = 0; // bits of non-negative numbers are ordered as the numbers, NaN above infinity
-    auto take = [&](const float4 &va, const float4 &vb, float4 &v) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float e = value(part(va, i), part(vb, i));
-            if constexpr (IS_NORM) ss = fma((double)part(va, i), (double)part(va, i), ss);
-            most = max(most, __float_as_uint(e) & 0x7FFFFFFFu);
-            if constexpr (OP == GLU) up = max(up, __float_as_uint(part(vb, i)) & 0x7FFFFFFFu);
-            (i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w) = e;
+    uint32_t most = 0, most_2 = 0;
+    auto take = [&](uint32_t i, float4 a, float4 b) {
+        if constexpr (OP == ADD_NORM) a = add4(h + 4 * i, a, b);
+        if constexpr (IS_NORM) {
+            const float squares = fmaf(a.x, a.x, a.y * a.y) + fmaf(a.z, a.z, a.w * a.w);
+            ss += (double)squares;
+            most_2 = max(most_2, magnitude(squares));
         }
+        if constexpr (OP == GLU) most_2 = max(most_2, magnitude(b));
+        const float4 v = IS_NORM ? values(a, w4[i]) : values(a, b);
+        most = max(most, magnitude(v));
+        if constexpr (STAGED) kept[i] = IS_NORM ? a : v;
     };
+    constexpr uint32_t AHEAD = 4; // loads of either input that are under way together
+    uint32_t i = tid;
+    for (; i + (AHEAD - 1) * NT < n4; i += AHEAD * NT) {
+        float4 a[AHEAD], b[AHEAD];
 #pragma unroll
-    for (int j = 0; j < CACHED; j++)
-        if (tid + STEP * j < n4) {
-            float4 v;
-            take(a[j], b[OP == PLAIN ? 0 : j], v);
-            if constexpr (!IS_NORM) a[j] = v;
+        for (uint32_t j = 0; j < AHEAD; j++) {
+            a[j] = load4(x + 4 * (i + j * NT));
+            if constexpr (OP == ADD_NORM || OP == GLU) b[j] = load4(r + 4 * (i + j * NT));
         }
-    for (uint32_t i = tid + STEP * CACHED; i < n4; i += STEP) {
-        float4 va, vb, v;
-        beyond(i, va, vb, true);
-        take(va, vb, v);
+#pragma unroll
+        for (uint32_t j = 0; j < AHEAD; j++) take(i + j * NT, a[j], b[j]);
     }
+    if (i < n4) {
+        float4 a[AHEAD - 1], b[AHEAD - 1];
+#pragma unroll
+        for (uint32_t j = 0; j < AHEAD - 1; j++)
+            if (i + j * NT < n4) {
+                a[j] = load4(x + 4 * (i + j * NT));
+                if constexpr (OP == ADD_NORM || OP == GLU) b[j] = load4(r + 4 * (i + j * NT));
+            }
+#pragma unroll
+        for (uint32_t j = 0; j < AHEAD - 1; j++)
+            if (i + j * NT < n4) take(i + j * NT, a[j], b[j]);
+    }
+    const uint32_t own_most = most;
     if constexpr (IS_NORM)
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
     most = __reduce_max_sync(0xffffffffu, most);
-    if constexpr (OP == GLU) up = __reduce_max_sync(0xffffffffu, up);
-    if constexpr (WPR > 1) {
+    if constexpr (OP != PLAIN) most_2 = __reduce_max_sync(0xffffffffu, most_2);
+    if constexpr (!ONE_WARP) {
         if (lane == 0) {
             part_ss[warp] = ss;
             part_max[warp] = most;
-            part_up[warp] = up;
+            part_2[warp] = most_2;
         }
         __syncthreads();
-        const uint32_t l = lane < WPR ? lane : 0;
-        most = __reduce_max_sync(0xffffffffu, part_max[l]);
-        if constexpr (OP == GLU) up = __reduce_max_sync(0xffffffffu, part_up[l]);
+        most = __reduce_max_sync(0xffffffffu, part_max[lane % W]);
+        if constexpr (OP != PLAIN) most_2 = __reduce_max_sync(0xffffffffu, part_2[lane % W]);
     }
 
     // The row's largest |v|, exactly.
+    const bool fast = __uint_as_float(most) >= LEAST && __uint_as_float(most) <= MOST &&
+                      (OP == PLAIN || (__uint_as_float(most_2) >= LEAST_2<OP> && __uint_as_float(most_2) <= MOST_2<OP>));
     double a64 = 0.0;
-    const bool fast = __uint_as_float(most) >= LEAST && __uint_as_float(most) <= MOST && (OP != GLU || __uint_as_float(up) < MOST_UP);
     bool bad = false;
     if (fast) {
-        if constexpr (OP == PLAIN) a64 = (double)__uint_as_float(most);
-        else {
-            const uint32_t floor = most - BELOW<OP>;
-            auto look = [&](float v, uint32_t i) {
-                if ((__float_as_uint(v) & 0x7FFFFFFFu) >= floor) a64 = fmax(a64, fabs(exact(i)));
-            };
-#pragma unroll
-            for (int j = 0; j < CACHED; j++)
-                if (tid + STEP * j < n4)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) look(IS_NORM ? part(a[j], i) * part(b[j], i) : part(a[j], i), 4 * (tid + STEP * j) + i);
-            for (uint32_t i = tid + STEP * CACHED; i < n4; i += STEP) {
-                float4 va, vb;
-                beyond(i, va, vb, false);
-                for (int k = 0; k < 4; k++) look(value(part(va, k), part(vb, k)), 4 * i + k);
+        if (OP == PLAIN) a64 = (double)__uint_as_float(most);
+        else if (own_most >= most - BELOW<OP>)
+            for (uint32_t i = tid; i < n4; i += NT) {
+                const float4 v = again(i);
+#pragma unroll 1
+                for (uint32_t k = 0; k < 4; k++)
+                    if (magnitude(k == 0 ? v.x : k == 1 ? v.y : k == 2 ? v.z : v.w) >= most - BELOW<OP>) a64 = fmax(a64, fabs(exact(4 * i + k)));
             }
-        }
     } else {
-        for (uint32_t i = tid; i < n4; i += STEP)
+        ss = 0.0;
+        for (uint32_t i = tid; i < n4; i += NT)
+#pragma unroll 1
             for (uint32_t k = 0; k < 4; k++) {
                 const double v = fabs(exact(4 * i + k));
                 bad |= !(v <= 3.4028234663852886e38);
                 a64 = fmax(a64, v);
+                if constexpr (IS_NORM) {
+                    const double a = (double)load1(OP == ADD_NORM ? (const T *)h + 4 * i + k : x + 4 * i + k);
+                    ss = fma(a, a, ss);
+                }
             }
+        if constexpr (IS_NORM) {
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
+            if (!ONE_WARP && lane == 0) part_ss[warp] = ss;
+        }
     }
     if (OP != PLAIN || !fast) {
-        if constexpr (WPR == 1) {
+        if constexpr (ONE_WARP) {
             bad = __any_sync(0xffffffffu, bad);
 #pragma unroll
             for (int off = 16; off > 0; off >>= 1) a64 = fmax(a64, __shfl_xor_sync(0xffffffffu, a64, off));
         } else {
-            if (a64 > 0.0) atomicMax(&most64, (unsigned long long)__double_as_longlong(a64));
+            if (a64 > 0.0) atomicMax(&largest, (unsigned long long)__double_as_longlong(a64));
             bad = __syncthreads_or(bad);
-            a64 = __longlong_as_double((long long)most64);
+            a64 = __longlong_as_double((long long)largest);
         }
     }
-    if (tid == 0) {
+    if (tid == NT - 1) { // not the first warp, which may have one group more of the row than the last
         double c = 1.0;
         if constexpr (IS_NORM) {
-            if constexpr (WPR > 1) {
+            if constexpr (!ONE_WARP) {
                 ss = 0.0;
-                for (int i = 0; i < WPR; i++) ss += part_ss[i];
+                for (int i = 0; i < W; i++) ss += part_ss[i];
             }
             c = 1.0 / sqrt(ss / (double)n + (double)eps);
         }
         scales[row] = bad ? __int_as_float(0x7fc00000) : (float)(a64 * c / 127.0);
     }
 
-    uint32_t *out = reinterpret_cast<uint32_t *>(q);
+    auto rounded = [&](uint32_t i) { return (uint32_t)__double2int_rn(exact(i) * 127.0 / a64) & 0xFFu; };
     if (!fast) {
-        for (uint32_t i = tid; i < n4; i += STEP) {
+        for (uint32_t i = tid; i < n4; i += NT) {
             uint32_t packed = 0;
             if (!bad && a64 > 0.0)
-                for (uint32_t k = 0; k < 4; k++) packed |= (uint32_t)(uint8_t)(int8_t)__double2int_rn(exact(4 * i + k) * 127.0 / a64) << (8 * k);
+#pragma unroll 1
+                for (uint32_t k = 0; k < 4; k++) packed |= rounded(4 * i + k) << (8 * k);
             out[i] = packed;
         }
         return;
     }
-    const float f = (float)(127.0 / a64);
-    auto quantise = [&](const float4 &v, uint32_t i) {
-        uint32_t bytes[4];
-        bool near = false;
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            // Added to 1.5 * 2^23 a number is rounded to a whole one, whose low byte is the sum's.
-            const float t = part(v, k) * f, whole = __fadd_rn(t, 12582912.f);
-            bytes[k] = __float_as_uint(whole);
-            near |= fabsf(t - __fsub_rn(whole, 12582912.f)) > 0.5f - NEAR<OP>;
-        }
-        if (near)
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const float t = part(v, k) * f;
-                if (fabsf(t - __fsub_rn(__uint_as_float(bytes[k]), 12582912.f)) > 0.5f - NEAR<OP>) bytes[k] = (uint32_t)__double2int_rn(exact(4 * i + k) * 127.0 / a64);
-            }
-        out[i] = __byte_perm(__byte_perm(bytes[0], bytes[1], 0x0040), __byte_perm(bytes[2], bytes[3], 0x0040), 0x5410);
+    const float f = 127.f / (float)a64;
+    // Added to 1.5 * 2^23 a number is rounded to a whole one, whose low byte is the sum's; `rest` is what the rounding took.
+    auto step = [&](float v, uint32_t &bytes, float &rest) {
+        const float whole = fmaf(v, f, 12582912.f);
+        bytes = __float_as_uint(whole);
+        rest = fabsf(fmaf(v, f, -__fsub_rn(whole, 12582912.f)));
     };
-    auto product = [](const float4 &va, const float4 &vb) { return make_float4(va.x * vb.x, va.y * vb.y, va.z * vb.z, va.w * vb.w); };
-#pragma unroll
-    for (int j = 0; j < CACHED; j++)
-        if (tid + STEP * j < n4) quantise(IS_NORM ? product(a[j], b[IS_NORM ? j : 0]) : a[j], tid + STEP * j);
-    for (uint32_t i = tid + STEP * CACHED; i < n4; i += STEP) {
-        float4 va, vb;
-        beyond(i, va, vb, false);
-        quantise(make_float4(value(va.x, vb.x), value(va.y, vb.y), value(va.z, vb.z), value(va.w, vb.w)), i);
+#pragma unroll 2
+    for (uint32_t i = tid; i < n4; i += NT) {
+        const float4 v = again(i);
+        uint32_t b0, b1, b2, b3;
+        float r0, r1, r2, r3;
+        step(v.x, b0, r0), step(v.y, b1, r1), step(v.z, b2, r2), step(v.w, b3, r3);
+        uint32_t packed = __byte_perm(__byte_perm(b0, b1, 0x0040), __byte_perm(b2, b3, 0x0040), 0x5410);
+        if (fmaxf(fmaxf(r0, r1), fmaxf(r2, r3)) > 0.5f - 128 * OFF<OP>) { // one may be on the wrong side: by its own size?
+#pragma unroll 1
+            for (uint32_t k = 0; k < 4; k++) {
+                const float e = k == 0 ? v.x : k == 1 ? v.y : k == 2 ? v.z : v.w, rest = k == 0 ? r0 : k == 1 ? r1 : k == 2 ? r2 : r3;
+                if (rest > 0.5f - (fabsf(e * f) + 0.5f) * OFF<OP>) packed = (packed & ~(0xFFu << (8 * k))) | rounded(4 * i + k) << (8 * k);
+            }
+        }
+        out[i] = packed;
     }
+}
+
+constexpr size_t STAGE_MOST = 200 << 10;
+
+template <int OP, typename T, int NT>
+cudaError_t launch_nt(fq_device *dev, const T *x, const T *r, const float *w, uint32_t n, float eps, uint32_t rows, T *h, int8_t *q, float *scales) {
+    const size_t bytes = (size_t)n * 4 * (NT == 32 ? 8 : 1);
+    const dim3 grid(NT == 32 ? (rows + 7) / 8 : rows), block(NT == 32 ? 256 : NT);
+    if (bytes > STAGE_MOST) return launch_pdl(k_rows_i8<OP, T, NT, false>, grid, block, 0, dev->stream, x, r, w, n, eps, rows, h, q, scales);
+    auto kernel = k_rows_i8<OP, T, NT, true>;
+    if (bytes > (40 << 10)) { // beyond what a kernel may use unasked (48 KB with its own arrays): asked for once per device
+        static std::atomic<uint64_t> asked{0};
+        const uint64_t bit = 1ull << (dev->ordinal & 63);
+        if (!(asked.load(std::memory_order_relaxed) & bit) || dev->ordinal > 63) {
+            if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)STAGE_MOST)) return e;
+            asked.fetch_or(bit, std::memory_order_relaxed);
+        }
+    }
+    return launch_pdl(kernel, grid, block, bytes, dev->stream, x, r, w, n, eps, rows, h, q, scales);
 }
 
 template <int OP>
 int launch_rows(fq_device *dev, const char *what, const void *x, const void *r, int dtype, const float *w, uint32_t n, float eps, uint32_t rows,
                 void *h, int8_t *q, float *scales) {
-    auto go = [&](auto zero, auto wpr, auto cached) {
-        using T = decltype(zero);
-        constexpr int WPR = decltype(wpr)::value;
-        return launch_pdl(k_rows_i8<OP, T, WPR, decltype(cached)::value>, dim3(WPR == 1 ? (rows + 7) / 8 : rows), dim3(WPR == 1 ? 256 : WPR * 32), 0, dev->stream,
-                          (const T *)x, (const T *)r, w, n, eps, rows, (T *)h, q, scales);
-    };
     auto shape = [&](auto zero) {
-        using std::integral_constant;
-        constexpr integral_constant<int, 8> eight;
-        if (n <= 1024) return go(zero, integral_constant<int, 1>{}, eight);
-        if (rows <= 2 * (uint32_t)dev->sm_count || n > 8192) return go(zero, integral_constant<int, 16>{}, integral_constant<int, 10>{});
-        if (n > 4096) return go(zero, eight, eight);
-        return go(zero, integral_constant<int, 4>{}, eight);
+        using T = decltype(zero);
+        const T *tx = (const T *)x, *tr = (const T *)r;
+        if (n <= 1024) return launch_nt<OP, T, 32>(dev, tx, tr, w, n, eps, rows, (T *)h, q, scales);
+        if (n > 8192 || rows <= 2 * (uint32_t)dev->sm_count) return launch_nt<OP, T, 512>(dev, tx, tr, w, n, eps, rows, (T *)h, q, scales);
+        return launch_nt<OP, T, 256>(dev, tx, tr, w, n, eps, rows, (T *)h, q, scales);
     };
     const cudaError_t e = dtype == FQ_BF16 ? shape(__nv_bfloat16{}) : shape(float{});
     if (int rc = fq_check_cuda(dev, e, what)) return rc;
