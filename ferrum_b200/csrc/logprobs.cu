@@ -17,8 +17,8 @@
 //
 // The most likely tokens: every warp keeps its best 32 as a sorted list, one (value, index) key per lane, and puts a value in
 // only if it can still matter: above a bound that k values of the block are known to reach.  The bound starts with what is read
-// first -- each warp's m-th largest thread maximum, m * warps >= k, and of these the least -- so that few values pass it, and
-// rises with the lists.  Keys are unique (of equal values the lower index is larger), so the result does not depend on order.
+// first -- the k-th largest of some 64 thread maxima, the best of every warp -- so that few values pass it, and rises with the
+// lists.  Keys are unique (of equal values the lower index is larger), so the result does not depend on the order of warps.
 #include <algorithm>
 #include <cmath>
 
@@ -29,7 +29,8 @@ namespace {
 using namespace fqk;
 
 constexpr uint32_t MAX_TOP = 32, MAX_CLUSTER = 8;
-constexpr int UNROLL = 4; // 16-byte loads of a thread in flight
+constexpr int UNROLL = 4;        // 16-byte loads of a thread in flight
+constexpr uint32_t FIRSTS = 64;  // thread maxima that the first bound is taken from
 constexpr float LOG2E = 1.44269502f; // b: log2(e) rounded to fp32
 constexpr float SLACK = 20.f;        // how far b l may be above the pivot
 // Beyond a million the rounding of c is no longer small: a row whose largest logit lies there is summed in 64 bits (sum_64).
@@ -179,7 +180,8 @@ template <typename T, int NT, bool TOP>
 __global__ void __launch_bounds__(NT, 1024 / NT)
 k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids, uint32_t k, uint32_t parts, Outputs out) {
     constexpr int W = NT / 32, V = PER_LOAD<T>;
-    __shared__ uint32_t first_max[W], first_bound[W], bound;
+    __shared__ uint32_t first_max[W], bound;
+    __shared__ uint4 firsts[FIRSTS / 4];
     __shared__ Sums sums[W];
     __shared__ uint32_t counts[W], bads[W];
     __shared__ uint64_t lists[TOP ? W : 1][32];
@@ -217,17 +219,21 @@ k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids
         }
         return make_uint4(w[0], w[1], w[2], w[3]);
     };
+    const uint32_t whole_from = skip ? 1 : 0, whole_to = min(end, (uint32_t)(((uint64_t)skip + n) / V)); // pieces that lie in the row
     uint4 next[UNROLL];
-    auto fetch = [&](uint32_t j0) {
+    auto fetch = [&](uint32_t j0) { // of the block's UNROLL * NT pieces from j0 this thread's
+        if (j0 >= whole_from && j0 + UNROLL * NT <= whole_to) {
 #pragma unroll
-        for (int u = 0; u < UNROLL; u++) {
-            const uint32_t j = j0 + u * NT;
-            next[u] = make_uint4(0xFF800000u, 0xFF800000u, 0xFF800000u, 0xFF800000u); // nothing: -infinity, or in bf16 -infinity and 0
-            if constexpr (sizeof(T) == 2) next[u] = make_uint4(0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u);
-            if (j < end) next[u] = load(j);
+            for (int u = 0; u < UNROLL; u++) next[u] = __ldcg(reinterpret_cast<const uint4 *>(aligned) + j0 + u * NT + tid);
+        } else {
+#pragma unroll
+            for (int u = 0; u < UNROLL; u++) {
+                const uint32_t j = j0 + u * NT + tid, none = sizeof(T) == 2 ? 0xFF80FF80u : 0xFF800000u; // -infinity
+                next[u] = j < end ? load(j) : make_uint4(none, none, none, none);
+            }
         }
     };
-    fetch(begin + tid);
+    fetch(begin);
     const float given = id < n ? load1(l, id) : __int_as_float(0x7fc00000);
 
     // What is read first gives the pivot and a bound that k values of the block reach.
@@ -239,21 +245,35 @@ k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids
     uint32_t high = __reduce_max_sync(0xffffffffu, best);
     if (lane == 0) first_max[warp] = high;
     if constexpr (TOP) {
-        const uint32_t m = warps ? (k + warps - 1) / warps : 1; // this warp's m-th largest maximum
+        const uint32_t m = min(32u, FIRSTS / max(warps, 1u)); // of every warp, m * warps >= k
+        uint32_t *mine = reinterpret_cast<uint32_t *>(firsts) + warp * m;
+        if (warp < warps) {
 #pragma unroll 1
-        for (uint32_t i = 1; i < m; i++) {
-            const uint32_t holders = __ballot_sync(0xffffffffu, best == high && best != 0);
-            if (holders && lane == (uint32_t)__ffs(holders) - 1) best = 0;
-            high = __reduce_max_sync(0xffffffffu, best);
+            for (uint32_t i = 0; i < m; i++) {
+                if (lane == 0) mine[i] = high;
+                const uint32_t holders = __ballot_sync(0xffffffffu, best == high);
+                if (lane == (uint32_t)__ffs(holders) - 1) best = 0;
+                high = __reduce_max_sync(0xffffffffu, best);
+            }
         }
-        if (lane == 0) first_bound[warp] = high;
+        for (uint32_t i = m * warps + tid; i < FIRSTS; i += NT) reinterpret_cast<uint32_t *>(firsts)[i] = 0;
     }
     __syncthreads();
     const float top = value_of(max(__reduce_max_sync(0xffffffffu, first_max[lane % W]), 1u << 23)); // -infinity where there is nothing (or NaN)
     Sums a{fmaxf(top, LEAST) * LOG2E, 0.f, 0.f};
     float limit = fminf(fmaf(SLACK, 1.f / LOG2E, fmaxf(top, LEAST)), MOST); // logits above it move the pivot
     uint32_t least = 0; // values of a lower order do not matter any more; 0: all do
-    if constexpr (TOP) least = __reduce_min_sync(0xffffffffu, lane < warps ? first_bound[lane] : 0xFFFFFFFFu);
+    if constexpr (TOP) { // the least of those that fewer than k are above
+        const uint32_t x = reinterpret_cast<const uint32_t *>(firsts)[lane], y = reinterpret_cast<const uint32_t *>(firsts)[lane + 32];
+        uint32_t above_x = 0, above_y = 0;
+#pragma unroll 4
+        for (uint32_t i = 0; i < FIRSTS / 4; i++) {
+            const uint4 f = firsts[i];
+            above_x += (f.x > x) + (f.y > x) + (f.z > x) + (f.w > x);
+            above_y += (f.x > y) + (f.y > y) + (f.z > y) + (f.w > y);
+        }
+        least = __reduce_min_sync(0xffffffffu, min(above_x < k ? x : 0xFFFFFFFFu, above_y < k ? y : 0xFFFFFFFFu));
+    }
     float below = just_below(least);
     bool bad = false, beyond = false, some = false; // a NaN or +infinity; a logit above MOST; one above -infinity
     uint32_t count = 0;
@@ -266,7 +286,7 @@ k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids
         float mx[UNROLL];
 #pragma unroll
         for (int u = 0; u < UNROLL; u++) now[u] = next[u];
-        fetch(j0 + UNROLL * NT + tid);
+        fetch(j0 + UNROLL * NT);
 #pragma unroll
         for (int u = 0; u < UNROLL; u++) mx[u] = piece_max<T>(now[u]);
         if constexpr (TOP) {
@@ -284,12 +304,14 @@ k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids
                         uint4 piece = u == 0 ? now[0] : u == 1 ? now[1] : u == 2 ? now[2] : now[3];
                         piece = make_uint4(__shfl_sync(0xffffffffu, piece.x, src), __shfl_sync(0xffffffffu, piece.y, src), __shfl_sync(0xffffffffu, piece.z, src),
                                            __shfl_sync(0xffffffffu, piece.w, src));
-#pragma unroll 1
-                        for (int i = 0; i < V; i++) {
-                            const uint32_t w = word(piece, sizeof(T) == 2 ? i / 2 : i), at = j * V - skip + i;
-                            const uint32_t order = order_of(sizeof(T) == 4 ? __uint_as_float(w) : (i & 1) ? high_half(w) : low_half(w));
-                            if (order < least || at >= n) continue;
-                            const uint64_t key = key_of(order, at);
+                        // Lane i looks at value i; those that may matter go in one after the other.
+                        const uint32_t i = lane % V, w = word(piece, sizeof(T) == 2 ? i / 2 : i), at = j * V - skip + i;
+                        const uint32_t order = order_of(sizeof(T) == 4 ? __uint_as_float(w) : (i & 1) ? high_half(w) : low_half(w));
+                        uint32_t fit = __ballot_sync(0xffffffffu, lane < V && at < n && order >= least);
+                        while (fit) {
+                            const uint64_t key = __shfl_sync(0xffffffffu, key_of(order, at), __ffs(fit) - 1);
+                            fit &= fit - 1;
+                            if ((uint32_t)(key >> 32) < least) continue; // (uniform)
                             const uint32_t pos = __popc(__ballot_sync(0xffffffffu, list > key));
                             const uint64_t up = __shfl_up_sync(0xffffffffu, list, 1);
                             if (lane >= pos) list = lane == pos ? key : up;
@@ -305,15 +327,25 @@ k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids
         float highest = mx[0];
 #pragma unroll
         for (int u = 1; u < UNROLL; u++) highest = max_nan(highest, mx[u]);
-        if (!(highest <= given))
+        if (!(highest <= given)) {
+            if constexpr (sizeof(T) == 2) { // ones added in bf16: 4 * UNROLL at most
+                const __nv_bfloat162 g = __float2bfloat162_rn(given);
+                __nv_bfloat162 above = __float2bfloat162_rn(0.f);
 #pragma unroll
-            for (int u = 0; u < UNROLL; u++)
+                for (int u = 0; u < UNROLL; u++)
 #pragma unroll
-                for (int i = 0; i < V / 2; i++) {
-                    const float2 v = pair_of<T>(now[u], i);
-                    count += v.x > given;
-                    count += v.y > given;
-                }
+                    for (int i = 0; i < 4; i++) {
+                        const uint32_t w = word(now[u], i);
+                        above = __hadd2(above, __hgt2(*reinterpret_cast<const __nv_bfloat162 *>(&w), g));
+                    }
+                count += (uint32_t)(__low2float(above) + __high2float(above));
+            } else {
+#pragma unroll
+                for (int u = 0; u < UNROLL; u++)
+#pragma unroll
+                    for (int i = 0; i < V; i++) count += __uint_as_float(word(now[u], i)) > given;
+            }
+        }
         some |= highest > -INFINITY;
         if (!(highest <= limit)) {
             bad |= !(highest < INFINITY);
@@ -424,6 +456,8 @@ template <typename T>
 cudaError_t launch_rows(fq_device *dev, const T *logits, uint32_t n, size_t stride, uint32_t rows, const uint32_t *ids, uint32_t k, const Outputs &out) {
     uint32_t parts = 1;
     while (parts < MAX_CLUSTER && rows * (2 * parts) <= 2 * (uint32_t)dev->sm_count && n / (2 * parts) >= 4096) parts *= 2;
+    // TODO
+    if (parts == 1 && n > 8192) return k ? launch_shape<T, 256, true>(dev, logits, n, stride, rows, ids, k, parts, out) : launch_shape<T, 256, false>(dev, logits, n, stride, rows, ids, k, parts, out);
     if (n <= 8192) return k ? launch_shape<T, 128, true>(dev, logits, n, stride, rows, ids, k, parts, out) : launch_shape<T, 128, false>(dev, logits, n, stride, rows, ids, k, parts, out);
     return k ? launch_shape<T, 512, true>(dev, logits, n, stride, rows, ids, k, parts, out) : launch_shape<T, 512, false>(dev, logits, n, stride, rows, ids, k, parts, out);
 }

@@ -9,8 +9,8 @@
 // over threads.
 //
 // A row is read from memory once and kept in shared memory, every thread its own values of it.  v is computed in 32 bits; the
-// few values that decide are taken again in 64: those that may be the row's largest, and those whose quotient lies within
-// the error of 32 bits of the border between two whole numbers.  Squares are added by fours in 32 bits and from there in 64.
+// few values that decide are taken again in 64: those that may be the row's largest, by one thread while the others round, and
+// after it those whose quotient lies within the error of 32 bits of the border between two whole numbers.  Squares are added by fours in 32 bits and from there in 64.
 // (Held in registers, unrolled over a row, the same took 105 registers and 63 instructions a value, a third of the time
 // waiting for instructions: 2048 x 5120 bf16 45 us.)
 #include <atomic>
@@ -25,11 +25,13 @@ using namespace fqk;
 enum Op { PLAIN, NORM, ADD_NORM, GLU };
 
 // Four values at a time.
-__device__ __forceinline__ float4 load4(const float *p) { return __ldcg(reinterpret_cast<const float4 *>(p)); }
-__device__ __forceinline__ float4 load4(const __nv_bfloat16 *p) {
-    const uint2 b = __ldcg(reinterpret_cast<const uint2 *>(p));
+__device__ __forceinline__ float4 raw4(const float *p) { return __ldcg(reinterpret_cast<const float4 *>(p)); }
+__device__ __forceinline__ uint2 raw4(const __nv_bfloat16 *p) { return __ldcg(reinterpret_cast<const uint2 *>(p)); }
+__device__ __forceinline__ float4 floats(const float4 &v) { return v; }
+__device__ __forceinline__ float4 floats(const uint2 &b) {
     return make_float4(__uint_as_float(b.x << 16), __uint_as_float(b.x & 0xFFFF0000u), __uint_as_float(b.y << 16), __uint_as_float(b.y & 0xFFFF0000u));
 }
+template <typename T> __device__ __forceinline__ float4 load4(const T *p) { return floats(raw4(p)); }
 __device__ __forceinline__ float load1(const float *p) { return __ldcg(p); }
 __device__ __forceinline__ float load1(const __nv_bfloat16 *p) { return __uint_as_float((uint32_t)__ldcg(reinterpret_cast<const unsigned short *>(p)) << 16); }
 // a + b, stored as its type keeps it, and as it is kept.
@@ -42,19 +44,37 @@ __device__ __forceinline__ float4 add4(__nv_bfloat16 *p, const float4 &a, const 
     const __nv_bfloat162 lo = __floats2bfloat162_rn(a.x + b.x, a.y + b.y), hi = __floats2bfloat162_rn(a.z + b.z, a.w + b.w);
     const uint2 u = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
     *reinterpret_cast<uint2 *>(p) = u;
-    return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xFFFF0000u));
+    return floats(u);
 }
-__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; } // ordered as |v|, NaN above infinity
-__device__ __forceinline__ uint32_t magnitude(const float4 &v) { return max(max(magnitude(v.x), magnitude(v.y)), max(magnitude(v.z), magnitude(v.w))); }
+__device__ __forceinline__ float max_abs(float a, float b) { // NaN if one is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
+    return r;
+}
+__device__ __forceinline__ float max_abs(const float4 &v) { return max_abs(max_abs(v.x, v.y), max_abs(v.z, v.w)); }
+// Two values an instruction.
+__device__ __forceinline__ float4 mul4(const float4 &a, const float4 &b) {
+    const float2 lo = __fmul2_rn(make_float2(a.x, a.y), make_float2(b.x, b.y)), hi = __fmul2_rn(make_float2(a.z, a.w), make_float2(b.z, b.w));
+    return make_float4(lo.x, lo.y, hi.x, hi.y);
+}
+__device__ __forceinline__ float4 fma4(const float4 &a, float b, const float4 &c) {
+    const float2 b2 = make_float2(b, b);
+    const float2 lo = __ffma2_rn(make_float2(a.x, a.y), b2, make_float2(c.x, c.y)), hi = __ffma2_rn(make_float2(a.z, a.w), b2, make_float2(c.z, c.w));
+    return make_float4(lo.x, lo.y, hi.x, hi.y);
+}
+__device__ __forceinline__ float4 rsub4(float a, const float4 &b) { // a - b
+    const float2 lo = __fadd2_rn(make_float2(-b.x, -b.y), make_float2(a, a)), hi = __fadd2_rn(make_float2(-b.z, -b.w), make_float2(a, a));
+    return make_float4(lo.x, lo.y, hi.x, hi.y);
+}
 
 // silu(g) u.  Relative error: 2 steps (2^-22) of the exponential and as much of the quotient, two roundings: 10 * 2^-24; beyond
 // g = -87, where e^-g leaves the range of the quotient, 0 instead of less than 2^-118 |u|.
 __device__ __forceinline__ float gated(float g, float u) { return __fdividef(g, 1.f + expf(-g)) * u; }
 __device__ __forceinline__ double gated64(double g, double u) { return g / (1.0 + exp(-g)) * u; }
 
-// The part of a quotient t = 127 v / a that its computation in 32 bits may be off: v as above or (norms) once rounded, a and
+// The part of a quotient t = 127 v / a that its computation in 32 bits may be off: v and a as above or (norms) once rounded,
 // 127 / a rounded.
-template <int OP> constexpr float OFF = OP == GLU ? 14 * 0x1p-24f : 4 * 0x1p-24f;
+template <int OP> constexpr float OFF = OP == GLU ? 24 * 0x1p-24f : 4 * 0x1p-24f;
 // How many steps of fp32 the exact largest value may lie below the largest fp32 one: single roundings keep their order; a
 // gated unit is off by at most 10 steps, and so is the largest.
 template <int OP> constexpr uint32_t BELOW = OP == GLU ? 24 : 0;
@@ -67,7 +87,7 @@ template <int OP> constexpr float MOST_2 = OP == GLU ? 1048576.f : 1e37f;
 // NT threads per row: a block, or one of its eight warps.  STAGED: the row is kept in shared memory (for the norms h, otherwise
 // v); longer rows are computed again from memory for every step.
 template <int OP, typename T, int NT, bool STAGED>
-__global__ void __launch_bounds__(NT == 32 ? 256 : NT)
+__global__ void __launch_bounds__(NT == 32 ? 256 : NT, NT == 512 ? 2 : 5)
 k_rows_i8(const T *x, const T *r, const float *w, uint32_t n, float eps, uint32_t rows, T *h, int8_t *q, float *scales) {
     constexpr bool IS_NORM = OP == NORM || OP == ADD_NORM, ONE_WARP = NT == 32;
     constexpr int W = NT / 32;
@@ -91,7 +111,7 @@ k_rows_i8(const T *x, const T *r, const float *w, uint32_t n, float eps, uint32_
     auto values = [&](const float4 &a, const float4 &b) {
         if constexpr (OP == PLAIN) return a;
         else if constexpr (OP == GLU) return make_float4(gated(a.x, b.x), gated(a.y, b.y), gated(a.z, b.z), gated(a.w, b.w));
-        else return make_float4(a.x * b.x, a.y * b.y, a.z * b.z, a.w * b.w);
+        else return mul4(a, b);
     };
     // v of group i of four, after the row has been read once.
     auto again = [&](uint32_t i) {
@@ -101,58 +121,46 @@ k_rows_i8(const T *x, const T *r, const float *w, uint32_t n, float eps, uint32_
         else if constexpr (OP == GLU) return values(load4(x + 4 * i), load4(r + 4 * i));
         else return load4(x + 4 * i);
     };
-    // Value i in 64 bits, from memory (of h this thread has written its own values there).
+    // Value i in 64 bits.  (In memory a thread has written its own values of h.)
     auto exact = [&](uint32_t i) {
-        const float a = load1(OP == ADD_NORM ? (const T *)h + i : x + i);
+        const float a = STAGED && OP != GLU ? reinterpret_cast<const float *>(kept)[i] : load1(OP == ADD_NORM ? (const T *)h + i : x + i);
         if constexpr (OP == PLAIN) return (double)a;
         else if constexpr (OP == GLU) return gated64((double)a, (double)load1(r + i));
         else return (double)a * (double)w[i];
     };
 
     double ss = 0.0;
-    uint32_t most = 0, most_2 = 0;
+    float own = 0.f, own_2 = 0.f;
     auto take = [&](uint32_t i, float4 a, float4 b) {
         if constexpr (OP == ADD_NORM) a = add4(h + 4 * i, a, b);
         if constexpr (IS_NORM) {
             const float squares = fmaf(a.x, a.x, a.y * a.y) + fmaf(a.z, a.z, a.w * a.w);
             ss += (double)squares;
-            most_2 = max(most_2, magnitude(squares));
+            own_2 = max_abs(own_2, squares);
         }
-        if constexpr (OP == GLU) most_2 = max(most_2, magnitude(b));
+        if constexpr (OP == GLU) own_2 = max_abs(own_2, max_abs(b));
         const float4 v = IS_NORM ? values(a, w4[i]) : values(a, b);
-        most = max(most, magnitude(v));
+        own = max_abs(own, max_abs(v));
         if constexpr (STAGED) kept[i] = IS_NORM ? a : v;
     };
-    constexpr uint32_t AHEAD = 4; // loads of either input that are under way together
-    uint32_t i = tid;
-    for (; i + (AHEAD - 1) * NT < n4; i += AHEAD * NT) {
-        float4 a[AHEAD], b[AHEAD];
+    constexpr uint32_t AHEAD = sizeof(T) == 2 ? 4 : 2; // loads of either input that are under way together
+    for (uint32_t i = tid; i < n4; i += AHEAD * NT) {
+        decltype(raw4(x)) a[AHEAD], b[AHEAD];
 #pragma unroll
-        for (uint32_t j = 0; j < AHEAD; j++) {
-            a[j] = load4(x + 4 * (i + j * NT));
-            if constexpr (OP == ADD_NORM || OP == GLU) b[j] = load4(r + 4 * (i + j * NT));
-        }
-#pragma unroll
-        for (uint32_t j = 0; j < AHEAD; j++) take(i + j * NT, a[j], b[j]);
-    }
-    if (i < n4) {
-        float4 a[AHEAD - 1], b[AHEAD - 1];
-#pragma unroll
-        for (uint32_t j = 0; j < AHEAD - 1; j++)
+        for (uint32_t j = 0; j < AHEAD; j++)
             if (i + j * NT < n4) {
-                a[j] = load4(x + 4 * (i + j * NT));
-                if constexpr (OP == ADD_NORM || OP == GLU) b[j] = load4(r + 4 * (i + j * NT));
+                a[j] = raw4(x + 4 * (i + j * NT));
+                if constexpr (OP == ADD_NORM || OP == GLU) b[j] = raw4(r + 4 * (i + j * NT));
             }
 #pragma unroll
-        for (uint32_t j = 0; j < AHEAD - 1; j++)
-            if (i + j * NT < n4) take(i + j * NT, a[j], b[j]);
+        for (uint32_t j = 0; j < AHEAD; j++)
+            if (i + j * NT < n4) take(i + j * NT, floats(a[j]), floats(b[j]));
     }
-    const uint32_t own_most = most;
     if constexpr (IS_NORM)
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-    most = __reduce_max_sync(0xffffffffu, most);
-    if constexpr (OP != PLAIN) most_2 = __reduce_max_sync(0xffffffffu, most_2);
+    // Bits of numbers that are not negative are ordered as the numbers, NaN above infinity.
+    uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(own)), most_2 = OP == PLAIN ? 0 : __reduce_max_sync(0xffffffffu, __float_as_uint(own_2));
     if constexpr (!ONE_WARP) {
         if (lane == 0) {
             part_ss[warp] = ss;
@@ -164,20 +172,20 @@ k_rows_i8(const T *x, const T *r, const float *w, uint32_t n, float eps, uint32_
         if constexpr (OP != PLAIN) most_2 = __reduce_max_sync(0xffffffffu, part_2[lane % W]);
     }
 
-    // The row's largest |v|, exactly.
     const bool fast = __uint_as_float(most) >= LEAST && __uint_as_float(most) <= MOST &&
                       (OP == PLAIN || (__uint_as_float(most_2) >= LEAST_2<OP> && __uint_as_float(most_2) <= MOST_2<OP>));
-    double a64 = 0.0;
+    double a64 = 0.0; // the row's largest |v|, exactly: of the thread's own values first
     bool bad = false;
+    uint32_t near = 0; // groups of the thread with a value next to a border
     if (fast) {
-        if (OP == PLAIN) a64 = (double)__uint_as_float(most);
-        else if (own_most >= most - BELOW<OP>)
+        if (__float_as_uint(own) >= most - BELOW<OP>)
             for (uint32_t i = tid; i < n4; i += NT) {
                 const float4 v = again(i);
 #pragma unroll 1
                 for (uint32_t k = 0; k < 4; k++)
-                    if (magnitude(k == 0 ? v.x : k == 1 ? v.y : k == 2 ? v.z : v.w) >= most - BELOW<OP>) a64 = fmax(a64, fabs(exact(4 * i + k)));
+                    if (__float_as_uint(fabsf(k == 0 ? v.x : k == 1 ? v.y : k == 2 ? v.z : v.w)) >= most - BELOW<OP>) a64 = fmax(a64, fabs(exact(4 * i + k)));
             }
+        if (!ONE_WARP && a64 > 0.0) atomicMax(&largest, (unsigned long long)__double_as_longlong(a64));
     } else {
         ss = 0.0;
         for (uint32_t i = tid; i < n4; i += NT)
@@ -191,22 +199,34 @@ k_rows_i8(const T *x, const T *r, const float *w, uint32_t n, float eps, uint32_
                     ss = fma(a, a, ss);
                 }
             }
+        if (!ONE_WARP && a64 > 0.0) atomicMax(&largest, (unsigned long long)__double_as_longlong(a64));
         if constexpr (IS_NORM) {
 #pragma unroll
             for (int off = 16; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
             if (!ONE_WARP && lane == 0) part_ss[warp] = ss;
         }
     }
-    if (OP != PLAIN || !fast) {
-        if constexpr (ONE_WARP) {
-            bad = __any_sync(0xffffffffu, bad);
-#pragma unroll
-            for (int off = 16; off > 0; off >>= 1) a64 = fmax(a64, __shfl_xor_sync(0xffffffffu, a64, off));
-        } else {
-            if (a64 > 0.0) atomicMax(&largest, (unsigned long long)__double_as_longlong(a64));
-            bad = __syncthreads_or(bad);
-            a64 = __longlong_as_double((long long)largest);
+    // t = 127 v / a: added to 1.5 * 2^23 it is rounded to a whole number, whose low byte is the sum's; `rest` is what that took.
+    constexpr float MAGIC = 12582912.f;
+    const float f = 127.f / __uint_as_float(most);
+    auto rests = [&](const float4 &v, const float4 &whole) { return fma4(v, f, rsub4(MAGIC, whole)); };
+    auto wholes = [&](const float4 &v) { return fma4(v, f, make_float4(MAGIC, MAGIC, MAGIC, MAGIC)); };
+    if (fast) { // while the largest value is taken in 64 bits elsewhere
+        uint32_t at = 0;
+#pragma unroll 2
+        for (uint32_t i = tid; i < n4; i += NT, at++) {
+            const float4 v = again(i), whole = wholes(v);
+            out[i] = __byte_perm(__byte_perm(__float_as_uint(whole.x), __float_as_uint(whole.y), 0x0040), __byte_perm(__float_as_uint(whole.z), __float_as_uint(whole.w), 0x0040), 0x5410);
+            if (max_abs(rests(v, whole)) > 0.5f - 128 * OFF<OP>) near |= 1u << (at & 31);
         }
+    }
+    if constexpr (ONE_WARP) {
+        bad = __any_sync(0xffffffffu, bad);
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) a64 = fmax(a64, __shfl_xor_sync(0xffffffffu, a64, off));
+    } else {
+        bad = __syncthreads_or(bad);
+        a64 = __longlong_as_double((long long)largest);
     }
     if (tid == NT - 1) { // not the first warp, which may have one group more of the row than the last
         double c = 1.0;
@@ -221,7 +241,21 @@ k_rows_i8(const T *x, const T *r, const float *w, uint32_t n, float eps, uint32_
     }
 
     auto rounded = [&](uint32_t i) { return (uint32_t)__double2int_rn(exact(i) * 127.0 / a64) & 0xFFu; };
-    if (!fast) {
+    if (fast) {
+        // Values that may be on the wrong side of a border, by their own size (bit b of `near`: groups b, b + 32, ...).
+        while (near) {
+            const uint32_t b = __ffs(near) - 1;
+            near &= near - 1;
+            for (uint32_t i = tid + b * NT; i < n4; i += 32 * NT) {
+                const float4 v = again(i), whole = wholes(v), rest = rests(v, whole);
+#pragma unroll 1
+                for (uint32_t k = 0; k < 4; k++) {
+                    const float e = k == 0 ? v.x : k == 1 ? v.y : k == 2 ? v.z : v.w, part = k == 0 ? rest.x : k == 1 ? rest.y : k == 2 ? rest.z : rest.w;
+                    if (fabsf(part) > 0.5f - (fabsf(e * f) + 0.5f) * OFF<OP>) reinterpret_cast<uint8_t *>(out)[4 * i + k] = (uint8_t)rounded(4 * i + k);
+                }
+            }
+        }
+    } else {
         for (uint32_t i = tid; i < n4; i += NT) {
             uint32_t packed = 0;
             if (!bad && a64 > 0.0)
@@ -229,30 +263,6 @@ k_rows_i8(const T *x, const T *r, const float *w, uint32_t n, float eps, uint32_
                 for (uint32_t k = 0; k < 4; k++) packed |= rounded(4 * i + k) << (8 * k);
             out[i] = packed;
         }
-        return;
-    }
-    const float f = 127.f / (float)a64;
-    // Added to 1.5 * 2^23 a number is rounded to a whole one, whose low byte is the sum's; `rest` is what the rounding took.
-    auto step = [&](float v, uint32_t &bytes, float &rest) {
-        const float whole = fmaf(v, f, 12582912.f);
-        bytes = __float_as_uint(whole);
-        rest = fabsf(fmaf(v, f, -__fsub_rn(whole, 12582912.f)));
-    };
-#pragma unroll 2
-    for (uint32_t i = tid; i < n4; i += NT) {
-        const float4 v = again(i);
-        uint32_t b0, b1, b2, b3;
-        float r0, r1, r2, r3;
-        step(v.x, b0, r0), step(v.y, b1, r1), step(v.z, b2, r2), step(v.w, b3, r3);
-        uint32_t packed = __byte_perm(__byte_perm(b0, b1, 0x0040), __byte_perm(b2, b3, 0x0040), 0x5410);
-        if (fmaxf(fmaxf(r0, r1), fmaxf(r2, r3)) > 0.5f - 128 * OFF<OP>) { // one may be on the wrong side: by its own size?
-#pragma unroll 1
-            for (uint32_t k = 0; k < 4; k++) {
-                const float e = k == 0 ? v.x : k == 1 ? v.y : k == 2 ? v.z : v.w, rest = k == 0 ? r0 : k == 1 ? r1 : k == 2 ? r2 : r3;
-                if (rest > 0.5f - (fabsf(e * f) + 0.5f) * OFF<OP>) packed = (packed & ~(0xFFu << (8 * k))) | rounded(4 * i + k) << (8 * k);
-            }
-        }
-        out[i] = packed;
     }
 }
 
