@@ -59,12 +59,12 @@ struct Job {
 };
 
 struct Ctl {
-    uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc_full[2], acc_empty[2], drained;
+    uint64_t full[MAX_STAGES], empty[MAX_STAGES], peer_full[MAX_STAGES], acc_full[2], acc_empty[2], drained;
     uint32_t tmem_base, abort_flag;
 };
 
 // kind::i8: D = s32, A = B = s8, both K-major.
-__device__ __forceinline__ uint32_t idesc_i8(uint32_t n) { return (2u << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((BM >> 4) << 24); }
+__device__ __forceinline__ uint32_t idesc_i8(uint32_t m, uint32_t n) { return (2u << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((m >> 4) << 24); }
 __device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
     asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}"
                  ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
@@ -116,6 +116,21 @@ __device__ __forceinline__ void store_value(const Job &J, const Target &T, uint3
     const size_t at = (size_t)token * T.rows + row;
     if (J.bf16) static_cast<__nv_bfloat16 *>(T.y)[at] = __float2bfloat16_rn(v);
     else static_cast<float *>(T.y)[at] = v;
+}
+
+// `live` tokens from m0 of the accumulator at `acc`: one weight row a lane, so that a warp's stores of a token are contiguous.
+__device__ __forceinline__ void store_tile(const Job &J, const Target &T, uint32_t acc, uint32_t m0, uint32_t live, uint32_t row, float ws, uint32_t lane) {
+    for (uint32_t c0 = 0; c0 < live; c0 += 16) {
+        const uint32_t mine = c0 + (lane & 15);
+        const float xs = mine < live ? __ldcg(J.x_scales + m0 + mine) : 0.f;
+        int v[16];
+        tmem_ld16(acc + c0, v);
+#pragma unroll
+        for (uint32_t c = 0; c < 16; c++) {
+            const float f = __shfl_sync(0xffffffffu, xs, c);
+            if (row < T.rows && c0 + c < live) store_value(J, T, m0 + c0 + c, row, v[c], f, ws);
+        }
+    }
 }
 
 template <bool SLICED>
@@ -187,7 +202,7 @@ k_gemm_i8(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ Job 
     } else if (warp == 1) {
         if (elect_one()) {
             pdl_wait(); // the clock of the bounded waits starts when there is something to wait for
-            const uint32_t idesc = idesc_i8(J.bn);
+            const uint32_t idesc = idesc_i8(BM, J.bn);
             uint32_t s = 0, phase = 0, buf = 0, buf_phase = 0;
             bool ok = true;
             for (uint32_t item = unit; item < J.items && ok; item += units) {
@@ -225,18 +240,7 @@ k_gemm_i8(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ Job 
                 const float ws = row < T.rows ? T.scales[row] : 0.f;
                 if (!__all_sync(0xffffffffu, mbar_wait(&ctl.acc_full[buf], buf_phase, &ctl, status))) break; // the warp agrees
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t acc = tmem + buf * J.bn + ((32 * quarter) << 16);
-                for (uint32_t c0 = 0; c0 < live; c0 += 16) {
-                    const uint32_t mine = c0 + (lane & 15);
-                    const float xs = mine < live ? __ldcg(J.x_scales + p.m0 + mine) : 0.f;
-                    int v[16];
-                    tmem_ld16(acc + c0, v);
-#pragma unroll
-                    for (uint32_t c = 0; c < 16; c++) {
-                        const float f = __shfl_sync(0xffffffffu, xs, c);
-                        if (row < T.rows && c0 + c < live) store_value(J, T, p.m0 + c0 + c, row, v[c], f, ws);
-                    }
-                }
+                store_tile(J, T, tmem + buf * J.bn + ((32 * quarter) << 16), p.m0, live, row, ws, lane);
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 mbar_arrive(&ctl.acc_empty[buf]);
                 if (++buf == 2) buf = 0, buf_phase ^= 1;
@@ -288,6 +292,148 @@ k_gemm_i8(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ Job 
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(J.tmem_cols) : "memory");
 }
 
+// Many tokens: two blocks of a cluster share one MMA (cta_group::2, M = 256): each holds 128 of the 256 weight rows and half of
+// the tokens in its shared memory, and the sums of its own rows in its tensor memory.  A block then takes in 16 KB of weights
+// and only half of a token tile for as many products, and what it takes in per product is what binds the kernel above.
+//
+// The even block issues the MMAs.  It learns that the other block's stage is full from that block's warp 1, which waits for it
+// and passes the arrival on; the commits that release a stage and hand over an accumulator arrive in both blocks; both blocks'
+// epilogues return the accumulator to the even one.
+__device__ __forceinline__ void umma_i8_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}"
+                 ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+__device__ __forceinline__ void umma_commit_pair(uint64_t *bar) { // arrives at this barrier in both blocks
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((uint16_t)3)
+                 : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_at(uint64_t *bar, uint32_t rank) { // the same barrier of block `rank` of the cluster
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_address(smem_u32(bar), rank)) : "memory");
+}
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS)
+k_gemm_i8_pair(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ Job J, int *status) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ Ctl ctl;
+    uint8_t *ring = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023); // the same place in both blocks
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = blockIdx.x & 1, unit = blockIdx.x >> 1, units = gridDim.x >> 1;
+    const uint32_t half = J.bn / 2, stage_bytes = TILE_BYTES + half * BK;
+    pdl_trigger();
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < J.stages; s++) {
+            mbar_init(&ctl.full[s], 1);
+            mbar_init(&ctl.empty[s], 1);
+            mbar_init(&ctl.peer_full[s], 1);
+        }
+        for (int b = 0; b < 2; b++) {
+            mbar_init(&ctl.acc_full[b], 1);
+            mbar_init(&ctl.acc_empty[b], 2 * EPILOGUE_WARPS);
+        }
+        mbar_init(&ctl.drained, 1);
+        ctl.abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&xmap) : "memory");
+    }
+    __syncthreads();
+    cluster_sync(); // both blocks run and their barriers are there
+    if (warp == 1) {
+        __syncwarp();
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl.tmem_base)), "r"(J.tmem_cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    cluster_sync(); // both have their accumulators
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *(volatile uint32_t *)&ctl.tmem_base;
+
+    if (warp == 0) {
+        if (elect_one()) {
+            auto weights = [&](const Place &p, uint32_t it) { return J.t[p.which].w + ((size_t)(2 * p.tile + rank) * J.k_blocks + it) * TILE_BYTES; };
+            const uint32_t primed = unit < J.items ? min(J.stages, J.k_blocks) : 0;
+            for (uint32_t it = 0; it < primed; it++) {
+                mbar_expect_tx(&ctl.full[it], TILE_BYTES + J.box_bytes);
+                bulk_load(ring + it * stage_bytes, weights(place_of(J, unit), it), TILE_BYTES, &ctl.full[it]);
+            }
+            pdl_wait();
+            uint32_t s = 0, phase = 0, issued = 0;
+            bool ok = true;
+            for (uint32_t item = unit; item < J.items && ok; item += units) {
+                const Place p = place_of(J, item);
+                for (uint32_t it = 0; it < J.k_blocks; it++) {
+                    if (issued >= primed) {
+                        if (!(ok = mbar_wait(&ctl.empty[s], phase ^ 1, &ctl, status))) break;
+                        mbar_expect_tx(&ctl.full[s], TILE_BYTES + J.box_bytes);
+                        bulk_load(ring + s * stage_bytes, weights(p, it), TILE_BYTES, &ctl.full[s]);
+                    }
+                    tma_load_2d(ring + s * stage_bytes + TILE_BYTES, &xmap, (int)(it * BK), (int)(p.m0 + rank * half), &ctl.full[s]);
+                    issued++;
+                    if (++s == J.stages) s = 0, phase ^= 1;
+                }
+            }
+            if (*(volatile uint32_t *)&ctl.abort_flag)
+                for (uint32_t ib = issued > J.stages ? issued - J.stages : 0; ib < issued; ib++)
+                    for (uint32_t i = 0; i < WAIT_LIMIT && !mbar_try(&ctl.full[ib % J.stages], (ib / J.stages) & 1); i++) {}
+        }
+    } else if (warp == 1) {
+        if (elect_one()) {
+            pdl_wait();
+            const uint32_t idesc = idesc_i8(2 * BM, J.bn);
+            uint32_t s = 0, phase = 0, buf = 0, buf_phase = 0;
+            bool ok = true;
+            for (uint32_t item = unit; item < J.items && ok; item += units) {
+                if (rank == 0 && !(ok = mbar_wait(&ctl.acc_empty[buf], buf_phase ^ 1, &ctl, status))) break;
+                const uint32_t acc = tmem + buf * J.bn;
+                for (uint32_t it = 0; it < J.k_blocks; it++) {
+                    if (!(ok = mbar_wait(&ctl.full[s], phase, &ctl, status))) break;
+                    if (rank != 0) {
+                        mbar_arrive_at(&ctl.peer_full[s], 0);
+                    } else {
+                        if (!(ok = mbar_wait(&ctl.peer_full[s], phase, &ctl, status))) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        const uint32_t at = smem_u32(ring + s * stage_bytes);
+                        const uint64_t a = umma_desc(at), b = umma_desc(at + TILE_BYTES);
+#pragma unroll
+                        for (uint32_t k = 0; k < BK / 32; k++) umma_i8_pair(acc, a + 2 * k, b + 2 * k, idesc, (it | k) != 0);
+                        umma_commit_pair(&ctl.empty[s]);
+                    }
+                    if (++s == J.stages) s = 0, phase ^= 1;
+                }
+                if (ok && rank == 0) umma_commit_pair(&ctl.acc_full[buf]);
+                if (++buf == 2) buf = 0, buf_phase ^= 1;
+            }
+            if (rank == 0) { // everything this thread issued has finished before either block goes on to its end
+                asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(&ctl.drained)) : "memory");
+                for (uint32_t i = 0; i < WAIT_LIMIT && !mbar_try(&ctl.drained, 0, WAIT_HINT_NS); i++) {}
+            }
+        }
+    } else {
+        pdl_wait();
+        const uint32_t quarter = warp & 3;
+        uint32_t buf = 0, buf_phase = 0;
+        for (uint32_t item = unit; item < J.items; item += units) {
+            const Place p = place_of(J, item);
+            const Target &T = J.t[p.which];
+            const uint32_t row = (2 * p.tile + rank) * BM + 32 * quarter + lane, live = min(J.bn, J.m - p.m0);
+            const float ws = row < T.rows ? T.scales[row] : 0.f;
+            if (!__all_sync(0xffffffffu, mbar_wait(&ctl.acc_full[buf], buf_phase, &ctl, status))) break; // the warp agrees
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            store_tile(J, T, tmem + buf * J.bn + ((32 * quarter) << 16), p.m0, live, row, ws, lane);
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive_at(&ctl.acc_empty[buf], 0);
+            if (++buf == 2) buf = 0, buf_phase ^= 1;
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    cluster_sync(); // no MMA reads, and no arrival is on its way to, a block that is gone
+    if (warp == 1) {
+        __syncwarp();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(J.tmem_cols) : "memory");
+    }
+}
+
 // A matrix of rows of `cols` bytes as swizzled tiles: 16 bytes a thread, zero past the matrix's end.
 __global__ void __launch_bounds__(256) k_tile_i8(const uint8_t *__restrict__ src, uint64_t rows, uint64_t cols, uint32_t k_blocks,
                                                         uint8_t *__restrict__ dst) {
@@ -299,39 +445,70 @@ __global__ void __launch_bounds__(256) k_tile_i8(const uint8_t *__restrict__ src
     *reinterpret_cast<uint4 *>(dst + (tile << 14) + r * 128 + chunk * 16) = v;
 }
 
-// How a product is cut: tokens of a tile, and the blocks among which an item's K is shared.
+// How a product is cut: tokens of a tile, the blocks among which an item's K is shared, blocks per SM, pairs or single blocks.
 struct Plan {
     uint32_t bn, token_tiles, slices, per, stages, per_sm;
+    bool pair;
 };
-Plan plan(uint32_t row_tiles, uint32_t k_blocks, uint32_t m, uint32_t sms) {
+Plan plan(const fq_matrix *const *w, uint32_t count, uint32_t k_blocks, uint32_t m, uint32_t sms) {
+    uint32_t tiles = 0, pairs = 0;
+    for (uint32_t i = 0; i < count; i++) {
+        tiles += (uint32_t)((w[i]->rows + BM - 1) / BM);
+        pairs += (uint32_t)((w[i]->rows + 2 * BM - 1) / (2 * BM));
+    }
     Plan p{};
-    p.token_tiles = (m + 255) / 256;
-    p.bn = ((m + p.token_tiles - 1) / p.token_tiles + 15) / 16 * 16;
-    p.token_tiles = (m + p.bn - 1) / p.bn;
-    p.per_sm = p.bn <= 64 ? 2 : 1;
-    const uint32_t items = row_tiles * p.token_tiles, slots = sms * p.per_sm;
-    p.slices = std::max(1u, std::min({slots / items, MAX_SLICES, k_blocks}));
-    p.per = (k_blocks + p.slices - 1) / p.slices;
-    p.slices = (k_blocks + p.per - 1) / p.per; // no slice is left without work
-    p.stages = std::min((SMEM_MAX / p.per_sm - 3072) / (TILE_BYTES + p.bn * BK), MAX_STAGES);
+    double best = 0.0;
+    auto round16 = [](uint32_t v, uint32_t to) { return (v + to - 1) / to * to; };
+    auto consider = [&](uint32_t token_tiles, bool pair, uint32_t slices) {
+        Plan c{};
+        c.pair = pair;
+        c.bn = round16((m + token_tiles - 1) / token_tiles, pair ? 32 : 16);
+        if (c.bn > 256) return;
+        c.token_tiles = (m + c.bn - 1) / c.bn;
+        c.per_sm = m <= 64 ? 2 : 1;
+        const uint32_t items = (pair ? pairs : tiles) * c.token_tiles, slots = pair ? sms / 2 : sms * c.per_sm;
+        c.per = (k_blocks + slices - 1) / slices;
+        c.slices = (k_blocks + c.per - 1) / c.per; // no slice is left without work
+        if (c.slices > 1 && items * c.slices > slots) return;
+        // Clocks of a k-block on an SM: its MMAs (measured, profiles/tcgen05_mma_rate.md), or what it takes in at 44 bytes a clock,
+        // the rate at which all SMs together are fed from L2.
+        const double mma = 4.0 * std::max(32.0 + c.bn / 4.0, c.bn / 2.0), feed = (TILE_BYTES + (pair ? c.bn / 2 : c.bn) * BK) / 44.0;
+        const double rounds = (items + slots - 1) / slots;
+        const double cost = rounds * (c.per * std::max(mma, feed) + 4.0 * c.bn) + (c.slices > 1 ? 2000.0 + 8.0 * c.bn : 0.0) + (pair ? 1000.0 : 0.0);
+        if (p.bn == 0 || cost < best) {
+            best = cost;
+            p = c;
+        }
+    };
+    if (m <= 64) { // as much of the weights under way as the machine holds
+        consider(1, false, std::max(1u, std::min({2 * sms / tiles, MAX_SLICES, k_blocks})));
+    } else {
+        for (uint32_t t = (m + 255) / 256; t <= (m + 255) / 256 + 7 && t <= (m + 15) / 16; t++) {
+            for (uint32_t slices = 1; slices <= std::min(MAX_SLICES, k_blocks); slices++) consider(t, false, slices);
+            consider(t, true, 1);
+        }
+    }
+    p.stages = std::min((SMEM_MAX / p.per_sm - 3072) / (TILE_BYTES + (p.pair ? p.bn / 2 : p.bn) * BK), MAX_STAGES);
     return p;
 }
 
 // Once per handle's device: the kernels may use all of an SM's shared memory.
 cudaError_t allow_shared_memory() {
-    cudaError_t e = cudaFuncSetAttribute(k_gemm_i8<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(SMEM_MAX - 2048));
-    return e != cudaSuccess ? e : cudaFuncSetAttribute(k_gemm_i8<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(SMEM_MAX - 2048));
+    for (auto kernel : {k_gemm_i8<false>, k_gemm_i8<true>, k_gemm_i8_pair})
+        if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(SMEM_MAX - 2048))) return e;
+    return cudaSuccess;
 }
 
 int launch(fq_device *dev, const fq_matrix *const *w, uint32_t count, const int8_t *x, const float *x_scales, uint32_t m, void *const *y, int y_dtype) {
     const uint32_t cols = (uint32_t)w[0]->cols, k_blocks = (cols + BK - 1) / BK;
+    const Plan p = plan(w, count, k_blocks, m, (uint32_t)dev->sm_count);
     Job J{};
-    uint32_t tiles = 0;
+    uint32_t tiles = 0; // of 128 rows, or for pairs of 256
     for (uint32_t i = 0; i < count; i++) {
-        tiles += (uint32_t)((w[i]->rows + BM - 1) / BM);
+        const uint32_t bm = p.pair ? 2 * BM : BM;
+        tiles += (uint32_t)((w[i]->rows + bm - 1) / bm);
         J.t[i] = {w[i]->data, w[i]->scales, y[i], (uint32_t)w[i]->rows, tiles};
     }
-    const Plan p = plan(tiles, k_blocks, m, (uint32_t)dev->sm_count);
     J.x_scales = x_scales;
     J.count = count;
     J.m = m;
@@ -347,7 +524,7 @@ int launch(fq_device *dev, const fq_matrix *const *w, uint32_t count, const int8
     EncodeTiled encode = encode_fn();
     if (!encode) return fq_fail(dev, FQ_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
     CUtensorMap map;
-    const uint32_t box_rows = std::min(m, p.bn);
+    const uint32_t box_rows = std::min(m, p.pair ? p.bn / 2 : p.bn);
     const cuuint64_t dims[2] = {cols, m}, strides[1] = {cols};
     const cuuint32_t box[2] = {BK, box_rows}, step[2] = {1, 1};
     const CUresult r = encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t *>(x), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -355,9 +532,10 @@ int launch(fq_device *dev, const fq_matrix *const *w, uint32_t count, const int8
     if (r != CUDA_SUCCESS) return fq_fail(dev, FQ_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
     J.box_bytes = box_rows * BK;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(p.slices > 1 ? J.items * p.slices : std::min(J.items, (uint32_t)dev->sm_count * p.per_sm));
+    const uint32_t sms = (uint32_t)dev->sm_count;
+    cfg.gridDim = dim3(p.pair ? 2 * std::min(J.items, sms / 2) : p.slices > 1 ? J.items * p.slices : std::min(J.items, sms * p.per_sm));
     cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = 1024 + p.stages * (TILE_BYTES + p.bn * BK);
+    cfg.dynamicSmemBytes = 1024 + p.stages * (TILE_BYTES + (p.pair ? p.bn / 2 : p.bn) * BK);
     cfg.stream = dev->stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -367,7 +545,7 @@ int launch(fq_device *dev, const fq_matrix *const *w, uint32_t count, const int8
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = p.slices > 1 ? 2 : 1;
-    const cudaError_t e = p.slices > 1 ? cudaLaunchKernelEx(&cfg, k_gemm_i8<true>, map, J, dev->status_dev) : cudaLaunchKernelEx(&cfg, k_gemm_i8<false>, map, J, dev->status_dev);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, p.pair ? k_gemm_i8_pair : p.slices > 1 ? k_gemm_i8<true> : k_gemm_i8<false>, map, J, dev->status_dev);
     return fq_check_cuda(dev, e, "8-bit projection launch");
 }
 
@@ -404,7 +582,7 @@ extern "C" int fq_matrix_create_i8(fq_device *dev, uint64_t rows, uint64_t cols,
     w->byte_size = rows * (cols + 4);
     w->block_elems = w->block_bytes = 1;
     const uint32_t k_blocks = (uint32_t)((cols + BK - 1) / BK);
-    const uint64_t tiles = (rows + BM - 1) / BM * k_blocks;
+    const uint64_t tiles = (rows + 2 * BM - 1) / (2 * BM) * 2 * k_blocks; // an even number of row tiles, for pairs of blocks
     const size_t len = tiles * TILE_BYTES;
     // The tiles are laid out on the device; rows in host memory (or off their 16 bytes) go through a copy of their own.
     uint8_t *staged = nullptr;

@@ -417,15 +417,15 @@ class Matrix:
             pass
 
 
-def _ptr(t: Optional[torch.Tensor]) -> C.c_void_p:
-    return C.c_void_p(0 if t is None else t.data_ptr())
+def _ptr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _need(d: Device, *tensors: torch.Tensor) -> None:
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda or t.device != d.torch_device:
+        if t.get_device() != d.ordinal:  # -1 on the CPU
             raise DeviceMismatch(f"tensor on {t.device}, device handle on {d.torch_device}")
         if not t.is_contiguous():
             raise ShapeError("tensor is not contiguous")
