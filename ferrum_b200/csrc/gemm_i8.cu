@@ -19,6 +19,7 @@
 // block r of the cluster collects and stores the tokens of its share.  All waits are bounded (tcgen05.cuh).
 #include <algorithm>
 #include <cmath>
+#include <cstring>
 #include <vector>
 
 #include "gemv_common.cuh"
@@ -37,6 +38,7 @@ constexpr uint32_t MAX_STAGES = 12;
 constexpr uint32_t MAX_MANY = 8, MAX_SLICES = 8;
 constexpr uint32_t EPILOGUE_WARPS = 4, THREADS = (2 + EPILOGUE_WARPS) * 32;
 constexpr uint32_t SMEM_MAX = 227 * 1024;
+constexpr uint64_t DRAIN_NS = 200000;
 
 struct Target {
     const uint8_t *w; // tiles
@@ -59,7 +61,7 @@ struct Job {
 };
 
 struct Ctl {
-    uint64_t full[MAX_STAGES], empty[MAX_STAGES], peer_full[MAX_STAGES], acc_full[2], acc_empty[2], drained;
+    uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc_full[2], acc_empty[2], drained;
     uint32_t tmem_base, abort_flag;
 };
 
@@ -111,6 +113,8 @@ __device__ __forceinline__ Place place_of(const Job &J, uint32_t item) {
     return p;
 }
 
+__device__ __forceinline__ void put(float *p, float v) { *p = v; }
+__device__ __forceinline__ void put(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void store_value(const Job &J, const Target &T, uint32_t token, uint32_t row, int acc, float xs, float ws) {
     const float v = (float)acc * xs * ws;
     const size_t at = (size_t)token * T.rows + row;
@@ -118,19 +122,32 @@ __device__ __forceinline__ void store_value(const Job &J, const Target &T, uint3
     else static_cast<float *>(T.y)[at] = v;
 }
 
+// The scales of a token tile, in shared memory of the warp's own; asked for before the accumulator is waited for.
+__device__ __forceinline__ void stage_scales(const Job &J, uint32_t m0, uint32_t live, float *xs, uint32_t lane) {
+    __syncwarp(); // the tile before has been stored
+    for (uint32_t c = lane; c < live; c += 32) xs[c] = __ldcg(J.x_scales + m0 + c);
+    __syncwarp();
+}
 // `live` tokens from m0 of the accumulator at `acc`: one weight row a lane, so that a warp's stores of a token are contiguous.
-__device__ __forceinline__ void store_tile(const Job &J, const Target &T, uint32_t acc, uint32_t m0, uint32_t live, uint32_t row, float ws, uint32_t lane) {
+template <typename YT>
+__device__ __forceinline__ void store_rows(YT *y, uint32_t rows, uint32_t acc, uint32_t live, bool in, float ws, const float *xs) {
     for (uint32_t c0 = 0; c0 < live; c0 += 16) {
-        const uint32_t mine = c0 + (lane & 15);
-        const float xs = mine < live ? __ldcg(J.x_scales + m0 + mine) : 0.f;
         int v[16];
         tmem_ld16(acc + c0, v);
+        if (!in) continue;
+        const float4 *x4 = reinterpret_cast<const float4 *>(xs + c0);
 #pragma unroll
         for (uint32_t c = 0; c < 16; c++) {
-            const float f = __shfl_sync(0xffffffffu, xs, c);
-            if (row < T.rows && c0 + c < live) store_value(J, T, m0 + c0 + c, row, v[c], f, ws);
+            const float4 x = x4[c / 4];
+            if (c0 + c < live) put(y, (float)v[c] * (c % 4 == 0 ? x.x : c % 4 == 1 ? x.y : c % 4 == 2 ? x.z : x.w) * ws);
+            y += rows;
         }
     }
+}
+__device__ __forceinline__ void store_tile(const Job &J, const Target &T, uint32_t acc, uint32_t m0, uint32_t live, uint32_t row, float ws, const float *xs) {
+    const size_t at = (size_t)m0 * T.rows + row;
+    if (J.bf16) store_rows(static_cast<__nv_bfloat16 *>(T.y) + at, T.rows, acc, live, row < T.rows, ws, xs);
+    else store_rows(static_cast<float *>(T.y) + at, T.rows, acc, live, row < T.rows, ws, xs);
 }
 
 template <bool SLICED>
@@ -138,6 +155,7 @@ __global__ void __launch_bounds__(THREADS)
 k_gemm_i8(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ Job J, int *status) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ Ctl ctl;
+    __shared__ __align__(16) float xs[EPILOGUE_WARPS][256];
     uint8_t *ring = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, stage_bytes = TILE_BYTES + J.bn * BK;
     const uint32_t slice = SLICED ? blockIdx.x % J.slices : 0, unit = SLICED ? blockIdx.x / J.slices : blockIdx.x, units = SLICED ? gridDim.x / J.slices : gridDim.x;
@@ -238,9 +256,10 @@ k_gemm_i8(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ Job 
                 const Target &T = J.t[p.which];
                 const uint32_t row = p.tile * BM + 32 * quarter + lane, live = min(J.bn, J.m - p.m0);
                 const float ws = row < T.rows ? T.scales[row] : 0.f;
+                stage_scales(J, p.m0, live, xs[quarter], lane);
                 if (!__all_sync(0xffffffffu, mbar_wait(&ctl.acc_full[buf], buf_phase, &ctl, status))) break; // the warp agrees
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                store_tile(J, T, tmem + buf * J.bn + ((32 * quarter) << 16), p.m0, live, row, ws, lane);
+                store_tile(J, T, tmem + buf * J.bn + ((32 * quarter) << 16), p.m0, live, row, ws, xs[quarter]);
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 mbar_arrive(&ctl.acc_empty[buf]);
                 if (++buf == 2) buf = 0, buf_phase ^= 1;
@@ -296,9 +315,17 @@ k_gemm_i8(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ Job 
 // the tokens in its shared memory, and the sums of its own rows in its tensor memory.  A block then takes in 16 KB of weights
 // and only half of a token tile for as many products, and what it takes in per product is what binds the kernel above.
 //
-// The even block issues the MMAs.  It learns that the other block's stage is full from that block's warp 1, which waits for it
-// and passes the arrival on; the commits that release a stage and hand over an accumulator arrive in both blocks; both blocks'
-// epilogues return the accumulator to the even one.
+// The even block issues the MMAs.  Both blocks' copies report to its barriers (TMA with .cta_group::2; through a thread of the
+// other block that waits and passes the arrival on, gate|up of 2048 rows took 50 instead of 48 us for 509 rows of 17408); the commits that release a
+// stage and hand over an accumulator arrive in both blocks; both blocks' epilogues return the accumulator to the even one.
+struct PairMaps {
+    CUtensorMap x, w[MAX_MANY]; // tokens; the tiles of each matrix as rows of 128 bytes
+};
+__device__ __forceinline__ void tma_load_pair(void *dst, const CUtensorMap *map, int x, int y, uint32_t bar) { // bar: cluster address
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(bar)
+                 : "memory");
+}
 __device__ __forceinline__ void umma_i8_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
     asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}"
                  ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
@@ -312,9 +339,10 @@ __device__ __forceinline__ void mbar_arrive_at(uint64_t *bar, uint32_t rank) { /
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_address(smem_u32(bar), rank)) : "memory");
 }
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS)
-k_gemm_i8_pair(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ Job J, int *status) {
+k_gemm_i8_pair(const __grid_constant__ PairMaps maps, const __grid_constant__ Job J, int *status) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ Ctl ctl;
+    __shared__ __align__(16) float xs[EPILOGUE_WARPS][256];
     uint8_t *ring = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023); // the same place in both blocks
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = blockIdx.x & 1, unit = blockIdx.x >> 1, units = gridDim.x >> 1;
     const uint32_t half = J.bn / 2, stage_bytes = TILE_BYTES + half * BK;
@@ -323,7 +351,6 @@ k_gemm_i8_pair(const __grid_constant__ CUtensorMap xmap, const __grid_constant__
         for (uint32_t s = 0; s < J.stages; s++) {
             mbar_init(&ctl.full[s], 1);
             mbar_init(&ctl.empty[s], 1);
-            mbar_init(&ctl.peer_full[s], 1);
         }
         for (int b = 0; b < 2; b++) {
             mbar_init(&ctl.acc_full[b], 1);
@@ -332,7 +359,7 @@ k_gemm_i8_pair(const __grid_constant__ CUtensorMap xmap, const __grid_constant__
         mbar_init(&ctl.drained, 1);
         ctl.abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        asm volatile("prefetch.tensormap [%0];" ::"l"(&xmap) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.x) : "memory");
     }
     __syncthreads();
     cluster_sync(); // both blocks run and their barriers are there
@@ -349,12 +376,13 @@ k_gemm_i8_pair(const __grid_constant__ CUtensorMap xmap, const __grid_constant__
 
     if (warp == 0) {
         if (elect_one()) {
-            auto weights = [&](const Place &p, uint32_t it) { return J.t[p.which].w + ((size_t)(2 * p.tile + rank) * J.k_blocks + it) * TILE_BYTES; };
+            const uint32_t both = 2 * (TILE_BYTES + J.box_bytes);
+            auto weights = [&](const Place &p, uint32_t it, uint32_t s) {
+                if (rank == 0) mbar_expect_tx(&ctl.full[s], both); // (the other block's copies may report before)
+                tma_load_pair(ring + s * stage_bytes, &maps.w[p.which], 0, (int)(((2 * p.tile + rank) * J.k_blocks + it) * BM), cluster_address(smem_u32(&ctl.full[s]), 0));
+            };
             const uint32_t primed = unit < J.items ? min(J.stages, J.k_blocks) : 0;
-            for (uint32_t it = 0; it < primed; it++) {
-                mbar_expect_tx(&ctl.full[it], TILE_BYTES + J.box_bytes);
-                bulk_load(ring + it * stage_bytes, weights(place_of(J, unit), it), TILE_BYTES, &ctl.full[it]);
-            }
+            for (uint32_t it = 0; it < primed; it++) weights(place_of(J, unit), it, it);
             pdl_wait();
             uint32_t s = 0, phase = 0, issued = 0;
             bool ok = true;
@@ -363,49 +391,42 @@ k_gemm_i8_pair(const __grid_constant__ CUtensorMap xmap, const __grid_constant__
                 for (uint32_t it = 0; it < J.k_blocks; it++) {
                     if (issued >= primed) {
                         if (!(ok = mbar_wait(&ctl.empty[s], phase ^ 1, &ctl, status))) break;
-                        mbar_expect_tx(&ctl.full[s], TILE_BYTES + J.box_bytes);
-                        bulk_load(ring + s * stage_bytes, weights(p, it), TILE_BYTES, &ctl.full[s]);
+                        weights(p, it, s);
                     }
-                    tma_load_2d(ring + s * stage_bytes + TILE_BYTES, &xmap, (int)(it * BK), (int)(p.m0 + rank * half), &ctl.full[s]);
+                    tma_load_pair(ring + s * stage_bytes + TILE_BYTES, &maps.x, (int)(it * BK), (int)(p.m0 + rank * half), cluster_address(smem_u32(&ctl.full[s]), 0));
                     issued++;
                     if (++s == J.stages) s = 0, phase ^= 1;
                 }
             }
+            // After an abort the copies under way still land, some of them reporting to the other block: they are given time.
             if (*(volatile uint32_t *)&ctl.abort_flag)
-                for (uint32_t ib = issued > J.stages ? issued - J.stages : 0; ib < issued; ib++)
-                    for (uint32_t i = 0; i < WAIT_LIMIT && !mbar_try(&ctl.full[ib % J.stages], (ib / J.stages) & 1); i++) {}
+                for (const uint64_t t0 = now_ns(); now_ns() - t0 < DRAIN_NS;) {}
         }
     } else if (warp == 1) {
-        if (elect_one()) {
+        if (rank == 0 && elect_one()) {
             pdl_wait();
             const uint32_t idesc = idesc_i8(2 * BM, J.bn);
             uint32_t s = 0, phase = 0, buf = 0, buf_phase = 0;
             bool ok = true;
             for (uint32_t item = unit; item < J.items && ok; item += units) {
-                if (rank == 0 && !(ok = mbar_wait(&ctl.acc_empty[buf], buf_phase ^ 1, &ctl, status))) break;
+                if (!mbar_wait(&ctl.acc_empty[buf], buf_phase ^ 1, &ctl, status)) break;
                 const uint32_t acc = tmem + buf * J.bn;
                 for (uint32_t it = 0; it < J.k_blocks; it++) {
                     if (!(ok = mbar_wait(&ctl.full[s], phase, &ctl, status))) break;
-                    if (rank != 0) {
-                        mbar_arrive_at(&ctl.peer_full[s], 0);
-                    } else {
-                        if (!(ok = mbar_wait(&ctl.peer_full[s], phase, &ctl, status))) break;
-                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        const uint32_t at = smem_u32(ring + s * stage_bytes);
-                        const uint64_t a = umma_desc(at), b = umma_desc(at + TILE_BYTES);
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t at = smem_u32(ring + s * stage_bytes);
+                    const uint64_t a = umma_desc(at), b = umma_desc(at + TILE_BYTES);
 #pragma unroll
-                        for (uint32_t k = 0; k < BK / 32; k++) umma_i8_pair(acc, a + 2 * k, b + 2 * k, idesc, (it | k) != 0);
-                        umma_commit_pair(&ctl.empty[s]);
-                    }
+                    for (uint32_t k = 0; k < BK / 32; k++) umma_i8_pair(acc, a + 2 * k, b + 2 * k, idesc, (it | k) != 0);
+                    umma_commit_pair(&ctl.empty[s]);
                     if (++s == J.stages) s = 0, phase ^= 1;
                 }
-                if (ok && rank == 0) umma_commit_pair(&ctl.acc_full[buf]);
+                if (ok) umma_commit_pair(&ctl.acc_full[buf]);
                 if (++buf == 2) buf = 0, buf_phase ^= 1;
             }
-            if (rank == 0) { // everything this thread issued has finished before either block goes on to its end
-                asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(&ctl.drained)) : "memory");
-                for (uint32_t i = 0; i < WAIT_LIMIT && !mbar_try(&ctl.drained, 0, WAIT_HINT_NS); i++) {}
-            }
+            // Everything this thread issued has finished before either block goes on to its end.
+            asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(&ctl.drained)) : "memory");
+            for (uint32_t i = 0; i < WAIT_LIMIT && !mbar_try(&ctl.drained, 0, WAIT_HINT_NS); i++) {}
         }
     } else {
         pdl_wait();
@@ -416,9 +437,10 @@ k_gemm_i8_pair(const __grid_constant__ CUtensorMap xmap, const __grid_constant__
             const Target &T = J.t[p.which];
             const uint32_t row = (2 * p.tile + rank) * BM + 32 * quarter + lane, live = min(J.bn, J.m - p.m0);
             const float ws = row < T.rows ? T.scales[row] : 0.f;
+            stage_scales(J, p.m0, live, xs[quarter], lane);
             if (!__all_sync(0xffffffffu, mbar_wait(&ctl.acc_full[buf], buf_phase, &ctl, status))) break; // the warp agrees
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            store_tile(J, T, tmem + buf * J.bn + ((32 * quarter) << 16), p.m0, live, row, ws, lane);
+            store_tile(J, T, tmem + buf * J.bn + ((32 * quarter) << 16), p.m0, live, row, ws, xs[quarter]);
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive_at(&ctl.acc_empty[buf], 0);
@@ -488,15 +510,26 @@ Plan plan(const fq_matrix *const *w, uint32_t count, uint32_t k_blocks, uint32_t
             consider(t, true, 1);
         }
     }
-    p.stages = std::min((SMEM_MAX / p.per_sm - 3072) / (TILE_BYTES + (p.pair ? p.bn / 2 : p.bn) * BK), MAX_STAGES);
+    p.stages = std::min((SMEM_MAX / p.per_sm - 8192) / (TILE_BYTES + (p.pair ? p.bn / 2 : p.bn) * BK), MAX_STAGES);
     return p;
 }
 
 // Once per handle's device: the kernels may use all of an SM's shared memory.
 cudaError_t allow_shared_memory() {
-    for (auto kernel : {k_gemm_i8<false>, k_gemm_i8<true>, k_gemm_i8_pair})
-        if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(SMEM_MAX - 2048))) return e;
+    for (const void *kernel : {(const void *)k_gemm_i8<false>, (const void *)k_gemm_i8<true>, (const void *)k_gemm_i8_pair})
+        if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(SMEM_MAX - 6144))) return e;
     return cudaSuccess;
+}
+
+// Rows of `cols` bytes for boxes of 128 bytes of `box_rows` rows.
+int encode_bytes(fq_device *dev, CUtensorMap *map, const void *p, uint64_t cols, uint64_t rows, uint32_t box_rows, CUtensorMapSwizzle swizzle) {
+    EncodeTiled encode = encode_fn();
+    if (!encode) return fq_fail(dev, FQ_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
+    const cuuint64_t dims[2] = {cols, rows}, strides[1] = {cols};
+    const cuuint32_t box[2] = {BK, box_rows}, step[2] = {1, 1};
+    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? FQ_OK : fq_fail(dev, FQ_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
 }
 
 int launch(fq_device *dev, const fq_matrix *const *w, uint32_t count, const int8_t *x, const float *x_scales, uint32_t m, void *const *y, int y_dtype) {
@@ -521,15 +554,9 @@ int launch(fq_device *dev, const fq_matrix *const *w, uint32_t count, const int8
     J.stages = p.stages;
     J.bf16 = y_dtype == FQ_BF16;
     for (J.tmem_cols = 32; J.tmem_cols < 2 * p.bn;) J.tmem_cols *= 2;
-    EncodeTiled encode = encode_fn();
-    if (!encode) return fq_fail(dev, FQ_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
     CUtensorMap map;
     const uint32_t box_rows = std::min(m, p.pair ? p.bn / 2 : p.bn);
-    const cuuint64_t dims[2] = {cols, m}, strides[1] = {cols};
-    const cuuint32_t box[2] = {BK, box_rows}, step[2] = {1, 1};
-    const CUresult r = encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t *>(x), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return fq_fail(dev, FQ_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    if (int rc = encode_bytes(dev, &map, x, cols, m, box_rows, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
     J.box_bytes = box_rows * BK;
     cudaLaunchConfig_t cfg{};
     const uint32_t sms = (uint32_t)dev->sm_count;
@@ -545,7 +572,15 @@ int launch(fq_device *dev, const fq_matrix *const *w, uint32_t count, const int8
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = p.slices > 1 ? 2 : 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, p.pair ? k_gemm_i8_pair : p.slices > 1 ? k_gemm_i8<true> : k_gemm_i8<false>, map, J, dev->status_dev);
+    cudaError_t e;
+    if (p.pair) {
+        PairMaps maps;
+        maps.x = map;
+        for (uint32_t i = 0; i < count; i++) memcpy(&maps.w[i], w[i]->tile_map, sizeof(CUtensorMap));
+        e = cudaLaunchKernelEx(&cfg, k_gemm_i8_pair, maps, J, dev->status_dev);
+    } else {
+        e = cudaLaunchKernelEx(&cfg, p.slices > 1 ? k_gemm_i8<true> : k_gemm_i8<false>, map, J, dev->status_dev);
+    }
     return fq_check_cuda(dev, e, "8-bit projection launch");
 }
 
@@ -602,10 +637,13 @@ extern "C" int fq_matrix_create_i8(fq_device *dev, uint64_t rows, uint64_t cols,
     if (e == cudaSuccess) e = cudaMemcpyAsync(w->scales, host.data(), rows * 4, cudaMemcpyHostToDevice, dev->stream);
     if (e == cudaSuccess) e = cudaStreamSynchronize(dev->stream);
     if (staged) cudaFree(staged);
-    if (e != cudaSuccess) {
+    int rc = fq_check_cuda(dev, e, "weight upload");
+    static_assert(sizeof(CUtensorMap) == sizeof w->tile_map, "fq_matrix holds a tensor map");
+    if (!rc) rc = encode_bytes(dev, (CUtensorMap *)w->tile_map, w->data, BK, tiles * BM, BM, CU_TENSOR_MAP_SWIZZLE_NONE);
+    if (rc) {
         if (w->data) cudaFree(w->data);
         delete w;
-        return fq_check_cuda(dev, e, "weight upload");
+        return rc;
     }
     dev->counters.bytes_uploaded += w->byte_size;
     *out = w;

@@ -96,6 +96,7 @@ struct fq_matrix {
     uint32_t block_elems = 0, block_bytes = 0;
     uint8_t *data = nullptr; // device copy of the blocks in the device layout
     float *scales = nullptr; // FQ_I8: one per row, in the allocation of `data`
+    alignas(64) unsigned char tile_map[128]; // FQ_I8: CUtensorMap of `data` as rows of 128 bytes
     uint64_t expert_rows() const { return rows / experts; }
 };
 
