@@ -16,7 +16,8 @@
 //
 // Blocks walk (row tile, token tile) items.  Where there are fewer items than blocks the machine holds, a cluster of up to
 // eight blocks cuts an item's K and adds the partial sums (whole numbers, so in any order) through distributed shared memory:
-// block r of the cluster collects and stores the tokens of its share.  All waits are bounded (tcgen05.cuh).
+// block r of the cluster collects and stores the tokens of its share, which the others send as one bulk copy each (value by
+// value, remote stores took 45 instead of XXX us for q|k|v of 128 rows).  All waits are bounded (tcgen05.cuh).
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -61,7 +62,7 @@ struct Job {
 };
 
 struct Ctl {
-    uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc_full[2], acc_empty[2], drained;
+    uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc_full[2], acc_empty[2], drained, received;
     uint32_t tmem_base, abort_flag;
 };
 
@@ -89,7 +90,11 @@ __device__ __forceinline__ uint32_t cluster_address(uint32_t saddr, uint32_t ran
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
     return r;
 }
-__device__ __forceinline__ void store_cluster(uint32_t addr, int v) { asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
+// From this block's shared memory to another's, whose barrier learns of it (cluster addresses).
+__device__ __forceinline__ void bulk_send(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "r"(smem_u32(src)), "r"(bytes), "r"(bar)
+                 : "memory");
+}
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
 }
@@ -115,13 +120,6 @@ __device__ __forceinline__ Place place_of(const Job &J, uint32_t item) {
 
 __device__ __forceinline__ void put(float *p, float v) { *p = v; }
 __device__ __forceinline__ void put(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }
-__device__ __forceinline__ void store_value(const Job &J, const Target &T, uint32_t token, uint32_t row, int acc, float xs, float ws) {
-    const float v = (float)acc * xs * ws;
-    const size_t at = (size_t)token * T.rows + row;
-    if (J.bf16) static_cast<__nv_bfloat16 *>(T.y)[at] = __float2bfloat16_rn(v);
-    else static_cast<float *>(T.y)[at] = v;
-}
-
 // The scales of a token tile, in shared memory of the warp's own; asked for before the accumulator is waited for.
 __device__ __forceinline__ void stage_scales(const Job &J, uint32_t m0, uint32_t live, float *xs, uint32_t lane) {
     __syncwarp(); // the tile before has been stored
@@ -171,6 +169,7 @@ k_gemm_i8(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ Job 
             mbar_init(&ctl.acc_empty[b], EPILOGUE_WARPS * 32);
         }
         mbar_init(&ctl.drained, 1);
+        mbar_init(&ctl.received, 1);
         ctl.abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&xmap) : "memory");
@@ -269,42 +268,46 @@ k_gemm_i8(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ Job 
         const Place p = place_of(J, unit);
         const Target &T = J.t[p.which];
         const uint32_t live = min(J.bn, J.m - p.m0), share = (live + J.slices - 1) / J.slices;
-        const uint32_t mine = slice * share, mine_end = min(live, mine + share), acc = tmem + ((32 * quarter) << 16);
-        if (warp >= 2 && mbar_wait(&ctl.acc_full[0], 0, &ctl, status)) asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t mine = min(live, slice * share), mine_end = min(live, mine + share), acc = tmem + ((32 * quarter) << 16);
+        const uint32_t row = p.tile * BM + 32 * quarter + lane;
+        int *sums = reinterpret_cast<int *>(ring) + 32 * quarter + lane, *others = sums + J.bn * BM; // [token][row]; [block][token][row]
+        float ws = 0.f;
+        if (threadIdx.x == 0 && mine_end > mine) mbar_expect_tx(&ctl.received, (J.slices - 1) * (mine_end - mine) * BM * 4);
+        if (warp >= 2) {
+            if (row < T.rows) ws = T.scales[row];
+            stage_scales(J, p.m0, live, xs[quarter], lane);
+            if (mbar_wait(&ctl.acc_full[0], 0, &ctl, status)) asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        }
         __syncthreads();
-        cluster_sync(); // every block's MMAs have read their ring (or given up): it takes the partial sums now
+        cluster_sync(); // every block's MMAs have read their ring (or given up): it takes the sums now
         if (warp >= 2 && *(volatile uint32_t *)&ctl.abort_flag == 0) {
             for (uint32_t c0 = 0; c0 < live; c0 += 16) {
                 int v[16];
                 tmem_ld16(acc + c0, v);
 #pragma unroll
-                for (uint32_t c = 0; c < 16; c++) {
-                    const uint32_t col = c0 + c, owner = col / share;
-                    if (col >= live || owner == slice) continue;
-                    const uint32_t from = slice < owner ? slice : slice - 1;
-                    store_cluster(cluster_address(smem_u32(ring), owner) + ((from * share + col - owner * share) * BM + 32 * quarter + lane) * 4, v[c]);
-                }
+                for (uint32_t c = 0; c < 16; c++)
+                    if (c0 + c < live) sums[(c0 + c) * BM] = v[c];
             }
+            asm volatile("fence.proxy.async.shared::cta;\nbar.sync 1, 128;" ::: "memory");
+            if (threadIdx.x == 64)
+                for (uint32_t to = 0; to < J.slices; to++) {
+                    const uint32_t first = min(live, to * share), n = min(live, first + share) - first;
+                    if (to == slice || n == 0) continue;
+                    const uint32_t from = slice < to ? slice : slice - 1;
+                    bulk_send(cluster_address(smem_u32(ring), to) + (J.bn + from * share) * BM * 4, ring + first * BM * 4, n * BM * 4, cluster_address(smem_u32(&ctl.received), to));
+                }
+            if (mine_end > mine && mbar_wait(&ctl.received, 0, &ctl, status) && row < T.rows)
+                for (uint32_t c = mine; c < mine_end; c++) {
+                    int sum = sums[c * BM];
+                    for (uint32_t from = 0; from + 1 < J.slices; from++) sum += others[(from * share + c - mine) * BM];
+                    const float f = (float)sum * xs[quarter][c] * ws;
+                    const size_t at = (size_t)(p.m0 + c) * T.rows + row;
+                    if (J.bf16) put(static_cast<__nv_bfloat16 *>(T.y) + at, f);
+                    else put(static_cast<float *>(T.y) + at, f);
+                }
         }
         __syncwarp();
-        cluster_sync();
-        if (warp >= 2 && *(volatile uint32_t *)&ctl.abort_flag == 0) {
-            const uint32_t row = p.tile * BM + 32 * quarter + lane;
-            const float ws = row < T.rows ? T.scales[row] : 0.f;
-            const int *part = reinterpret_cast<const int *>(ring) + 32 * quarter + lane;
-            for (uint32_t c0 = mine & ~15u; c0 < mine_end; c0 += 16) {
-                int v[16];
-                tmem_ld16(acc + c0, v);
-#pragma unroll
-                for (uint32_t c = 0; c < 16; c++) {
-                    const uint32_t col = c0 + c;
-                    if (col < mine || col >= mine_end) continue;
-                    int sum = v[c];
-                    for (uint32_t from = 0; from + 1 < J.slices; from++) sum += part[(from * share + col - mine) * BM];
-                    if (row < T.rows) store_value(J, T, p.m0 + col, row, sum, __ldcg(J.x_scales + p.m0 + col), ws);
-                }
-            }
-        }
+        cluster_sync(); // what a block sent has been received
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -472,7 +475,9 @@ struct Plan {
     uint32_t bn, token_tiles, slices, per, stages, per_sm;
     bool pair;
 };
-Plan plan(const fq_matrix *const *w, uint32_t count, uint32_t k_blocks, uint32_t m, uint32_t sms) {
+uint32_t ring_bytes(const Plan &p) { return p.stages * (TILE_BYTES + (p.pair ? p.bn / 2 : p.bn) * BK); }
+Plan plan(const fq_device *dev, const fq_matrix *const *w, uint32_t count, uint32_t k_blocks, uint32_t m) {
+    const uint32_t sms = (uint32_t)dev->sm_count;
     uint32_t tiles = 0, pairs = 0;
     for (uint32_t i = 0; i < count; i++) {
         tiles += (uint32_t)((w[i]->rows + BM - 1) / BM);
@@ -491,7 +496,11 @@ Plan plan(const fq_matrix *const *w, uint32_t count, uint32_t k_blocks, uint32_t
         const uint32_t items = (pair ? pairs : tiles) * c.token_tiles, slots = pair ? sms / 2 : sms * c.per_sm;
         c.per = (k_blocks + slices - 1) / slices;
         c.slices = (k_blocks + c.per - 1) / c.per; // no slice is left without work
-        if (c.slices > 1 && items * c.slices > slots) return;
+        c.stages = std::min((SMEM_MAX / c.per_sm - 8192) / (TILE_BYTES + (pair ? c.bn / 2 : c.bn) * BK), MAX_STAGES);
+        if (c.slices > 1) { // all at once, and the sums fit where the ring was
+            if (items > dev->i8_clusters[c.per_sm - 1][c.slices]) return;
+            if ((c.bn + (c.slices - 1) * ((c.bn + c.slices - 1) / c.slices)) * BM * 4 > ring_bytes(c)) return;
+        }
         // Clocks of a k-block on an SM: its MMAs (measured, profiles/tcgen05_mma_rate.md), or what it takes in at 44 bytes a clock,
         // the rate at which all SMs together are fed from L2.
         const double mma = 4.0 * std::max(32.0 + c.bn / 4.0, c.bn / 2.0), feed = (TILE_BYTES + (pair ? c.bn / 2 : c.bn) * BK) / 44.0;
@@ -503,21 +512,44 @@ Plan plan(const fq_matrix *const *w, uint32_t count, uint32_t k_blocks, uint32_t
         }
     };
     if (m <= 64) { // as much of the weights under way as the machine holds
-        consider(1, false, std::max(1u, std::min({2 * sms / tiles, MAX_SLICES, k_blocks})));
+        for (uint32_t slices = 1; slices <= std::min(MAX_SLICES, k_blocks); slices++) {
+            best = 0.0;
+            const Plan before = p;
+            p.bn = 0;
+            consider(1, false, slices);
+            if (p.bn == 0) p = before;
+        }
     } else {
         for (uint32_t t = (m + 255) / 256; t <= (m + 255) / 256 + 7 && t <= (m + 15) / 16; t++) {
             for (uint32_t slices = 1; slices <= std::min(MAX_SLICES, k_blocks); slices++) consider(t, false, slices);
             consider(t, true, 1);
         }
     }
-    p.stages = std::min((SMEM_MAX / p.per_sm - 8192) / (TILE_BYTES + (p.pair ? p.bn / 2 : p.bn) * BK), MAX_STAGES);
     return p;
 }
 
-// Once per handle's device: the kernels may use all of an SM's shared memory.
-cudaError_t allow_shared_memory() {
+// Once per handle: the kernels may use all of an SM's shared memory, and how many clusters of each size run at once (a cluster's
+// blocks share a GPC, so fewer than blocks would).
+cudaError_t prepare_device(fq_device *dev) {
+    if (dev->i8_clusters[0][1]) return cudaSuccess;
     for (const void *kernel : {(const void *)k_gemm_i8<false>, (const void *)k_gemm_i8<true>, (const void *)k_gemm_i8_pair})
         if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(SMEM_MAX - 6144))) return e;
+    for (uint32_t per_sm = 2; per_sm >= 1; per_sm--)
+        for (uint32_t slices = MAX_SLICES; slices >= 1; slices--) {
+            cudaLaunchConfig_t cfg{};
+            cfg.gridDim = dim3(slices * (uint32_t)dev->sm_count);
+            cfg.blockDim = dim3(THREADS);
+            cfg.dynamicSmemBytes = SMEM_MAX / per_sm - 8192 + 1024;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = slices;
+            attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            int clusters = 0;
+            if (const cudaError_t e = cudaOccupancyMaxActiveClusters(&clusters, k_gemm_i8<true>, &cfg)) return e;
+            dev->i8_clusters[per_sm - 1][slices] = (uint16_t)clusters; // [0][1], the last, is never 0
+        }
     return cudaSuccess;
 }
 
@@ -534,7 +566,7 @@ int encode_bytes(fq_device *dev, CUtensorMap *map, const void *p, uint64_t cols,
 
 int launch(fq_device *dev, const fq_matrix *const *w, uint32_t count, const int8_t *x, const float *x_scales, uint32_t m, void *const *y, int y_dtype) {
     const uint32_t cols = (uint32_t)w[0]->cols, k_blocks = (cols + BK - 1) / BK;
-    const Plan p = plan(w, count, k_blocks, m, (uint32_t)dev->sm_count);
+    const Plan p = plan(dev, w, count, k_blocks, m);
     Job J{};
     uint32_t tiles = 0; // of 128 rows, or for pairs of 256
     for (uint32_t i = 0; i < count; i++) {
@@ -562,7 +594,7 @@ int launch(fq_device *dev, const fq_matrix *const *w, uint32_t count, const int8
     const uint32_t sms = (uint32_t)dev->sm_count;
     cfg.gridDim = dim3(p.pair ? 2 * std::min(J.items, sms / 2) : p.slices > 1 ? J.items * p.slices : std::min(J.items, sms * p.per_sm));
     cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = 1024 + p.stages * (TILE_BYTES + (p.pair ? p.bn / 2 : p.bn) * BK);
+    cfg.dynamicSmemBytes = 1024 + ring_bytes(p);
     cfg.stream = dev->stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -622,7 +654,7 @@ extern "C" int fq_matrix_create_i8(fq_device *dev, uint64_t rows, uint64_t cols,
     // The tiles are laid out on the device; rows in host memory (or off their 16 bytes) go through a copy of their own.
     uint8_t *staged = nullptr;
     const uint8_t *src = (const uint8_t *)values;
-    e = allow_shared_memory();
+    e = prepare_device(dev);
     if (e == cudaSuccess) e = cudaMalloc((void **)&w->data, len + rows * 4);
     w->scales = (float *)(w->data + len);
     if (e == cudaSuccess && (!on_device || ((uintptr_t)values & 15))) {
