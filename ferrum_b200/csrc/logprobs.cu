@@ -18,9 +18,11 @@
 // The most likely tokens: every warp keeps its best 32 as a sorted list, one (value, index) key per lane, and puts a value in
 // only if it can still matter: above a bound that k values of the block are known to reach.  The bound starts with what is read
 // first -- the k-th largest of some 64 thread maxima, the best of every warp -- so that few values pass it, and rises with the
-// lists.  Keys are unique (of equal values the lower index is larger), so the result does not depend on the order of warps.
+// lists.  Keys are unique (of equal values the lower index is larger), so the result does not depend on the order of warps.  At
+// the end what is left above the bound, little more than k values of all lists, is put in order by counting.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "gemv_common.cuh"
 #include "internal.h"
@@ -80,13 +82,19 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a
 
 template <typename T> constexpr int PER_LOAD = 16 / (int)sizeof(T);
 __device__ __forceinline__ uint32_t word(const uint4 &u, int i) { return i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w; }
-// The largest of a 16-byte piece; NaN if one is.
-template <typename T> __device__ __forceinline__ float piece_max(const uint4 &u) {
+// The largest of 16-byte pieces; NaN if one is.
+template <typename T, int N> __device__ __forceinline__ float largest(const uint4 (&u)[N]) {
     if constexpr (sizeof(T) == 2) {
-        const uint32_t m = max_nan_bf16x2(max_nan_bf16x2(u.x, u.y), max_nan_bf16x2(u.z, u.w));
+        uint32_t m = max_nan_bf16x2(max_nan_bf16x2(u[0].x, u[0].y), max_nan_bf16x2(u[0].z, u[0].w));
+#pragma unroll
+        for (int i = 1; i < N; i++) m = max_nan_bf16x2(m, max_nan_bf16x2(max_nan_bf16x2(u[i].x, u[i].y), max_nan_bf16x2(u[i].z, u[i].w)));
         return max_nan(low_half(m), high_half(m));
     } else {
-        return max_nan(max_nan(__uint_as_float(u.x), __uint_as_float(u.y)), max_nan(__uint_as_float(u.z), __uint_as_float(u.w)));
+        float m = __uint_as_float(u[0].x);
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            m = max_nan(m, max_nan(max_nan(__uint_as_float(u[i].x), __uint_as_float(u[i].y)), max_nan(__uint_as_float(u[i].z), __uint_as_float(u[i].w))));
+        return m;
     }
 }
 // Values 2 i and 2 i + 1 of a piece.
@@ -108,10 +116,26 @@ template <typename T> __device__ __forceinline__ float load1(const T *l, uint32_
     else return __ldcg(l + i);
 }
 
+// The 16-byte piece at elements first .. of a row's end: one element at a time, -infinity outside the row.
+template <typename T> __device__ __noinline__ uint4 ends(const T *l, uint32_t n, uint32_t first) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (sizeof(T) == 2) {
+            const uint32_t a = first + 2 * i, b = a + 1; // wrap in the piece that begins before the row
+            const uint32_t lo = a < n ? __ldcg(reinterpret_cast<const unsigned short *>(l) + a) : 0xFF80u, hi = b < n ? __ldcg(reinterpret_cast<const unsigned short *>(l) + b) : 0xFF80u;
+            w[i] = lo | hi << 16;
+        } else {
+            const uint32_t a = first + i;
+            w[i] = a < n ? __float_as_uint(__ldcg(l + a)) : 0xFF800000u;
+        }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 struct Sums {
     float c, s, t; // pivot, sum 2^(b l - c), sum 2^(b l - c) (b l - c)
 };
-constexpr float NO_PIVOT = LEAST * LOG2E;
 // The sums about another pivot.
 __device__ __forceinline__ void move_pivot(Sums &a, float c) {
     const float f = exp2_fast(a.c - c);
@@ -126,9 +150,19 @@ __device__ __forceinline__ void join(Sums &a, Sums b) {
     a.s += b.s;
     a.t += b.t;
 }
-__device__ __forceinline__ Sums join_warp(Sums a) {
+// Over the first `lanes` lanes (a power of two).  Pivots are the same nearly always.
+__device__ __forceinline__ Sums join_warp(Sums a, int lanes = 32) {
+    if (__all_sync(0xffffffffu, a.c == __shfl_sync(0xffffffffu, a.c, 0))) {
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1)
+            if (off < lanes) {
+                a.s += __shfl_xor_sync(0xffffffffu, a.s, off);
+                a.t += __shfl_xor_sync(0xffffffffu, a.t, off);
+            }
+        return a;
+    }
 #pragma unroll 1
-    for (int off = 16; off > 0; off >>= 1) {
+    for (int off = lanes / 2; off > 0; off >>= 1) {
         const Sums b{__shfl_xor_sync(0xffffffffu, a.c, off), __shfl_xor_sync(0xffffffffu, a.s, off), __shfl_xor_sync(0xffffffffu, a.t, off)};
         join(a, b);
     }
@@ -180,11 +214,11 @@ template <typename T, int NT, bool TOP>
 __global__ void __launch_bounds__(NT, 1024 / NT)
 k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids, uint32_t k, uint32_t parts, Outputs out) {
     constexpr int W = NT / 32, V = PER_LOAD<T>;
-    __shared__ uint32_t first_max[W], bound;
+    __shared__ uint32_t first_max[W], bound, left;
     __shared__ uint4 firsts[FIRSTS / 4];
     __shared__ Sums sums[W];
     __shared__ uint32_t counts[W], bads[W];
-    __shared__ uint64_t lists[TOP ? W : 1][32];
+    __shared__ uint64_t keys[TOP ? NT : 1], list_out[32];
     // Of block 0: what the blocks of the cluster found.
     __shared__ Sums all_sums[MAX_CLUSTER];
     __shared__ uint32_t all_counts[MAX_CLUSTER], all_bads[MAX_CLUSTER];
@@ -193,43 +227,30 @@ k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids
     if (parts > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
     pdl_trigger();
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.x / parts, rank = blockIdx.x - row * parts;
-    if (tid == 0) bound = 0;
+    if (tid == 0) bound = left = 0;
     pdl_wait();
     // The row in whole 16-byte pieces from the boundary below its start: piece j holds elements j * V - skip ...
     const T *l = logits + (size_t)row * stride;
     const uint32_t skip = (uint32_t)(((uintptr_t)l & 15) / sizeof(T));
-    const T *aligned = l - skip;
+    const uint4 *aligned = reinterpret_cast<const uint4 *>(l - skip);
     const uint32_t pieces = (uint32_t)(((uint64_t)skip + n + V - 1) / V), per = (pieces + parts - 1) / parts;
     const uint32_t begin = min(rank * per, pieces), end = min(begin + per, pieces);
-    const uint32_t id = ids ? __ldcg(ids + row) : n;
-    auto load = [&](uint32_t j) {
-        const uint32_t first = j * V - skip; // wraps in the piece that begins before the row
-        if (first <= n && n - first >= (uint32_t)V) return __ldcg(reinterpret_cast<const uint4 *>(aligned) + j);
-        uint32_t w[4]; // the row's ends: elements one at a time, -infinity outside
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if constexpr (sizeof(T) == 2) {
-                const uint32_t a = first + 2 * i, b = a + 1;
-                const uint32_t lo = a < n ? __ldcg(reinterpret_cast<const unsigned short *>(l) + a) : 0xFF80u, hi = b < n ? __ldcg(reinterpret_cast<const unsigned short *>(l) + b) : 0xFF80u;
-                w[i] = lo | hi << 16;
-            } else {
-                const uint32_t at = first + i;
-                w[i] = at < n ? __float_as_uint(__ldcg(l + at)) : 0xFF800000u;
-            }
-        }
-        return make_uint4(w[0], w[1], w[2], w[3]);
-    };
     const uint32_t whole_from = skip ? 1 : 0, whole_to = min(end, (uint32_t)(((uint64_t)skip + n) / V)); // pieces that lie in the row
-    uint4 next[UNROLL];
-    auto fetch = [&](uint32_t j0) { // of the block's UNROLL * NT pieces from j0 this thread's
+    const uint32_t id = ids ? __ldcg(ids + row) : n;
+    constexpr uint32_t NONE = sizeof(T) == 2 ? 0xFF80FF80u : 0xFF800000u; // -infinity
+    uint4 now[UNROLL];
+    // This thread's UNROLL pieces of the block's UNROLL * NT from j0 on.
+    auto fetch = [&](uint32_t j0) {
         if (j0 >= whole_from && j0 + UNROLL * NT <= whole_to) {
 #pragma unroll
-            for (int u = 0; u < UNROLL; u++) next[u] = __ldcg(reinterpret_cast<const uint4 *>(aligned) + j0 + u * NT + tid);
+            for (int u = 0; u < UNROLL; u++) now[u] = __ldcg(aligned + j0 + u * NT + tid);
         } else {
 #pragma unroll
             for (int u = 0; u < UNROLL; u++) {
-                const uint32_t j = j0 + u * NT + tid, none = sizeof(T) == 2 ? 0xFF80FF80u : 0xFF800000u; // -infinity
-                next[u] = j < end ? load(j) : make_uint4(none, none, none, none);
+                const uint32_t j = j0 + u * NT + tid;
+                now[u] = make_uint4(NONE, NONE, NONE, NONE);
+                if (j >= whole_from && j < whole_to) now[u] = __ldcg(aligned + j);
+                else if (j < end) now[u] = ends(l, n, j * V - skip);
             }
         }
     };
@@ -237,10 +258,7 @@ k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids
     const float given = id < n ? load1(l, id) : __int_as_float(0x7fc00000);
 
     // What is read first gives the pivot and a bound that k values of the block reach.
-    uint32_t best = 0;
-#pragma unroll
-    for (int u = 0; u < UNROLL; u++)
-        if (begin + tid + u * NT < end) best = max(best, order_of(piece_max<T>(next[u]))); // (a piece with a NaN does not count)
+    uint32_t best = begin + tid < end ? order_of(largest<T>(now)) : 0; // (a thread with a NaN does not count)
     const uint32_t warps = min((uint32_t)W, (end - begin + 31) / 32); // with something to read
     uint32_t high = __reduce_max_sync(0xffffffffu, best);
     if (lane == 0) first_max[warp] = high;
@@ -259,7 +277,7 @@ k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids
         for (uint32_t i = m * warps + tid; i < FIRSTS; i += NT) reinterpret_cast<uint32_t *>(firsts)[i] = 0;
     }
     __syncthreads();
-    const float top = value_of(max(__reduce_max_sync(0xffffffffu, first_max[lane % W]), 1u << 23)); // -infinity where there is nothing (or NaN)
+    const float top = value_of(max(__reduce_max_sync(0xffffffffu, first_max[lane % W]), 1u << 23)); // the lowest number where there is nothing (or NaN)
     Sums a{fmaxf(top, LEAST) * LOG2E, 0.f, 0.f};
     float limit = fminf(fmaf(SLACK, 1.f / LOG2E, fmaxf(top, LEAST)), MOST); // logits above it move the pivot
     uint32_t least = 0; // values of a lower order do not matter any more; 0: all do
@@ -273,6 +291,7 @@ k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids
             above_y += (f.x > y) + (f.y > y) + (f.z > y) + (f.w > y);
         }
         least = __reduce_min_sync(0xffffffffu, min(above_x < k ? x : 0xFFFFFFFFu, above_y < k ? y : 0xFFFFFFFFu));
+        if (tid == 0) atomicMax(&bound, least);
     }
     float below = just_below(least);
     bool bad = false, beyond = false, some = false; // a NaN or +infinity; a logit above MOST; one above -infinity
@@ -282,32 +301,25 @@ k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids
 
 #pragma unroll 1
     for (uint32_t j0 = begin; j0 < end; j0 += UNROLL * NT) {
-        uint4 now[UNROLL];
-        float mx[UNROLL];
-#pragma unroll
-        for (int u = 0; u < UNROLL; u++) now[u] = next[u];
-        fetch(j0 + UNROLL * NT);
-#pragma unroll
-        for (int u = 0; u < UNROLL; u++) mx[u] = piece_max<T>(now[u]);
-        if constexpr (TOP) {
-            uint32_t maybe = 0;
-#pragma unroll
-            for (int u = 0; u < UNROLL; u++) maybe |= (uint32_t)!(mx[u] <= below) << u;
-            if (__any_sync(0xffffffffu, maybe)) { // some pieces are looked into, in the order of their indexes
+        const float highest = largest<T>(now);
+        if constexpr (TOP)
+            if (__any_sync(0xffffffffu, !(highest <= below))) { // some pieces are looked into, in the order of their indexes
                 least = max(least, *(volatile uint32_t *)&bound);
 #pragma unroll 1
                 for (int u = 0; u < UNROLL; u++) {
-                    uint32_t vote = __ballot_sync(0xffffffffu, (maybe >> u & 1) && j0 + u * NT + tid < end);
+                    const uint4 own[1] = {u == 0 ? now[0] : u == 1 ? now[1] : u == 2 ? now[2] : now[3]};
+                    uint32_t vote = __ballot_sync(0xffffffffu, !(largest<T>(own) <= below) && j0 + u * NT + tid < end);
+#pragma unroll 1
                     while (vote) {
-                        const uint32_t src = __ffs(vote) - 1, j = j0 + u * NT + 32 * warp + src;
+                        const uint32_t src = __ffs(vote) - 1, first = (j0 + u * NT + 32 * warp + src) * V - skip;
                         vote &= vote - 1;
-                        uint4 piece = u == 0 ? now[0] : u == 1 ? now[1] : u == 2 ? now[2] : now[3];
-                        piece = make_uint4(__shfl_sync(0xffffffffu, piece.x, src), __shfl_sync(0xffffffffu, piece.y, src), __shfl_sync(0xffffffffu, piece.z, src),
-                                           __shfl_sync(0xffffffffu, piece.w, src));
+                        const uint4 piece = make_uint4(__shfl_sync(0xffffffffu, own[0].x, src), __shfl_sync(0xffffffffu, own[0].y, src),
+                                                       __shfl_sync(0xffffffffu, own[0].z, src), __shfl_sync(0xffffffffu, own[0].w, src));
                         // Lane i looks at value i; those that may matter go in one after the other.
-                        const uint32_t i = lane % V, w = word(piece, sizeof(T) == 2 ? i / 2 : i), at = j * V - skip + i;
+                        const uint32_t i = lane % V, w = word(piece, sizeof(T) == 2 ? i / 2 : i), at = first + i;
                         const uint32_t order = order_of(sizeof(T) == 4 ? __uint_as_float(w) : (i & 1) ? high_half(w) : low_half(w));
                         uint32_t fit = __ballot_sync(0xffffffffu, lane < V && at < n && order >= least);
+#pragma unroll 1
                         while (fit) {
                             const uint64_t key = __shfl_sync(0xffffffffu, key_of(order, at), __ffs(fit) - 1);
                             fit &= fit - 1;
@@ -323,10 +335,6 @@ k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids
                 if (lane == k - 1 && list) atomicMax(&bound, (uint32_t)(list >> 32));
                 below = just_below(least);
             }
-        }
-        float highest = mx[0];
-#pragma unroll
-        for (int u = 1; u < UNROLL; u++) highest = max_nan(highest, mx[u]);
         if (!(highest <= given)) {
             if constexpr (sizeof(T) == 2) { // ones added in bf16: 4 * UNROLL at most
                 const __nv_bfloat162 g = __float2bfloat162_rn(given);
@@ -369,56 +377,75 @@ k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids
                 s2 = add2(s2, e);
                 t2 = fma2(d, e, t2);
             }
+        if (j0 + UNROLL * NT < end) fetch(j0 + UNROLL * NT);
     }
     a.s = s2.x + s2.y;
     a.t = t2.x + t2.y;
 
-    // The block's sums and list, then the cluster's.
+    // The block's sums and its best values, then the cluster's.
     a = join_warp(a);
     count = __reduce_add_sync(0xffffffffu, count);
-    const uint32_t flags = (__any_sync(0xffffffffu, bad) ? 1 : 0) | (__any_sync(0xffffffffu, beyond) ? 2 : 0) | (__any_sync(0xffffffffu, some) ? 4 : 0);
+    uint32_t flags = (__any_sync(0xffffffffu, bad) ? 1 : 0) | (__any_sync(0xffffffffu, beyond) ? 2 : 0) | (__any_sync(0xffffffffu, some) ? 4 : 0);
     if (lane == 0) {
         sums[warp] = a;
         counts[warp] = count;
         bads[warp] = flags;
     }
-    if constexpr (TOP) {
-        lists[warp][lane] = list;
-#pragma unroll 1
-        for (int half = W / 2; half > 0; half >>= 1) {
-            __syncthreads();
-            if (warp < (uint32_t)half) lists[warp][lane] = list = merge_lists(list, lists[warp + half], lane);
-        }
-    }
     __syncthreads();
-    uint32_t all = 0;
-    if (parts > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    if constexpr (TOP) {
+        const uint32_t kept = __ballot_sync(0xffffffffu, list != 0 && (uint32_t)(list >> 32) >= bound); // a list's first ones
+        uint32_t at = 0;
+        if (lane == 0 && kept) at = atomicAdd(&left, __popc(kept));
+        at = __shfl_sync(0xffffffffu, at, 0);
+        if (kept >> lane & 1) keys[at + lane] = list;
+    }
     if (warp == 0) {
-        a = join_warp(lane < W ? sums[lane] : Sums{NO_PIVOT, 0.f, 0.f});
+        a = join_warp(lane < W ? sums[lane] : Sums{sums[0].c, 0.f, 0.f});
         count = __reduce_add_sync(0xffffffffu, lane < W ? counts[lane] : 0u);
-        all = __reduce_or_sync(0xffffffffu, lane < W ? bads[lane] : 0u);
-        if (parts > 1) {
-            if (lane < 3) store_cluster(cluster_address(&all_sums[rank], 0) + 4 * lane, __float_as_uint(lane == 0 ? a.c : lane == 1 ? a.s : a.t));
-            if (lane == 3) store_cluster(cluster_address(&all_counts[rank], 0), count);
-            if (lane == 4) store_cluster(cluster_address(&all_bads[rank], 0), all);
-            if constexpr (TOP) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(cluster_address(&all_lists[rank][lane], 0)), "l"(list) : "memory");
+        flags = __reduce_or_sync(0xffffffffu, lane < W ? bads[lane] : 0u);
+        if constexpr (TOP) list_out[lane] = 0;
+    }
+    if constexpr (TOP) {
+        __syncthreads();
+        const uint32_t total = left;
+        if (tid < total) {
+            const uint64_t mine = keys[tid];
+            uint32_t above = 0;
+#pragma unroll 4
+            for (uint32_t i = 0; i < total; i++) above += keys[i] > mine;
+            if (above < 32) list_out[above] = mine;
         }
+        __syncthreads();
+        if (warp == 0) list = list_out[lane];
     }
     if (parts > 1) {
+        asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+        if (warp == 0) {
+            if (lane < 3) store_cluster(cluster_address(&all_sums[rank], 0) + 4 * lane, __float_as_uint(lane == 0 ? a.c : lane == 1 ? a.s : a.t));
+            if (lane == 3) store_cluster(cluster_address(&all_counts[rank], 0), count);
+            if (lane == 4) store_cluster(cluster_address(&all_bads[rank], 0), flags);
+            if constexpr (TOP) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(cluster_address(&all_lists[rank][lane], 0)), "l"(list) : "memory");
+        }
         __syncwarp();
         asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
-        if (rank != 0 || warp != 0) return;
-        a = join_warp(lane < parts ? all_sums[lane] : Sums{NO_PIVOT, 0.f, 0.f});
-        count = __reduce_add_sync(0xffffffffu, lane < parts ? all_counts[lane] : 0u);
-        all = __reduce_or_sync(0xffffffffu, lane < parts ? all_bads[lane] : 0u);
+        if (rank != 0) return;
+        if (warp == 0) {
+            a = join_warp(lane < parts ? all_sums[lane] : Sums{all_sums[0].c, 0.f, 0.f}, MAX_CLUSTER);
+            a = Sums{__shfl_sync(0xffffffffu, a.c, 0), __shfl_sync(0xffffffffu, a.s, 0), __shfl_sync(0xffffffffu, a.t, 0)};
+            count = __reduce_add_sync(0xffffffffu, lane < parts ? all_counts[lane] : 0u);
+            flags = __reduce_or_sync(0xffffffffu, lane < parts ? all_bads[lane] : 0u);
+        }
         if constexpr (TOP)
 #pragma unroll 1
-            for (uint32_t i = 1; i < parts; i++) list = merge_lists(list, all_lists[i], lane);
+            for (uint32_t half = parts / 2; half > 0; half /= 2) { // (parts is a power of two)
+                if (warp < half) all_lists[warp][lane] = list = merge_lists(all_lists[warp][lane], all_lists[warp + half], lane);
+                __syncthreads();
+            }
     }
     if (warp != 0) return;
     double z, entropy;
-    if ((all & 1) || !(all & 4)) z = entropy = NAN;
-    else if ((all & 2) || a.c < -MOST * LOG2E) sum_64(l, n, lane, z, entropy); // (the pivot is the row's largest or near it)
+    if ((flags & 1) || !(flags & 4)) z = entropy = NAN;
+    else if ((flags & 2) || a.c < -MOST * LOG2E) sum_64(l, n, lane, z, entropy); // (the pivot is the row's largest or near it)
     else {
         const double log2_s = log2((double)a.s);
         z = ((double)a.c + log2_s) / (double)LOG2E;
@@ -454,12 +481,17 @@ cudaError_t launch_shape(fq_device *dev, const T *logits, uint32_t n, size_t str
 }
 template <typename T>
 cudaError_t launch_rows(fq_device *dev, const T *logits, uint32_t n, size_t stride, uint32_t rows, const uint32_t *ids, uint32_t k, const Outputs &out) {
+    const uint32_t sms = (uint32_t)dev->sm_count;
+    const bool wide = rows * MAX_CLUSTER <= sms && n > 8192; // a few rows: as many threads as there can be
     uint32_t parts = 1;
-    while (parts < MAX_CLUSTER && rows * (2 * parts) <= 2 * (uint32_t)dev->sm_count && n / (2 * parts) >= 4096) parts *= 2;
-    // TODO
-    if (parts == 1 && n > 8192) return k ? launch_shape<T, 256, true>(dev, logits, n, stride, rows, ids, k, parts, out) : launch_shape<T, 256, false>(dev, logits, n, stride, rows, ids, k, parts, out);
-    if (n <= 8192) return k ? launch_shape<T, 128, true>(dev, logits, n, stride, rows, ids, k, parts, out) : launch_shape<T, 128, false>(dev, logits, n, stride, rows, ids, k, parts, out);
-    return k ? launch_shape<T, 512, true>(dev, logits, n, stride, rows, ids, k, parts, out) : launch_shape<T, 512, false>(dev, logits, n, stride, rows, ids, k, parts, out);
+    while (parts < MAX_CLUSTER && (wide || rows * (2 * parts) <= 4 * sms) && n / (2 * parts) >= 4096) parts *= 2;
+    auto go = [&](auto top) {
+        constexpr bool TOP = decltype(top)::value;
+        if (wide) return launch_shape<T, 512, TOP>(dev, logits, n, stride, rows, ids, k, parts, out);
+        if (n > 8192) return launch_shape<T, 256, TOP>(dev, logits, n, stride, rows, ids, k, parts, out);
+        return launch_shape<T, 128, TOP>(dev, logits, n, stride, rows, ids, k, parts, out);
+    };
+    return k ? go(std::true_type{}) : go(std::false_type{});
 }
 
 } // namespace

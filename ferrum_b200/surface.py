@@ -395,6 +395,9 @@ class Matrix:
             raise Unsupported(f"8-bit matrix of {values.dtype} with scales of {scales.dtype}")
         if values.dim() != 2 or scales.numel() != values.shape[0] or not values.is_contiguous() or not scales.is_contiguous():
             raise ShapeError(f"8-bit matrix {tuple(values.shape)} with {scales.numel()} scales")
+        for t in (values, scales):
+            if t.is_cuda:  # what makes it may still run, on a stream that is not the handle's
+                torch.cuda.current_stream(t.device).synchronize()
         h = C.c_void_p()
         device.check(device._L.fq_matrix_create_i8(device.handle, values.shape[0], values.shape[1], _ptr(values), _ptr(scales), C.byref(h)))
         return cls(device, h)
