@@ -15,12 +15,13 @@
 // than 20 / b above it (a term is 2^20 at most, far from fp32's end; a running maximum would rescale every few values).  Dividing by b as
 // it is keeps its own rounding out of z.
 //
-// The most likely tokens: every warp keeps its best 32 as a sorted list, one (value, index) key per lane, and puts a value in
-// only if it can still matter: above a bound that k values of the block are known to reach.  The bound starts with what is read
-// first -- the k-th largest of some 64 thread maxima, the best of every warp -- so that few values pass it, and rises with the
-// lists.  Keys are unique (of equal values the lower index is larger), so the result does not depend on the order of warps.  At
-// the end what is left above the bound, little more than k values of all lists, is put in order by counting.
+// The most likely tokens: while the row is read, every thread notes the largest of each 16 or 32 logits it takes in.  Of the
+// block's threads the k-th largest maximum is a bound that k tokens reach and few more do, so at the end only the few pieces that
+// reach it are read again, and what they hold is put in order by counting (what a piece could hold was looked at as it came
+// by, against a bound that rose slowly, in the first version: 20 to 90 us more for 8 to 32 alternatives of 1021 rows).
+// Keys (value, index) are unique, of equal values the lower index is larger, so nothing depends on the order of threads.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <type_traits>
 
@@ -32,7 +33,9 @@ using namespace fqk;
 
 constexpr uint32_t MAX_TOP = 32, MAX_CLUSTER = 8;
 constexpr int UNROLL = 4;        // 16-byte loads of a thread in flight
-constexpr uint32_t FIRSTS = 64;  // thread maxima that the first bound is taken from
+constexpr uint32_t FIRSTS = 64;  // thread maxima that the bound is taken from
+template <int NT> constexpr uint32_t NOTES = 40 * 256 / NT; // maxima that a thread notes (more tiles than these share one)
+constexpr uint32_t POOL = 512;   // pieces read again, and values kept of them
 constexpr float LOG2E = 1.44269502f; // b: log2(e) rounded to fp32
 constexpr float SLACK = 20.f;        // how far b l may be above the pivot
 // Beyond a million the rounding of c is no longer small: a row whose largest logit lies there is summed in 64 bits (sum_64).
@@ -46,11 +49,6 @@ __device__ __forceinline__ uint32_t order_of(float v) {
     return v != v ? 0u : (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float value_of(uint32_t order) { return __uint_as_float((order & 0x80000000u) ? order ^ 0x80000000u : ~order); }
-// A number below every one whose order is at least `least`, and not below the others by more than a step: NaN where there is none.
-__device__ __forceinline__ float just_below(uint32_t least) {
-    const uint32_t below = least - 1 == 0x7FFFFFFFu ? 0x7FFFFFFEu : least - 1; // -0 is not below +0
-    return least == 0 ? __int_as_float(0x7fc00000) : value_of(below);
-}
 __device__ __forceinline__ uint64_t key_of(uint32_t order, uint32_t i) { return (uint64_t)order << 32 | (uint32_t)~i; }
 
 __device__ __forceinline__ float exp2_fast(float d) { // within 2^-22 of itself; 0 below 2^-126
@@ -209,16 +207,153 @@ __device__ __forceinline__ uint32_t cluster_address(const void *p, uint32_t rank
 }
 __device__ __forceinline__ void store_cluster(uint32_t to, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to), "r"(v) : "memory"); }
 
+template <bool TOP> struct Best { // shared memory of best_of
+    uint4 firsts[FIRSTS / 4];
+    uint64_t keys[POOL + MAX_TOP], out[MAX_TOP];
+    uint32_t work[POOL], wanted, found, raised, before[32];
+};
+template <> struct Best<false> {};
+
+// The k best (value, index) keys of the block's pieces [begin, end), sorted, in the lanes of its first warp (0 where there are
+// fewer); all threads call it, after what they noted.
+template <typename T, int NT>
+__device__ __forceinline__ uint64_t best_of(Best<true> &S, const float *notes, uint32_t noted, uint32_t shared_by, const T *l, const uint4 *aligned, uint32_t n,
+                                            uint32_t skip, uint32_t begin, uint32_t end, uint32_t k) {
+    constexpr uint32_t W = NT / 32, V = PER_LOAD<T>, TILE = UNROLL * NT;
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    uint32_t *firsts = reinterpret_cast<uint32_t *>(S.firsts);
+    // This thread's first piece of a note; the threads that have one come first.
+    auto piece_of = [&](uint32_t note, uint32_t thread) { return begin + note * shared_by * TILE + thread; };
+    float most = __int_as_float(0x7fc00000);
+    for (uint32_t i = 0; i < noted && piece_of(i, tid) < end; i++) most = fmaxf(most, notes[i * NT + tid]);
+    uint32_t best = order_of(most); // a logit of the thread, or 0
+    const uint32_t warps = min(W, (end - begin + 31) / 32), m = min(32u, FIRSTS / max(warps, 1u)); // of every warp m maxima, m * warps >= k
+    if (warp < warps) {
+        uint32_t high = __reduce_max_sync(0xffffffffu, best);
+#pragma unroll 1
+        for (uint32_t i = 0; i < m; i++) {
+            if (lane == 0) firsts[warp * m + i] = high;
+            const uint32_t holders = __ballot_sync(0xffffffffu, best == high);
+            if (lane == (uint32_t)__ffs(holders) - 1) best = 0;
+            high = __reduce_max_sync(0xffffffffu, best);
+        }
+    }
+    for (uint32_t i = m * warps + tid; i < FIRSTS; i += NT) firsts[i] = 0;
+    if (tid == 0) S.wanted = S.found = 0;
+    __syncthreads();
+    // The bound: the least of those that fewer than k are above.  0, below everything, where there are fewer than k.
+    uint32_t least, above_x = 0, above_y = 0;
+    const uint32_t x = firsts[lane], y = firsts[lane + 32];
+#pragma unroll 4
+    for (uint32_t i = 0; i < FIRSTS / 4; i++) {
+        const uint4 f = S.firsts[i];
+        above_x += (f.x > x) + (f.y > x) + (f.z > x) + (f.w > x);
+        above_y += (f.x > y) + (f.y > y) + (f.z > y) + (f.w > y);
+    }
+    least = __reduce_min_sync(0xffffffffu, min(above_x < k ? x : 0xFFFFFFFFu, above_y < k ? y : 0xFFFFFFFFu));
+    auto load = [&](uint32_t j) { return j * V - skip <= n && n - (j * V - skip) >= V ? __ldcg(aligned + j) : ends(l, n, j * V - skip); };
+    auto order_at = [&](const uint4 &p, uint32_t i) {
+        const uint32_t w = word(p, sizeof(T) == 2 ? i / 2 : i);
+        return order_of(sizeof(T) == 4 ? __uint_as_float(w) : (i & 1) ? high_half(w) : low_half(w));
+    };
+    // All logits that reach the bound; where they are too many for the pool, many are equal to it, or the threads' maxima were
+    // not spread: then those above it, and where these are too many, those above the k-th of the ones at hand, and so on.
+    bool above = false; // only those above the bound
+    uint32_t total;
+    for (;;) {
+        const float reach = value_of(least);
+        for (uint32_t i = 0; i < noted && piece_of(i, tid) < end; i++) {
+            const float v = notes[i * NT + tid];
+            if (least == 0 ? !above || v == v : above ? v > reach : v >= reach) {
+                const uint32_t at = atomicAdd(&S.wanted, 1u);
+                if (at < POOL) S.work[at] = i * NT + tid;
+            }
+        }
+        __syncthreads();
+        const uint32_t wanted = S.wanted, per = UNROLL * shared_by;
+        for (uint32_t i = tid; i < min(wanted, POOL) * per; i += NT) {
+            const uint32_t entry = S.work[i / per], j = piece_of(entry / NT, entry % NT) + i % per * NT;
+            if (j >= end) continue;
+            const uint4 p = load(j);
+#pragma unroll 1
+            for (uint32_t e = 0; e < V; e++) {
+                const uint32_t order = order_at(p, e), at = j * V - skip + e;
+                if (at < n && (above ? order > least : order >= least)) {
+                    const uint32_t to = atomicAdd(&S.found, 1u);
+                    if (to < POOL) S.keys[to] = key_of(order, at);
+                }
+            }
+        }
+        __syncthreads();
+        total = min(S.found, POOL);
+        if (S.found <= POOL && wanted <= POOL) break;
+        if (above) { // POOL of them are there: the order that fewer than k of these are above
+            if (tid == 0) S.raised = 0xFFFFFFFFu;
+            __syncthreads();
+            for (uint32_t i = tid; i < total; i += NT) {
+                const uint32_t mine = (uint32_t)(S.keys[i] >> 32);
+                uint32_t higher = 0;
+                for (uint32_t o = 0; o < total; o++) higher += (uint32_t)(S.keys[o] >> 32) > mine;
+                if (higher < k) atomicMin(&S.raised, mine);
+            }
+            __syncthreads();
+            least = S.raised;
+        }
+        above = true;
+        __syncthreads();
+        if (tid == 0) S.wanted = S.found = 0;
+        __syncthreads();
+    }
+    // Of those equal to the bound the first in the row, as many as are still needed.
+    if (above && total < k)
+        for (uint32_t j0 = begin; j0 < end && total < k; j0 += NT) {
+            uint32_t equal = 0; // bits of the thread's piece
+            if (j0 + tid < end) {
+                const uint4 p = load(j0 + tid);
+#pragma unroll 1
+                for (uint32_t e = 0; e < V; e++)
+                    if (order_at(p, e) == least && (j0 + tid) * V - skip + e < n) equal |= 1u << e;
+            }
+            uint32_t ahead = __popc(equal);
+#pragma unroll
+            for (uint32_t d = 1; d < 32; d *= 2) {
+                const uint32_t v = __shfl_up_sync(0xffffffffu, ahead, d);
+                if (lane >= d) ahead += v;
+            }
+            if (lane == 31) S.before[warp] = ahead;
+            __syncthreads();
+            uint32_t at = total + ahead - __popc(equal);
+            for (uint32_t w = 0; w < W; w++) {
+                if (w < warp) at += S.before[w];
+                total += S.before[w];
+            }
+            for (; equal && at < k; at++, equal &= equal - 1) S.keys[at] = key_of(least, (j0 + tid) * V - skip + __ffs(equal) - 1);
+            total = min(total, max(k, 1u));
+            __syncthreads();
+        }
+    if (tid < MAX_TOP) S.out[tid] = 0;
+    __syncthreads();
+    for (uint32_t i = tid; i < total; i += NT) {
+        const uint64_t mine = S.keys[i];
+        uint32_t higher = 0;
+#pragma unroll 4
+        for (uint32_t o = 0; o < total; o++) higher += S.keys[o] > mine;
+        if (higher < MAX_TOP) S.out[higher] = mine;
+    }
+    __syncthreads();
+    return S.out[lane];
+}
+
 // Block `rank` of the `parts` of row blockIdx.x / parts.
 template <typename T, int NT, bool TOP>
 __global__ void __launch_bounds__(NT, 1024 / NT)
 k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids, uint32_t k, uint32_t parts, Outputs out) {
     constexpr int W = NT / 32, V = PER_LOAD<T>;
-    __shared__ uint32_t first_max[W], bound, left;
-    __shared__ uint4 firsts[FIRSTS / 4];
+    extern __shared__ float notes[]; // [NOTES or fewer][NT]: the largest of a thread's logits in a tile; NaN: it has no number there
+    __shared__ uint32_t first_max[W];
     __shared__ Sums sums[W];
     __shared__ uint32_t counts[W], bads[W];
-    __shared__ uint64_t keys[TOP ? NT : 1], list_out[32];
+    __shared__ Best<TOP> top;
     // Of block 0: what the blocks of the cluster found.
     __shared__ Sums all_sums[MAX_CLUSTER];
     __shared__ uint32_t all_counts[MAX_CLUSTER], all_bads[MAX_CLUSTER];
@@ -227,7 +362,6 @@ k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids
     if (parts > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
     pdl_trigger();
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.x / parts, rank = blockIdx.x - row * parts;
-    if (tid == 0) bound = left = 0;
     pdl_wait();
     // The row in whole 16-byte pieces from the boundary below its start: piece j holds elements j * V - skip ...
     const T *l = logits + (size_t)row * stride;
@@ -257,84 +391,43 @@ k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids
     fetch(begin);
     const float given = id < n ? load1(l, id) : __int_as_float(0x7fc00000);
 
-    // What is read first gives the pivot and a bound that k values of the block reach.
-    uint32_t best = begin + tid < end ? order_of(largest<T>(now)) : 0; // (a thread with a NaN does not count)
-    const uint32_t warps = min((uint32_t)W, (end - begin + 31) / 32); // with something to read
-    uint32_t high = __reduce_max_sync(0xffffffffu, best);
-    if (lane == 0) first_max[warp] = high;
-    if constexpr (TOP) {
-        const uint32_t m = min(32u, FIRSTS / max(warps, 1u)); // of every warp, m * warps >= k
-        uint32_t *mine = reinterpret_cast<uint32_t *>(firsts) + warp * m;
-        if (warp < warps) {
-#pragma unroll 1
-            for (uint32_t i = 0; i < m; i++) {
-                if (lane == 0) mine[i] = high;
-                const uint32_t holders = __ballot_sync(0xffffffffu, best == high);
-                if (lane == (uint32_t)__ffs(holders) - 1) best = 0;
-                high = __reduce_max_sync(0xffffffffu, best);
-            }
-        }
-        for (uint32_t i = m * warps + tid; i < FIRSTS; i += NT) reinterpret_cast<uint32_t *>(firsts)[i] = 0;
-    }
+    // The largest of what is read first is the pivot.
+    const uint32_t first = __reduce_max_sync(0xffffffffu, order_of(largest<T>(now))); // (a thread with a NaN does not count)
+    if (lane == 0) first_max[warp] = first;
     __syncthreads();
-    const float top = value_of(max(__reduce_max_sync(0xffffffffu, first_max[lane % W]), 1u << 23)); // the lowest number where there is nothing (or NaN)
-    Sums a{fmaxf(top, LEAST) * LOG2E, 0.f, 0.f};
-    float limit = fminf(fmaf(SLACK, 1.f / LOG2E, fmaxf(top, LEAST)), MOST); // logits above it move the pivot
-    uint32_t least = 0; // values of a lower order do not matter any more; 0: all do
-    if constexpr (TOP) { // the least of those that fewer than k are above
-        const uint32_t x = reinterpret_cast<const uint32_t *>(firsts)[lane], y = reinterpret_cast<const uint32_t *>(firsts)[lane + 32];
-        uint32_t above_x = 0, above_y = 0;
-#pragma unroll 4
-        for (uint32_t i = 0; i < FIRSTS / 4; i++) {
-            const uint4 f = firsts[i];
-            above_x += (f.x > x) + (f.y > x) + (f.z > x) + (f.w > x);
-            above_y += (f.x > y) + (f.y > y) + (f.z > y) + (f.w > y);
-        }
-        least = __reduce_min_sync(0xffffffffu, min(above_x < k ? x : 0xFFFFFFFFu, above_y < k ? y : 0xFFFFFFFFu));
-        if (tid == 0) atomicMax(&bound, least);
-    }
-    float below = just_below(least);
+    const float start = value_of(max(__reduce_max_sync(0xffffffffu, first_max[lane % W]), 1u << 23)); // the lowest number where there is none
+    Sums a{fmaxf(start, LEAST) * LOG2E, 0.f, 0.f};
+    float limit = fminf(fmaf(SLACK, 1.f / LOG2E, fmaxf(start, LEAST)), MOST); // logits above it move the pivot
     bool bad = false, beyond = false, some = false; // a NaN or +infinity; a logit above MOST; one above -infinity
     uint32_t count = 0;
-    uint64_t list = 0;
+    const uint32_t tiles = (end - begin + UNROLL * NT - 1) / (UNROLL * NT), shared_by = (tiles + NOTES<NT> - 1) / NOTES<NT>; // tiles of a note
+    float note = __int_as_float(0x7fc00000);
+    uint32_t noted = 0, at_note = 0;
     float2 s2 = make_float2(0.f, 0.f), t2 = make_float2(0.f, 0.f);
 
 #pragma unroll 1
     for (uint32_t j0 = begin; j0 < end; j0 += UNROLL * NT) {
         const float highest = largest<T>(now);
-        if constexpr (TOP)
-            if (__any_sync(0xffffffffu, !(highest <= below))) { // some pieces are looked into, in the order of their indexes
-                least = max(least, *(volatile uint32_t *)&bound);
-#pragma unroll 1
-                for (int u = 0; u < UNROLL; u++) {
-                    const uint4 own[1] = {u == 0 ? now[0] : u == 1 ? now[1] : u == 2 ? now[2] : now[3]};
-                    uint32_t vote = __ballot_sync(0xffffffffu, !(largest<T>(own) <= below) && j0 + u * NT + tid < end);
-#pragma unroll 1
-                    while (vote) {
-                        const uint32_t src = __ffs(vote) - 1, first = (j0 + u * NT + 32 * warp + src) * V - skip;
-                        vote &= vote - 1;
-                        const uint4 piece = make_uint4(__shfl_sync(0xffffffffu, own[0].x, src), __shfl_sync(0xffffffffu, own[0].y, src),
-                                                       __shfl_sync(0xffffffffu, own[0].z, src), __shfl_sync(0xffffffffu, own[0].w, src));
-                        // Lane i looks at value i; those that may matter go in one after the other.
-                        const uint32_t i = lane % V, w = word(piece, sizeof(T) == 2 ? i / 2 : i), at = first + i;
-                        const uint32_t order = order_of(sizeof(T) == 4 ? __uint_as_float(w) : (i & 1) ? high_half(w) : low_half(w));
-                        uint32_t fit = __ballot_sync(0xffffffffu, lane < V && at < n && order >= least);
-#pragma unroll 1
-                        while (fit) {
-                            const uint64_t key = __shfl_sync(0xffffffffu, key_of(order, at), __ffs(fit) - 1);
-                            fit &= fit - 1;
-                            if ((uint32_t)(key >> 32) < least) continue; // (uniform)
-                            const uint32_t pos = __popc(__ballot_sync(0xffffffffu, list > key));
-                            const uint64_t up = __shfl_up_sync(0xffffffffu, list, 1);
-                            if (lane >= pos) list = lane == pos ? key : up;
-                            const uint64_t kth = __shfl_sync(0xffffffffu, list, k - 1);
-                            if (kth) least = max(least, (uint32_t)(kth >> 32) + 1); // later values have higher indexes
-                        }
+        if constexpr (TOP) {
+            float h = highest;
+            if (j0 < whole_from || j0 + UNROLL * NT > whole_to || h != h) { // only the row's numbers count
+                h = __int_as_float(0x7fc00000);
+#pragma unroll
+                for (int u = 0; u < UNROLL; u++)
+#pragma unroll
+                    for (int i = 0; i < V / 2; i++) {
+                        const float2 v = pair_of<T>(now[u], i);
+                        const uint32_t j = j0 + u * NT + tid, at = j * V - skip + 2 * i;
+                        if (j < end && at < n) h = fmaxf(h, v.x);
+                        if (j < end && at + 1 < n) h = fmaxf(h, v.y);
                     }
-                }
-                if (lane == k - 1 && list) atomicMax(&bound, (uint32_t)(list >> 32));
-                below = just_below(least);
             }
+            note = noted ? fmaxf(note, h) : h;
+            if (++noted == shared_by || j0 + UNROLL * NT >= end) {
+                notes[at_note++ * NT + tid] = note;
+                noted = 0;
+            }
+        }
         if (!(highest <= given)) {
             if constexpr (sizeof(T) == 2) { // ones added in bf16: 4 * UNROLL at most
                 const __nv_bfloat162 g = __float2bfloat162_rn(given);
@@ -391,32 +484,16 @@ k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids
         counts[warp] = count;
         bads[warp] = flags;
     }
-    __syncthreads();
+    uint64_t list = 0;
     if constexpr (TOP) {
-        const uint32_t kept = __ballot_sync(0xffffffffu, list != 0 && (uint32_t)(list >> 32) >= bound); // a list's first ones
-        uint32_t at = 0;
-        if (lane == 0 && kept) at = atomicAdd(&left, __popc(kept));
-        at = __shfl_sync(0xffffffffu, at, 0);
-        if (kept >> lane & 1) keys[at + lane] = list;
+        list = best_of<T, NT>(top, notes, at_note, shared_by, l, aligned, n, skip, begin, end, k);
+    } else {
+        __syncthreads();
     }
     if (warp == 0) {
         a = join_warp(lane < W ? sums[lane] : Sums{sums[0].c, 0.f, 0.f});
         count = __reduce_add_sync(0xffffffffu, lane < W ? counts[lane] : 0u);
         flags = __reduce_or_sync(0xffffffffu, lane < W ? bads[lane] : 0u);
-        if constexpr (TOP) list_out[lane] = 0;
-    }
-    if constexpr (TOP) {
-        __syncthreads();
-        const uint32_t total = left;
-        if (tid < total) {
-            const uint64_t mine = keys[tid];
-            uint32_t above = 0;
-#pragma unroll 4
-            for (uint32_t i = 0; i < total; i++) above += keys[i] > mine;
-            if (above < 32) list_out[above] = mine;
-        }
-        __syncthreads();
-        if (warp == 0) list = list_out[lane];
     }
     if (parts > 1) {
         asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
@@ -468,6 +545,17 @@ cudaError_t launch_shape(fq_device *dev, const T *logits, uint32_t n, size_t str
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(rows * parts);
     cfg.blockDim = dim3(NT);
+    const uint32_t pieces = (n + PER_LOAD<T> - 1) / PER_LOAD<T> + 1, tiles = (pieces + parts - 1) / parts / (UNROLL * NT) + 1;
+    cfg.dynamicSmemBytes = TOP ? std::min(tiles, NOTES<NT>) * NT * sizeof(float) : 0;
+    auto kernel = k_token_logprobs<T, NT, TOP>;
+    if (cfg.dynamicSmemBytes > (36 << 10)) { // with the kernel's own arrays beyond what it may use unasked: asked for once per device
+        static std::atomic<uint64_t> asked{0};
+        const uint64_t bit = 1ull << (dev->ordinal & 63);
+        if (!(asked.load(std::memory_order_relaxed) & bit) || dev->ordinal > 63) {
+            if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(NOTES<NT> * NT * sizeof(float)))) return e;
+            asked.fetch_or(bit, std::memory_order_relaxed);
+        }
+    }
     cfg.stream = dev->stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -477,7 +565,7 @@ cudaError_t launch_shape(fq_device *dev, const T *logits, uint32_t n, size_t str
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = parts > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, k_token_logprobs<T, NT, TOP>, logits, n, stride, ids, k, parts, out);
+    return cudaLaunchKernelEx(&cfg, kernel, logits, n, stride, ids, k, parts, out);
 }
 template <typename T>
 cudaError_t launch_rows(fq_device *dev, const T *logits, uint32_t n, size_t stride, uint32_t rows, const uint32_t *ids, uint32_t k, const Outputs &out) {
