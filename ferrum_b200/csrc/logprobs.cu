@@ -210,24 +210,23 @@ __device__ __forceinline__ void store_cluster(uint32_t to, uint32_t v) { asm vol
 template <bool TOP> struct Best { // shared memory of best_of
     uint4 firsts[FIRSTS / 4];
     uint64_t keys[POOL + MAX_TOP], out[MAX_TOP];
-    uint32_t work[POOL], wanted, found, raised, before[32];
+    uint32_t work[POOL], wanted, found, bound, before[32];
 };
 template <> struct Best<false> {};
 
 // The k best (value, index) keys of the block's pieces [begin, end), sorted, in the lanes of its first warp (0 where there are
-// fewer); all threads call it, after what they noted.
+// fewer); all threads call it, after what they noted (`noted` times, the largest `most`).
 template <typename T, int NT>
-__device__ __forceinline__ uint64_t best_of(Best<true> &S, const float *notes, uint32_t noted, uint32_t shared_by, const T *l, const uint4 *aligned, uint32_t n,
+__device__ __forceinline__ uint64_t best_of(Best<true> &S, const float *notes, uint32_t noted, float most, uint32_t shared_by, const T *l, const uint4 *aligned, uint32_t n,
                                             uint32_t skip, uint32_t begin, uint32_t end, uint32_t k) {
     constexpr uint32_t W = NT / 32, V = PER_LOAD<T>, TILE = UNROLL * NT;
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     uint32_t *firsts = reinterpret_cast<uint32_t *>(S.firsts);
     // This thread's first piece of a note; the threads that have one come first.
     auto piece_of = [&](uint32_t note, uint32_t thread) { return begin + note * shared_by * TILE + thread; };
-    float most = __int_as_float(0x7fc00000);
-    for (uint32_t i = 0; i < noted && piece_of(i, tid) < end; i++) most = fmaxf(most, notes[i * NT + tid]);
     uint32_t best = order_of(most); // a logit of the thread, or 0
-    const uint32_t warps = min(W, (end - begin + 31) / 32), m = min(32u, FIRSTS / max(warps, 1u)); // of every warp m maxima, m * warps >= k
+    const uint32_t warps = min(W, (end - begin + 31) / 32); // with something to read
+    const uint32_t m = min(min(32u, FIRSTS / max(warps, 1u)), 2 * k / max(warps, 1u) + 2); // maxima of every warp, m * warps >= k
     if (warp < warps) {
         uint32_t high = __reduce_max_sync(0xffffffffu, best);
 #pragma unroll 1
@@ -239,18 +238,25 @@ __device__ __forceinline__ uint64_t best_of(Best<true> &S, const float *notes, u
         }
     }
     for (uint32_t i = m * warps + tid; i < FIRSTS; i += NT) firsts[i] = 0;
-    if (tid == 0) S.wanted = S.found = 0;
+    if (tid == 0) {
+        S.wanted = S.found = 0;
+        S.bound = 0xFFFFFFFFu;
+    }
     __syncthreads();
     // The bound: the least of those that fewer than k are above.  0, below everything, where there are fewer than k.
-    uint32_t least, above_x = 0, above_y = 0;
-    const uint32_t x = firsts[lane], y = firsts[lane + 32];
+    if (tid < FIRSTS) {
+        const uint32_t mine = firsts[tid];
+        uint32_t higher = 0;
 #pragma unroll 4
-    for (uint32_t i = 0; i < FIRSTS / 4; i++) {
-        const uint4 f = S.firsts[i];
-        above_x += (f.x > x) + (f.y > x) + (f.z > x) + (f.w > x);
-        above_y += (f.x > y) + (f.y > y) + (f.z > y) + (f.w > y);
+        for (uint32_t i = 0; i < FIRSTS / 4; i++) {
+            const uint4 f = S.firsts[i];
+            higher += (f.x > mine) + (f.y > mine) + (f.z > mine) + (f.w > mine);
+        }
+        const uint32_t mine_or_more = __reduce_min_sync(0xffffffffu, higher < k ? mine : 0xFFFFFFFFu);
+        if (lane == 0) atomicMin(&S.bound, mine_or_more);
     }
-    least = __reduce_min_sync(0xffffffffu, min(above_x < k ? x : 0xFFFFFFFFu, above_y < k ? y : 0xFFFFFFFFu));
+    __syncthreads();
+    uint32_t least = S.bound;
     auto load = [&](uint32_t j) { return j * V - skip <= n && n - (j * V - skip) >= V ? __ldcg(aligned + j) : ends(l, n, j * V - skip); };
     auto order_at = [&](const uint4 &p, uint32_t i) {
         const uint32_t w = word(p, sizeof(T) == 2 ? i / 2 : i);
@@ -262,11 +268,15 @@ __device__ __forceinline__ uint64_t best_of(Best<true> &S, const float *notes, u
     uint32_t total;
     for (;;) {
         const float reach = value_of(least);
-        for (uint32_t i = 0; i < noted && piece_of(i, tid) < end; i++) {
-            const float v = notes[i * NT + tid];
-            if (least == 0 ? !above || v == v : above ? v > reach : v >= reach) {
-                const uint32_t at = atomicAdd(&S.wanted, 1u);
-                if (at < POOL) S.work[at] = i * NT + tid;
+        if (!(most < reach)) {
+            const uint32_t last = piece_of(noted - 1, tid) < end ? noted : noted - 1;
+#pragma unroll 4
+            for (uint32_t i = 0; i < last; i++) {
+                const float v = notes[i * NT + tid];
+                if (least == 0 ? !above || v == v : above ? v > reach : v >= reach) {
+                    const uint32_t at = atomicAdd(&S.wanted, 1u);
+                    if (at < POOL) S.work[at] = i * NT + tid;
+                }
             }
         }
         __syncthreads();
@@ -288,16 +298,16 @@ __device__ __forceinline__ uint64_t best_of(Best<true> &S, const float *notes, u
         total = min(S.found, POOL);
         if (S.found <= POOL && wanted <= POOL) break;
         if (above) { // POOL of them are there: the order that fewer than k of these are above
-            if (tid == 0) S.raised = 0xFFFFFFFFu;
+            if (tid == 0) S.bound = 0xFFFFFFFFu;
             __syncthreads();
             for (uint32_t i = tid; i < total; i += NT) {
                 const uint32_t mine = (uint32_t)(S.keys[i] >> 32);
                 uint32_t higher = 0;
                 for (uint32_t o = 0; o < total; o++) higher += (uint32_t)(S.keys[o] >> 32) > mine;
-                if (higher < k) atomicMin(&S.raised, mine);
+                if (higher < k) atomicMin(&S.bound, mine);
             }
             __syncthreads();
-            least = S.raised;
+            least = S.bound;
         }
         above = true;
         __syncthreads();
@@ -401,7 +411,7 @@ k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids
     bool bad = false, beyond = false, some = false; // a NaN or +infinity; a logit above MOST; one above -infinity
     uint32_t count = 0;
     const uint32_t tiles = (end - begin + UNROLL * NT - 1) / (UNROLL * NT), shared_by = (tiles + NOTES<NT> - 1) / NOTES<NT>; // tiles of a note
-    float note = __int_as_float(0x7fc00000);
+    float note = __int_as_float(0x7fc00000), most = note;
     uint32_t noted = 0, at_note = 0;
     float2 s2 = make_float2(0.f, 0.f), t2 = make_float2(0.f, 0.f);
 
@@ -425,6 +435,7 @@ k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids
             note = noted ? fmaxf(note, h) : h;
             if (++noted == shared_by || j0 + UNROLL * NT >= end) {
                 notes[at_note++ * NT + tid] = note;
+                most = fmaxf(most, note);
                 noted = 0;
             }
         }
@@ -486,7 +497,7 @@ k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids
     }
     uint64_t list = 0;
     if constexpr (TOP) {
-        list = best_of<T, NT>(top, notes, at_note, shared_by, l, aligned, n, skip, begin, end, k);
+        list = best_of<T, NT>(top, notes, at_note, most, shared_by, l, aligned, n, skip, begin, end, k);
     } else {
         __syncthreads();
     }
