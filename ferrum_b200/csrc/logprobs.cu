@@ -472,15 +472,18 @@ k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids
             }
         }
         const float2 b2 = make_float2(LOG2E, LOG2E), c2 = make_float2(-a.c, -a.c);
+        float2 s_tile = make_float2(0.f, 0.f), t_tile = s_tile; // (a sum of short sums rounds off less)
 #pragma unroll
         for (int u = 0; u < UNROLL; u++)
 #pragma unroll
             for (int i = 0; i < V / 2; i++) {
                 const float2 d = fma2(pair_from_least<T>(now[u], i), b2, c2);
                 const float2 e = make_float2(exp2_fast(d.x), exp2_fast(d.y));
-                s2 = add2(s2, e);
-                t2 = fma2(d, e, t2);
+                s_tile = add2(s_tile, e);
+                t_tile = fma2(d, e, t_tile);
             }
+        s2 = add2(s2, s_tile);
+        t2 = add2(t2, t_tile);
         if (j0 + UNROLL * NT < end) fetch(j0 + UNROLL * NT);
     }
     a.s = s2.x + s2.y;

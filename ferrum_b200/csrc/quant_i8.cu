@@ -10,7 +10,8 @@
 //
 // A row is read from memory once and kept in shared memory, every thread its own values of it.  v is computed in 32 bits; the
 // few values that decide are taken again in 64: those that may be the row's largest, by one thread while the others round, and
-// after it those whose quotient lies within the error of 32 bits of the border between two whole numbers.  Squares are added by fours in 32 bits and from there in 64.
+// after it those whose quotient lies within the error of 32 bits of the border between two whole numbers.  Squares are added by fours or
+// eights in 32 bits and from there in 64.
 // (Held in registers, unrolled over a row, the same took 105 registers and 63 instructions a value, a third of the time
 // waiting for instructions: 2048 x 5120 bf16 45 us.)
 #include <atomic>
@@ -24,52 +25,104 @@ using namespace fqk;
 
 enum Op { PLAIN, NORM, ADD_NORM, GLU };
 
-// Four values at a time.
-__device__ __forceinline__ float4 raw4(const float *p) { return __ldcg(reinterpret_cast<const float4 *>(p)); }
-__device__ __forceinline__ uint2 raw4(const __nv_bfloat16 *p) { return __ldcg(reinterpret_cast<const uint2 *>(p)); }
-__device__ __forceinline__ float4 floats(const float4 &v) { return v; }
-__device__ __forceinline__ float4 floats(const uint2 &b) {
-    return make_float4(__uint_as_float(b.x << 16), __uint_as_float(b.x & 0xFFFF0000u), __uint_as_float(b.y << 16), __uint_as_float(b.y & 0xFFFF0000u));
+// VEC values of a row at a time: 16 bytes, or 8 of bf16 rows whose length is no multiple of eight.
+template <int VEC> struct Vec { float2 p[VEC / 2]; };
+template <int VEC> struct Raw; // as they lie in memory
+template <> struct Raw<4> { uint2 u; };
+template <> struct Raw<8> { uint4 u; };
+__device__ __forceinline__ uint32_t word(const uint2 &u, int i) { return i == 0 ? u.x : u.y; }
+__device__ __forceinline__ uint32_t word(const uint4 &u, int i) { return i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w; }
+__device__ __forceinline__ float2 floats(uint32_t bf16x2) { return make_float2(__uint_as_float(bf16x2 << 16), __uint_as_float(bf16x2 & 0xFFFF0000u)); }
+template <int VEC> __device__ __forceinline__ Vec<VEC> floats(const Raw<VEC> &r) {
+    Vec<VEC> v;
+#pragma unroll
+    for (int i = 0; i < VEC / 2; i++) v.p[i] = floats(word(r.u, i));
+    return v;
 }
-template <typename T> __device__ __forceinline__ float4 load4(const T *p) { return floats(raw4(p)); }
+template <int VEC> __device__ __forceinline__ const Vec<VEC> &floats(const Vec<VEC> &v) { return v; }
+template <int VEC> __device__ __forceinline__ Vec<VEC> load(const float *p) { // (in shared memory too)
+    Vec<VEC> v;
+#pragma unroll
+    for (int i = 0; i < VEC / 4; i++) {
+        const float4 f = reinterpret_cast<const float4 *>(p)[i];
+        v.p[2 * i] = make_float2(f.x, f.y);
+        v.p[2 * i + 1] = make_float2(f.z, f.w);
+    }
+    return v;
+}
+template <int VEC> __device__ __forceinline__ void store(float *p, const Vec<VEC> &v) {
+#pragma unroll
+    for (int i = 0; i < VEC / 4; i++) reinterpret_cast<float4 *>(p)[i] = make_float4(v.p[2 * i].x, v.p[2 * i].y, v.p[2 * i + 1].x, v.p[2 * i + 1].y);
+}
+// Activations: of a kernel that may still run when this one starts, so past L1.
+template <int VEC> __device__ __forceinline__ Vec<VEC> fetch(const float *p) {
+    static_assert(VEC == 4, "16 bytes");
+    const float4 f = __ldcg(reinterpret_cast<const float4 *>(p));
+    return Vec<VEC>{make_float2(f.x, f.y), make_float2(f.z, f.w)};
+}
+template <int VEC> __device__ __forceinline__ Raw<VEC> fetch(const __nv_bfloat16 *p) {
+    if constexpr (VEC == 8) return Raw<VEC>{__ldcg(reinterpret_cast<const uint4 *>(p))};
+    else return Raw<VEC>{__ldcg(reinterpret_cast<const uint2 *>(p))};
+}
 __device__ __forceinline__ float load1(const float *p) { return __ldcg(p); }
 __device__ __forceinline__ float load1(const __nv_bfloat16 *p) { return __uint_as_float((uint32_t)__ldcg(reinterpret_cast<const unsigned short *>(p)) << 16); }
-// a + b, stored as its type keeps it, and as it is kept.
-__device__ __forceinline__ float4 add4(float *p, const float4 &a, const float4 &b) {
-    const float4 s = make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
-    *reinterpret_cast<float4 *>(p) = s;
+// a + b as its type keeps it; stored.  (Of bf16 numbers it is the same rounded once or by way of fp32: one that reaches below
+// the 24 bits of the other's sum is less than a 2^7th of half a step of it.)
+__device__ __forceinline__ Vec<4> sum_to(float *p, const Vec<4> &a, const Vec<4> &b) {
+    const Vec<4> s{__fadd2_rn(a.p[0], b.p[0]), __fadd2_rn(a.p[1], b.p[1])};
+    store<4>(p, s);
     return s;
 }
-__device__ __forceinline__ float4 add4(__nv_bfloat16 *p, const float4 &a, const float4 &b) {
-    const __nv_bfloat162 lo = __floats2bfloat162_rn(a.x + b.x, a.y + b.y), hi = __floats2bfloat162_rn(a.z + b.z, a.w + b.w);
-    const uint2 u = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
-    *reinterpret_cast<uint2 *>(p) = u;
-    return floats(u);
+__device__ __forceinline__ uint32_t sum_bf16x2(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 s = __hadd2(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&b));
+    return *reinterpret_cast<const uint32_t *>(&s);
 }
-__device__ __forceinline__ float max_abs(float a, float b) { // NaN if one is
+template <int VEC> __device__ __forceinline__ Vec<VEC> sum_to(__nv_bfloat16 *p, const Raw<VEC> &a, const Raw<VEC> &b) {
+    Raw<VEC> s;
+    s.u.x = sum_bf16x2(a.u.x, b.u.x);
+    s.u.y = sum_bf16x2(a.u.y, b.u.y);
+    if constexpr (VEC == 8) {
+        s.u.z = sum_bf16x2(a.u.z, b.u.z);
+        s.u.w = sum_bf16x2(a.u.w, b.u.w);
+    }
+    *reinterpret_cast<decltype(s.u) *>(p) = s.u;
+    return floats(s);
+}
+// The largest of |a|, |b|, |c|; NaN if one is.
+__device__ __forceinline__ float max_abs(float a, float b, float c) {
     float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-__device__ __forceinline__ float max_abs(const float4 &v) { return max_abs(max_abs(v.x, v.y), max_abs(v.z, v.w)); }
-// Two values an instruction.
-__device__ __forceinline__ float4 mul4(const float4 &a, const float4 &b) {
-    const float2 lo = __fmul2_rn(make_float2(a.x, a.y), make_float2(b.x, b.y)), hi = __fmul2_rn(make_float2(a.z, a.w), make_float2(b.z, b.w));
-    return make_float4(lo.x, lo.y, hi.x, hi.y);
+template <int VEC> __device__ __forceinline__ float max_abs(float m, const Vec<VEC> &v) {
+#pragma unroll
+    for (int i = 0; i < VEC / 2; i++) m = max_abs(m, v.p[i].x, v.p[i].y);
+    return m;
 }
-__device__ __forceinline__ float4 fma4(const float4 &a, float b, const float4 &c) {
-    const float2 b2 = make_float2(b, b);
-    const float2 lo = __ffma2_rn(make_float2(a.x, a.y), b2, make_float2(c.x, c.y)), hi = __ffma2_rn(make_float2(a.z, a.w), b2, make_float2(c.z, c.w));
-    return make_float4(lo.x, lo.y, hi.x, hi.y);
-}
-__device__ __forceinline__ float4 rsub4(float a, const float4 &b) { // a - b
-    const float2 lo = __fadd2_rn(make_float2(-b.x, -b.y), make_float2(a, a)), hi = __fadd2_rn(make_float2(-b.z, -b.w), make_float2(a, a));
-    return make_float4(lo.x, lo.y, hi.x, hi.y);
-}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 minus(const float2 &v) { return make_float2(-v.x, -v.y); }
 
-// silu(g) u.  Relative error: 2 steps (2^-22) of the exponential and as much of the quotient, two roundings: 10 * 2^-24; beyond
-// g = -87, where e^-g leaves the range of the quotient, 0 instead of less than 2^-118 |u|.
-__device__ __forceinline__ float gated(float g, float u) { return __fdividef(g, 1.f + expf(-g)) * u; }
+__device__ __forceinline__ float ex2(float v) { // within 2^-22.5 of itself
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float rcp(float v) { // within 2^-23 of itself
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+// silu(g) u for two values, e^-g = 2^t (1 + d ln 2) with t = -g log2 e rounded and d what the rounding took.  Relative error at
+// most 10 * 2^-24: 5 of the exponential, 1 of 1 + e^-g, 2 of its reciprocal and one of each product.  Beyond g = -87, where t is
+// held at 126, it is off by less than 2^-118 |u|.
+__device__ __forceinline__ float2 gated(const float2 &g, const float2 &u) {
+    constexpr float LOG2E = 1.44269502f, LOG2E_REST = 1.92596299e-8f, LN2 = 0.693147182f;
+    const float2 t = __fmul2_rn(g, both(-LOG2E));
+    const float2 d = __ffma2_rn(g, both(-LOG2E_REST), __ffma2_rn(g, both(-LOG2E), minus(t)));
+    const float2 e = make_float2(ex2(fminf(t.x, 126.f)), ex2(fminf(t.y, 126.f)));
+    const float2 s = __fadd2_rn(__ffma2_rn(__fmul2_rn(d, both(LN2)), e, e), both(1.f));
+    return __fmul2_rn(__fmul2_rn(g, make_float2(rcp(s.x), rcp(s.y))), u);
+}
 __device__ __forceinline__ double gated64(double g, double u) { return g / (1.0 + exp(-g)) * u; }
 
 // The part of a quotient t = 127 v / a that its computation in 32 bits may be off: v and a as above or (norms) once rounded,
@@ -84,12 +137,12 @@ constexpr float LEAST = 1e-20f, MOST = 1e37f;
 template <int OP> constexpr float LEAST_2 = OP == NORM || OP == ADD_NORM ? 1e-20f : 0.f;
 template <int OP> constexpr float MOST_2 = OP == GLU ? 1048576.f : 1e37f;
 
-// NT threads per row: a block, or one of its eight warps.  STAGED: the row is kept in shared memory (for the norms h, otherwise
-// v); longer rows are computed again from memory for every step.
-template <int OP, typename T, int NT, bool STAGED>
-__global__ void __launch_bounds__(NT == 32 ? 256 : NT, NT == 512 ? 2 : 5)
+// NT threads per row: a block, or one of its eight warps.  STAGED: the row's v is kept in shared memory, every thread its own
+// values of it; of longer rows it is computed again from memory.
+template <int OP, typename T, int VEC, int NT, bool STAGED>
+__global__ void __launch_bounds__(NT == 32 ? 256 : NT, NT == 32 ? 5 : 1280 / NT)
 k_rows_i8(const T *x, const T *r, const float *w, uint32_t n, float eps, uint32_t rows, T *h, int8_t *q, float *scales) {
-    constexpr bool IS_NORM = OP == NORM || OP == ADD_NORM, ONE_WARP = NT == 32;
+    constexpr bool IS_NORM = OP == NORM || OP == ADD_NORM, TWO = OP == ADD_NORM || OP == GLU, ONE_WARP = NT == 32;
     constexpr int W = NT / 32;
     extern __shared__ float4 stage[];
     __shared__ double part_ss[W];
@@ -97,33 +150,32 @@ k_rows_i8(const T *x, const T *r, const float *w, uint32_t n, float eps, uint32_
     __shared__ unsigned long long largest;
     pdl_trigger();
     const uint32_t lane = threadIdx.x & 31, warp = ONE_WARP ? 0 : threadIdx.x >> 5, tid = ONE_WARP ? lane : threadIdx.x;
-    const uint32_t row = ONE_WARP ? blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x, n4 = n / 4;
+    const uint32_t row = ONE_WARP ? blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x, groups = n / VEC;
     if (!ONE_WARP && tid == 0) largest = 0;
     pdl_wait();
     if (row >= rows) return; // whole warps
-    float4 *const kept = stage + (ONE_WARP ? (threadIdx.x >> 5) * n4 : 0);
+    float *const kept = reinterpret_cast<float *>(stage) + (ONE_WARP ? (threadIdx.x >> 5) * n : 0);
     x += (size_t)row * n;
-    if constexpr (OP == ADD_NORM || OP == GLU) r += (size_t)row * n;
+    if constexpr (TWO) r += (size_t)row * n;
     if constexpr (OP == ADD_NORM) h += (size_t)row * n;
-    uint32_t *const out = reinterpret_cast<uint32_t *>(q + (size_t)row * n);
-    const float4 *const w4 = reinterpret_cast<const float4 *>(w);
+    q += (size_t)row * n;
 
-    auto values = [&](const float4 &a, const float4 &b) {
-        if constexpr (OP == PLAIN) return a;
-        else if constexpr (OP == GLU) return make_float4(gated(a.x, b.x), gated(a.y, b.y), gated(a.z, b.z), gated(a.w, b.w));
-        else return mul4(a, b);
+    auto product = [](const Vec<VEC> &a, const Vec<VEC> &b) {
+        Vec<VEC> v;
+#pragma unroll
+        for (int i = 0; i < VEC / 2; i++) v.p[i] = OP == GLU ? gated(a.p[i], b.p[i]) : __fmul2_rn(a.p[i], b.p[i]);
+        return v;
     };
-    // v of group i of four, after the row has been read once.
+    // v of group i, after the row has been read once.
     auto again = [&](uint32_t i) {
-        if constexpr (STAGED) return IS_NORM ? values(kept[i], w4[i]) : kept[i];
-        else if constexpr (OP == ADD_NORM) return values(load4((const T *)h + 4 * i), w4[i]);
-        else if constexpr (OP == NORM) return values(load4(x + 4 * i), w4[i]);
-        else if constexpr (OP == GLU) return values(load4(x + 4 * i), load4(r + 4 * i));
-        else return load4(x + 4 * i);
+        if constexpr (STAGED) return load<VEC>(kept + VEC * i);
+        else if constexpr (OP == PLAIN) return Vec<VEC>(floats(fetch<VEC>(x + VEC * i)));
+        else if constexpr (OP == GLU) return product(floats(fetch<VEC>(x + VEC * i)), floats(fetch<VEC>(r + VEC * i)));
+        else return product(floats(fetch<VEC>((OP == ADD_NORM ? (const T *)h : x) + VEC * i)), load<VEC>(w + VEC * i));
     };
-    // Value i in 64 bits.  (In memory a thread has written its own values of h.)
+    // Value i in 64 bits, from memory.  (Of h this thread has written its own values there.)
     auto exact = [&](uint32_t i) {
-        const float a = STAGED && OP != GLU ? reinterpret_cast<const float *>(kept)[i] : load1(OP == ADD_NORM ? (const T *)h + i : x + i);
+        const float a = load1(OP == ADD_NORM ? (const T *)h + i : x + i);
         if constexpr (OP == PLAIN) return (double)a;
         else if constexpr (OP == GLU) return gated64((double)a, (double)load1(r + i));
         else return (double)a * (double)w[i];
@@ -131,30 +183,39 @@ k_rows_i8(const T *x, const T *r, const float *w, uint32_t n, float eps, uint32_
 
     double ss = 0.0;
     float own = 0.f, own_2 = 0.f;
-    auto take = [&](uint32_t i, float4 a, float4 b) {
-        if constexpr (OP == ADD_NORM) a = add4(h + 4 * i, a, b);
-        if constexpr (IS_NORM) {
-            const float squares = fmaf(a.x, a.x, a.y * a.y) + fmaf(a.z, a.z, a.w * a.w);
-            ss += (double)squares;
-            own_2 = max_abs(own_2, squares);
-        }
-        if constexpr (OP == GLU) own_2 = max_abs(own_2, max_abs(b));
-        const float4 v = IS_NORM ? values(a, w4[i]) : values(a, b);
-        own = max_abs(own, max_abs(v));
-        if constexpr (STAGED) kept[i] = IS_NORM ? a : v;
-    };
-    constexpr uint32_t AHEAD = sizeof(T) == 2 ? 4 : 2; // loads of either input that are under way together
-    for (uint32_t i = tid; i < n4; i += AHEAD * NT) {
-        decltype(raw4(x)) a[AHEAD], b[AHEAD];
+    constexpr uint32_t AHEAD = sizeof(T) * VEC == 16 ? 2 : 4; // loads of either input that are under way together
+    for (uint32_t i = tid; i < groups; i += AHEAD * NT) {
+        decltype(fetch<VEC>(x)) a[AHEAD], b[AHEAD];
 #pragma unroll
         for (uint32_t j = 0; j < AHEAD; j++)
-            if (i + j * NT < n4) {
-                a[j] = raw4(x + 4 * (i + j * NT));
-                if constexpr (OP == ADD_NORM || OP == GLU) b[j] = raw4(r + 4 * (i + j * NT));
+            if (i + j * NT < groups) {
+                a[j] = fetch<VEC>(x + VEC * (i + j * NT));
+                if constexpr (TWO) b[j] = fetch<VEC>(r + VEC * (i + j * NT));
             }
 #pragma unroll
-        for (uint32_t j = 0; j < AHEAD; j++)
-            if (i + j * NT < n4) take(i + j * NT, floats(a[j]), floats(b[j]));
+        for (uint32_t j = 0; j < AHEAD; j++) {
+            if (i + j * NT >= groups) break;
+            const uint32_t at = VEC * (i + j * NT);
+            Vec<VEC> v;
+            if constexpr (OP == ADD_NORM) v = sum_to(h + at, a[j], b[j]);
+            else v = floats(a[j]);
+            if constexpr (IS_NORM) {
+                float2 squares = __fmul2_rn(v.p[0], v.p[0]);
+#pragma unroll
+                for (int k = 1; k < VEC / 2; k++) squares = __ffma2_rn(v.p[k], v.p[k], squares);
+                const float sum = squares.x + squares.y;
+                ss += (double)sum;
+                own_2 = max_abs(own_2, sum, sum);
+                v = product(v, load<VEC>(w + at));
+            }
+            if constexpr (OP == GLU) {
+                const Vec<VEC> u = floats(b[j]);
+                own_2 = max_abs(own_2, u);
+                v = product(v, u);
+            }
+            own = max_abs(own, v);
+            if constexpr (STAGED) store<VEC>(kept + at, v);
+        }
     }
     if constexpr (IS_NORM)
 #pragma unroll
@@ -179,23 +240,26 @@ k_rows_i8(const T *x, const T *r, const float *w, uint32_t n, float eps, uint32_
     uint32_t near = 0; // groups of the thread with a value next to a border
     if (fast) {
         if (__float_as_uint(own) >= most - BELOW<OP>)
-            for (uint32_t i = tid; i < n4; i += NT) {
-                const float4 v = again(i);
+            for (uint32_t i = tid; i < groups; i += NT) {
+                const Vec<VEC> v = again(i);
+                if (__float_as_uint(max_abs(0.f, v)) >= most - BELOW<OP>)
 #pragma unroll 1
-                for (uint32_t k = 0; k < 4; k++)
-                    if (__float_as_uint(fabsf(k == 0 ? v.x : k == 1 ? v.y : k == 2 ? v.z : v.w)) >= most - BELOW<OP>) a64 = fmax(a64, fabs(exact(4 * i + k)));
+                    for (uint32_t k = 0; k < VEC; k++) {
+                        const double e = fabs(exact(VEC * i + k)); // (those below the largest do no harm)
+                        a64 = fmax(a64, e);
+                    }
             }
         if (!ONE_WARP && a64 > 0.0) atomicMax(&largest, (unsigned long long)__double_as_longlong(a64));
     } else {
         ss = 0.0;
-        for (uint32_t i = tid; i < n4; i += NT)
+        for (uint32_t i = tid; i < groups; i += NT)
 #pragma unroll 1
-            for (uint32_t k = 0; k < 4; k++) {
-                const double v = fabs(exact(4 * i + k));
+            for (uint32_t k = 0; k < VEC; k++) {
+                const double v = fabs(exact(VEC * i + k));
                 bad |= !(v <= 3.4028234663852886e38);
                 a64 = fmax(a64, v);
                 if constexpr (IS_NORM) {
-                    const double a = (double)load1(OP == ADD_NORM ? (const T *)h + 4 * i + k : x + 4 * i + k);
+                    const double a = (double)load1(OP == ADD_NORM ? (const T *)h + VEC * i + k : x + VEC * i + k);
                     ss = fma(a, a, ss);
                 }
             }
@@ -207,17 +271,26 @@ k_rows_i8(const T *x, const T *r, const float *w, uint32_t n, float eps, uint32_
         }
     }
     // t = 127 v / a: added to 1.5 * 2^23 it is rounded to a whole number, whose low byte is the sum's; `rest` is what that took.
-    constexpr float MAGIC = 12582912.f;
-    const float f = 127.f / __uint_as_float(most);
-    auto rests = [&](const float4 &v, const float4 &whole) { return fma4(v, f, rsub4(MAGIC, whole)); };
-    auto wholes = [&](const float4 &v) { return fma4(v, f, make_float4(MAGIC, MAGIC, MAGIC, MAGIC)); };
+    const float2 magic = both(12582912.f), f = both(127.f / __uint_as_float(most));
+    auto whole_of = [&](const float2 &v) { return __ffma2_rn(v, f, magic); };
+    auto rest_of = [&](const float2 &v, const float2 &whole) { return __ffma2_rn(v, f, __fadd2_rn(minus(whole), magic)); };
+    auto low_bytes = [](const float2 &a, const float2 &b) {
+        return __byte_perm(__byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040), __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040), 0x5410);
+    };
     if (fast) { // while the largest value is taken in 64 bits elsewhere
         uint32_t at = 0;
 #pragma unroll 2
-        for (uint32_t i = tid; i < n4; i += NT, at++) {
-            const float4 v = again(i), whole = wholes(v);
-            out[i] = __byte_perm(__byte_perm(__float_as_uint(whole.x), __float_as_uint(whole.y), 0x0040), __byte_perm(__float_as_uint(whole.z), __float_as_uint(whole.w), 0x0040), 0x5410);
-            if (max_abs(rests(v, whole)) > 0.5f - 128 * OFF<OP>) near |= 1u << (at & 31);
+        for (uint32_t i = tid; i < groups; i += NT, at++) {
+            const Vec<VEC> v = again(i);
+            Vec<VEC> whole, rest;
+#pragma unroll
+            for (int k = 0; k < VEC / 2; k++) {
+                whole.p[k] = whole_of(v.p[k]);
+                rest.p[k] = rest_of(v.p[k], whole.p[k]);
+            }
+            if constexpr (VEC == 8) *reinterpret_cast<uint2 *>(q + VEC * i) = make_uint2(low_bytes(whole.p[0], whole.p[1]), low_bytes(whole.p[2], whole.p[3]));
+            else *reinterpret_cast<uint32_t *>(q + VEC * i) = low_bytes(whole.p[0], whole.p[1]);
+            if (max_abs(0.f, rest) > 0.5f - 128 * OFF<OP>) near |= 1u << (at & 31);
         }
     }
     if constexpr (ONE_WARP) {
@@ -240,40 +313,42 @@ k_rows_i8(const T *x, const T *r, const float *w, uint32_t n, float eps, uint32_
         scales[row] = bad ? __int_as_float(0x7fc00000) : (float)(a64 * c / 127.0);
     }
 
-    auto rounded = [&](uint32_t i) { return (uint32_t)__double2int_rn(exact(i) * 127.0 / a64) & 0xFFu; };
+    auto rounded = [&](uint32_t i) { return (int8_t)__double2int_rn(exact(i) * 127.0 / a64); };
     if (fast) {
         // Values that may be on the wrong side of a border, by their own size (bit b of `near`: groups b, b + 32, ...).
         while (near) {
             const uint32_t b = __ffs(near) - 1;
             near &= near - 1;
-            for (uint32_t i = tid + b * NT; i < n4; i += 32 * NT) {
-                const float4 v = again(i), whole = wholes(v), rest = rests(v, whole);
-#pragma unroll 1
-                for (uint32_t k = 0; k < 4; k++) {
-                    const float e = k == 0 ? v.x : k == 1 ? v.y : k == 2 ? v.z : v.w, part = k == 0 ? rest.x : k == 1 ? rest.y : k == 2 ? rest.z : rest.w;
-                    if (fabsf(part) > 0.5f - (fabsf(e * f) + 0.5f) * OFF<OP>) reinterpret_cast<uint8_t *>(out)[4 * i + k] = (uint8_t)rounded(4 * i + k);
+            for (uint32_t i = tid + b * NT; i < groups; i += 32 * NT) {
+                const Vec<VEC> v = again(i);
+                uint32_t which = 0;
+#pragma unroll
+                for (int k = 0; k < VEC / 2; k++) {
+                    const float2 rest = rest_of(v.p[k], whole_of(v.p[k]));
+                    if (fabsf(rest.x) > 0.5f - (fabsf(v.p[k].x * f.x) + 0.5f) * OFF<OP>) which |= 1u << (2 * k);
+                    if (fabsf(rest.y) > 0.5f - (fabsf(v.p[k].y * f.x) + 0.5f) * OFF<OP>) which |= 2u << (2 * k);
+                }
+                for (; which; which &= which - 1) {
+                    const uint32_t at = VEC * i + __ffs(which) - 1;
+                    q[at] = rounded(at);
                 }
             }
         }
     } else {
-        for (uint32_t i = tid; i < n4; i += NT) {
-            uint32_t packed = 0;
-            if (!bad && a64 > 0.0)
+        for (uint32_t i = tid; i < groups; i += NT)
 #pragma unroll 1
-                for (uint32_t k = 0; k < 4; k++) packed |= rounded(4 * i + k) << (8 * k);
-            out[i] = packed;
-        }
+            for (uint32_t k = 0; k < VEC; k++) q[VEC * i + k] = !bad && a64 > 0.0 ? rounded(VEC * i + k) : 0;
     }
 }
 
 constexpr size_t STAGE_MOST = 200 << 10;
 
-template <int OP, typename T, int NT>
+template <int OP, typename T, int VEC, int NT>
 cudaError_t launch_nt(fq_device *dev, const T *x, const T *r, const float *w, uint32_t n, float eps, uint32_t rows, T *h, int8_t *q, float *scales) {
     const size_t bytes = (size_t)n * 4 * (NT == 32 ? 8 : 1);
     const dim3 grid(NT == 32 ? (rows + 7) / 8 : rows), block(NT == 32 ? 256 : NT);
-    if (bytes > STAGE_MOST) return launch_pdl(k_rows_i8<OP, T, NT, false>, grid, block, 0, dev->stream, x, r, w, n, eps, rows, h, q, scales);
-    auto kernel = k_rows_i8<OP, T, NT, true>;
+    if (bytes > STAGE_MOST) return launch_pdl(k_rows_i8<OP, T, VEC, NT, false>, grid, block, 0, dev->stream, x, r, w, n, eps, rows, h, q, scales);
+    auto kernel = k_rows_i8<OP, T, VEC, NT, true>;
     if (bytes > (40 << 10)) { // beyond what a kernel may use unasked (48 KB with its own arrays): asked for once per device
         static std::atomic<uint64_t> asked{0};
         const uint64_t bit = 1ull << (dev->ordinal & 63);
@@ -285,17 +360,23 @@ cudaError_t launch_nt(fq_device *dev, const T *x, const T *r, const float *w, ui
     return launch_pdl(kernel, grid, block, bytes, dev->stream, x, r, w, n, eps, rows, h, q, scales);
 }
 
+template <int OP, typename T, int VEC>
+cudaError_t launch_vec(fq_device *dev, const void *x, const void *r, const float *w, uint32_t n, float eps, uint32_t rows, void *h, int8_t *q, float *scales) {
+    const T *tx = (const T *)x, *tr = (const T *)r;
+    const bool few = rows <= 2 * (uint32_t)dev->sm_count;
+    const uint32_t groups = n / VEC;
+    if (n <= 1024) return launch_nt<OP, T, VEC, 32>(dev, tx, tr, w, n, eps, rows, (T *)h, q, scales);
+    if (groups > (few ? 512 : 2600)) return launch_nt<OP, T, VEC, 512>(dev, tx, tr, w, n, eps, rows, (T *)h, q, scales);
+    if (groups > (few ? 256 : 800)) return launch_nt<OP, T, VEC, 256>(dev, tx, tr, w, n, eps, rows, (T *)h, q, scales);
+    return launch_nt<OP, T, VEC, 128>(dev, tx, tr, w, n, eps, rows, (T *)h, q, scales);
+}
+
 template <int OP>
 int launch_rows(fq_device *dev, const char *what, const void *x, const void *r, int dtype, const float *w, uint32_t n, float eps, uint32_t rows,
                 void *h, int8_t *q, float *scales) {
-    auto shape = [&](auto zero) {
-        using T = decltype(zero);
-        const T *tx = (const T *)x, *tr = (const T *)r;
-        if (n <= 1024) return launch_nt<OP, T, 32>(dev, tx, tr, w, n, eps, rows, (T *)h, q, scales);
-        if (n > 8192 || rows <= 2 * (uint32_t)dev->sm_count) return launch_nt<OP, T, 512>(dev, tx, tr, w, n, eps, rows, (T *)h, q, scales);
-        return launch_nt<OP, T, 256>(dev, tx, tr, w, n, eps, rows, (T *)h, q, scales);
-    };
-    const cudaError_t e = dtype == FQ_BF16 ? shape(__nv_bfloat16{}) : shape(float{});
+    const cudaError_t e = dtype == FQ_F32 ? launch_vec<OP, float, 4>(dev, x, r, w, n, eps, rows, h, q, scales)
+                          : n % 8 == 0    ? launch_vec<OP, __nv_bfloat16, 8>(dev, x, r, w, n, eps, rows, h, q, scales)
+                                          : launch_vec<OP, __nv_bfloat16, 4>(dev, x, r, w, n, eps, rows, h, q, scales);
     if (int rc = fq_check_cuda(dev, e, what)) return rc;
     return fq_end_enqueue(dev, what, 1);
 }

@@ -139,9 +139,14 @@ def test_rows_of_extreme_values(device, op, n, dtype):
     r[0] = 0 if op != "glu" else r[0]
     if op == "glu":
         r[7] = 0
+    x[8], r[8] = x[8] * 2.0 ** -130, r[8] * 2.0 ** -131  # a sum of subnormal numbers
+    x[9] *= 2.0 ** (rng.integers(-30, 30, n))            # and sums that lose the smaller one's last bits
     x, r, w = gpu(x, dtype), gpu(r, dtype), gpu(1 + 0.1 * rng.standard_normal(n))
-    q, s = run_op(device, op, x, r, w, 12, torch.zeros_like(x))
+    h = torch.zeros_like(x)
+    q, s = run_op(device, op, x, r, w, 12, h)
     check_rows(op, x, r, w, q, s)
+    if op == "add":
+        assert torch.equal(h.cpu(), values_of(op, x, r, w)[2])
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
