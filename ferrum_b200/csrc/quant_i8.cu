@@ -14,14 +14,22 @@
 // eights in 32 bits and from there in 64.
 // (Held in registers, unrolled over a row, the same took 105 registers and 63 instructions a value, a third of the time
 // waiting for instructions: 2048 x 5120 bf16 45 us.)
+#include <algorithm>
 #include <atomic>
 #include <type_traits>
 
 #include "gemv_common.cuh"
 #include "internal.h"
+#include "tcgen05.cuh"
 
 namespace {
 using namespace fqk;
+using namespace fqtc;
+
+struct Arrivals { // of a block's bulk copies
+    uint64_t full[2];
+    uint32_t abort_flag;
+};
 
 enum Op { PLAIN, NORM, ADD_NORM, GLU };
 
@@ -137,28 +145,56 @@ constexpr float LEAST = 1e-20f, MOST = 1e37f;
 template <int OP> constexpr float LEAST_2 = OP == NORM || OP == ADD_NORM ? 1e-20f : 0.f;
 template <int OP> constexpr float MOST_2 = OP == GLU ? 1048576.f : 1e37f;
 
-// NT threads per row: a block, or one of its eight warps.  STAGED: the row's v is kept in shared memory, every thread its own
-// values of it; of longer rows it is computed again from memory.
-template <int OP, typename T, int VEC, int NT, bool STAGED>
+// Where a thread's values of a row are between its steps.
+enum Mode {
+    DIRECT, // nowhere: v is computed again from memory (rows longer than shared memory)
+    KEPT,   // v in shared memory, read from memory by the threads
+    BULK    // bulk copies bring the inputs to shared memory, where v takes their place
+};
+
+// NT threads per row: a block, or one of its eight warps.  With BULK blocks walk the rows, `stages` of them on their way or in
+// work at a time; a stage is the row of x and, of the same size, the row of r or room for the other half of v.
+template <int OP, typename T, int VEC, int NT, int MODE>
 __global__ void __launch_bounds__(NT == 32 ? 256 : NT, NT == 32 ? 5 : 1280 / NT)
-k_rows_i8(const T *x, const T *r, const float *w, uint32_t n, float eps, uint32_t rows, T *h, int8_t *q, float *scales) {
+k_rows_i8(const T *x0, const T *r0, const float *w, uint32_t n, float eps, uint32_t rows, T *h0, int8_t *q0, float *scales, double inv_n, uint32_t stages, int *status) {
     constexpr bool IS_NORM = OP == NORM || OP == ADD_NORM, TWO = OP == ADD_NORM || OP == GLU, ONE_WARP = NT == 32;
     constexpr int W = NT / 32;
     extern __shared__ float4 stage[];
-    __shared__ double part_ss[W];
+    __shared__ double all_ss[2][W]; // rows alternate between two of each
     __shared__ uint32_t part_max[W], part_2[W];
-    __shared__ unsigned long long largest;
+    __shared__ unsigned long long all_largest[2];
+    __shared__ Arrivals arrivals;
     pdl_trigger();
     const uint32_t lane = threadIdx.x & 31, warp = ONE_WARP ? 0 : threadIdx.x >> 5, tid = ONE_WARP ? lane : threadIdx.x;
-    const uint32_t row = ONE_WARP ? blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x, groups = n / VEC;
-    if (!ONE_WARP && tid == 0) largest = 0;
+    const uint32_t first = ONE_WARP ? blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x, groups = n / VEC, half = n * (uint32_t)sizeof(T);
+    if (!ONE_WARP && tid == 0) all_largest[0] = all_largest[1] = 0;
+    if (MODE == BULK && tid == 0) {
+        for (uint32_t s = 0; s < stages; s++) mbar_init(&arrivals.full[s], 1);
+        arrivals.abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
     pdl_wait();
-    if (row >= rows) return; // whole warps
-    float *const kept = reinterpret_cast<float *>(stage) + (ONE_WARP ? (threadIdx.x >> 5) * n : 0);
-    x += (size_t)row * n;
-    if constexpr (TWO) r += (size_t)row * n;
-    if constexpr (OP == ADD_NORM) h += (size_t)row * n;
-    q += (size_t)row * n;
+    if (first >= rows) return; // whole warps
+    uint8_t *const base = reinterpret_cast<uint8_t *>(stage) + (ONE_WARP ? (threadIdx.x >> 5) * n * 4 : 0);
+    auto ask = [&](uint32_t row, uint32_t s) { // one thread
+        mbar_expect_tx(&arrivals.full[s], TWO ? 2 * half : half);
+        bulk_load(base + s * 2 * half, x0 + (size_t)row * n, half, &arrivals.full[s]);
+        if constexpr (TWO) bulk_load(base + s * 2 * half + half, r0 + (size_t)row * n, half, &arrivals.full[s]);
+    };
+    if constexpr (MODE == BULK) {
+        __syncthreads();
+        if (tid == 0)
+            for (uint32_t s = 0; s < stages && first + s * gridDim.x < rows; s++) ask(first + s * gridDim.x, s);
+    }
+    uint32_t s = 0, phase = 0, parity = 0;
+  for (uint32_t row = first; row < rows; row += MODE == BULK ? gridDim.x : rows, parity ^= 1) {
+    const T *const x = x0 + (size_t)row * n, *const r = TWO ? r0 + (size_t)row * n : nullptr;
+    T *const h = OP == ADD_NORM ? h0 + (size_t)row * n : nullptr;
+    int8_t *const q = q0 + (size_t)row * n;
+    double *const part_ss = all_ss[parity];
+    uint8_t *const kept = base + s * 2 * half; // of group i the VEC * sizeof(T) bytes at i and the same at `half` + i: v, its halves
+    bool late = false;
+    if constexpr (MODE == BULK) late = !mbar_wait(&arrivals.full[s], phase, &arrivals, status);
 
     auto product = [](const Vec<VEC> &a, const Vec<VEC> &b) {
         Vec<VEC> v;
@@ -168,7 +204,11 @@ k_rows_i8(const T *x, const T *r, const float *w, uint32_t n, float eps, uint32_
     };
     // v of group i, after the row has been read once.
     auto again = [&](uint32_t i) {
-        if constexpr (STAGED) return load<VEC>(kept + VEC * i);
+        if constexpr (MODE == KEPT) return load<VEC>(reinterpret_cast<const float *>(kept) + VEC * i);
+        else if constexpr (MODE == BULK && VEC == 8) {
+            const Vec<4> lo = load<4>(reinterpret_cast<const float *>(kept) + 4 * i), hi = load<4>(reinterpret_cast<const float *>(kept + half) + 4 * i);
+            return Vec<VEC>{lo.p[0], lo.p[1], hi.p[0], hi.p[1]};
+        } else if constexpr (MODE == BULK) return load<VEC>(reinterpret_cast<const float *>(kept) + VEC * i);
         else if constexpr (OP == PLAIN) return Vec<VEC>(floats(fetch<VEC>(x + VEC * i)));
         else if constexpr (OP == GLU) return product(floats(fetch<VEC>(x + VEC * i)), floats(fetch<VEC>(r + VEC * i)));
         else return product(floats(fetch<VEC>((OP == ADD_NORM ? (const T *)h : x) + VEC * i)), load<VEC>(w + VEC * i));
@@ -183,38 +223,53 @@ k_rows_i8(const T *x, const T *r, const float *w, uint32_t n, float eps, uint32_
 
     double ss = 0.0;
     float own = 0.f, own_2 = 0.f;
-    constexpr uint32_t AHEAD = sizeof(T) * VEC == 16 ? 2 : 4; // loads of either input that are under way together
-    for (uint32_t i = tid; i < groups; i += AHEAD * NT) {
-        decltype(fetch<VEC>(x)) a[AHEAD], b[AHEAD];
+    auto take = [&](uint32_t i, const decltype(fetch<VEC>(x)) &a, const decltype(fetch<VEC>(x)) &b) {
+        const uint32_t at = VEC * i;
+        Vec<VEC> v;
+        if constexpr (OP == ADD_NORM) v = sum_to(h + at, a, b);
+        else v = floats(a);
+        if constexpr (IS_NORM) {
+            float2 squares = __fmul2_rn(v.p[0], v.p[0]);
 #pragma unroll
-        for (uint32_t j = 0; j < AHEAD; j++)
-            if (i + j * NT < groups) {
-                a[j] = fetch<VEC>(x + VEC * (i + j * NT));
-                if constexpr (TWO) b[j] = fetch<VEC>(r + VEC * (i + j * NT));
-            }
+            for (int k = 1; k < VEC / 2; k++) squares = __ffma2_rn(v.p[k], v.p[k], squares);
+            const float sum = squares.x + squares.y;
+            ss += (double)sum;
+            own_2 = max_abs(own_2, sum, sum);
+            v = product(v, load<VEC>(w + at));
+        }
+        if constexpr (OP == GLU) {
+            const Vec<VEC> u = floats(b);
+            own_2 = max_abs(own_2, u);
+            v = product(v, u);
+        }
+        own = max_abs(own, v);
+        if constexpr (MODE == KEPT) store<VEC>(reinterpret_cast<float *>(kept) + at, v);
+        if constexpr (MODE == BULK && VEC == 8) {
+            store<4>(reinterpret_cast<float *>(kept) + 4 * i, Vec<4>{v.p[0], v.p[1]});
+            store<4>(reinterpret_cast<float *>(kept + half) + 4 * i, Vec<4>{v.p[2], v.p[3]});
+        } else if constexpr (MODE == BULK) {
+            store<VEC>(reinterpret_cast<float *>(kept) + at, v);
+        }
+    };
+    if constexpr (MODE == BULK) {
+        using In = decltype(fetch<VEC>(x));
+        static_assert(sizeof(In) == 16, "a group of a stage is one load");
+#pragma unroll 2
+        for (uint32_t i = tid; i < groups; i += NT)
+            take(i, reinterpret_cast<const In *>(kept)[i], reinterpret_cast<const In *>(kept + (TWO ? half : 0))[i]);
+    } else {
+        constexpr uint32_t AHEAD = sizeof(T) * VEC == 16 ? 2 : 4; // loads of either input that are under way together
+        for (uint32_t i = tid; i < groups; i += AHEAD * NT) {
+            decltype(fetch<VEC>(x)) a[AHEAD], b[AHEAD];
 #pragma unroll
-        for (uint32_t j = 0; j < AHEAD; j++) {
-            if (i + j * NT >= groups) break;
-            const uint32_t at = VEC * (i + j * NT);
-            Vec<VEC> v;
-            if constexpr (OP == ADD_NORM) v = sum_to(h + at, a[j], b[j]);
-            else v = floats(a[j]);
-            if constexpr (IS_NORM) {
-                float2 squares = __fmul2_rn(v.p[0], v.p[0]);
+            for (uint32_t j = 0; j < AHEAD; j++)
+                if (i + j * NT < groups) {
+                    a[j] = fetch<VEC>(x + VEC * (i + j * NT));
+                    if constexpr (TWO) b[j] = fetch<VEC>(r + VEC * (i + j * NT));
+                }
 #pragma unroll
-                for (int k = 1; k < VEC / 2; k++) squares = __ffma2_rn(v.p[k], v.p[k], squares);
-                const float sum = squares.x + squares.y;
-                ss += (double)sum;
-                own_2 = max_abs(own_2, sum, sum);
-                v = product(v, load<VEC>(w + at));
-            }
-            if constexpr (OP == GLU) {
-                const Vec<VEC> u = floats(b[j]);
-                own_2 = max_abs(own_2, u);
-                v = product(v, u);
-            }
-            own = max_abs(own, v);
-            if constexpr (STAGED) store<VEC>(kept + at, v);
+            for (uint32_t j = 0; j < AHEAD; j++)
+                if (i + j * NT < groups) take(i + j * NT, a[j], b[j]);
         }
     }
     if constexpr (IS_NORM)
@@ -228,7 +283,17 @@ k_rows_i8(const T *x, const T *r, const float *w, uint32_t n, float eps, uint32_
             part_max[warp] = most;
             part_2[warp] = most_2;
         }
-        __syncthreads();
+        late = __syncthreads_or(late);
+        if (late) break; // a copy did not come: the status says so
+        if (MODE == BULK && tid == 0) {
+            all_largest[parity ^ 1] = 0;
+            // Everyone is past the row before: the next row that takes its stage may come (its values were read and written here).
+            const uint32_t before = (s + stages - 1) % stages;
+            if (row != first && row + (size_t)(stages - 1) * gridDim.x < rows) {
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                ask(row + (stages - 1) * gridDim.x, before);
+            }
+        }
         most = __reduce_max_sync(0xffffffffu, part_max[lane % W]);
         if constexpr (OP != PLAIN) most_2 = __reduce_max_sync(0xffffffffu, part_2[lane % W]);
     }
@@ -242,14 +307,13 @@ k_rows_i8(const T *x, const T *r, const float *w, uint32_t n, float eps, uint32_
         if (__float_as_uint(own) >= most - BELOW<OP>)
             for (uint32_t i = tid; i < groups; i += NT) {
                 const Vec<VEC> v = again(i);
-                if (__float_as_uint(max_abs(0.f, v)) >= most - BELOW<OP>)
-#pragma unroll 1
-                    for (uint32_t k = 0; k < VEC; k++) {
-                        const double e = fabs(exact(VEC * i + k)); // (those below the largest do no harm)
-                        a64 = fmax(a64, e);
-                    }
+                const float floor = __uint_as_float(most - BELOW<OP>);
+                uint32_t which = 0;
+#pragma unroll
+                for (int k = 0; k < VEC / 2; k++) which |= (fabsf(v.p[k].x) >= floor ? 1u : 0u) << (2 * k) | (fabsf(v.p[k].y) >= floor ? 2u : 0u) << (2 * k);
+                for (; which; which &= which - 1) a64 = fmax(a64, fabs(exact(VEC * i + __ffs(which) - 1)));
             }
-        if (!ONE_WARP && a64 > 0.0) atomicMax(&largest, (unsigned long long)__double_as_longlong(a64));
+        if (!ONE_WARP && a64 > 0.0) atomicMax(&all_largest[parity], (unsigned long long)__double_as_longlong(a64));
     } else {
         ss = 0.0;
         for (uint32_t i = tid; i < groups; i += NT)
@@ -263,7 +327,7 @@ k_rows_i8(const T *x, const T *r, const float *w, uint32_t n, float eps, uint32_
                     ss = fma(a, a, ss);
                 }
             }
-        if (!ONE_WARP && a64 > 0.0) atomicMax(&largest, (unsigned long long)__double_as_longlong(a64));
+        if (!ONE_WARP && a64 > 0.0) atomicMax(&all_largest[parity], (unsigned long long)__double_as_longlong(a64));
         if constexpr (IS_NORM) {
 #pragma unroll
             for (int off = 16; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
@@ -299,7 +363,7 @@ k_rows_i8(const T *x, const T *r, const float *w, uint32_t n, float eps, uint32_
         for (int off = 16; off > 0; off >>= 1) a64 = fmax(a64, __shfl_xor_sync(0xffffffffu, a64, off));
     } else {
         bad = __syncthreads_or(bad);
-        a64 = __longlong_as_double((long long)largest);
+        a64 = __longlong_as_double((long long)all_largest[parity]);
     }
     if (tid == NT - 1) { // not the first warp, which may have one group more of the row than the last
         double c = 1.0;
@@ -308,9 +372,15 @@ k_rows_i8(const T *x, const T *r, const float *w, uint32_t n, float eps, uint32_
                 ss = 0.0;
                 for (int i = 0; i < W; i++) ss += part_ss[i];
             }
-            c = 1.0 / sqrt(ss / (double)n + (double)eps);
+            const double mean = fma(ss, inv_n, (double)eps);
+            if (fast) { // (in the range of fp32) a step of Newton's method squares the error of 2^-22
+                const double y = (double)rsqrtf((float)mean);
+                c = y * fma(-0.5 * mean * y, y, 1.5);
+            } else {
+                c = 1.0 / sqrt(mean);
+            }
         }
-        scales[row] = bad ? __int_as_float(0x7fc00000) : (float)(a64 * c / 127.0);
+        scales[row] = bad ? __int_as_float(0x7fc00000) : (float)(a64 * c * (1.0 / 127.0));
     }
 
     auto rounded = [&](uint32_t i) { return (int8_t)__double2int_rn(exact(i) * 127.0 / a64); };
@@ -339,25 +409,48 @@ k_rows_i8(const T *x, const T *r, const float *w, uint32_t n, float eps, uint32_
 #pragma unroll 1
             for (uint32_t k = 0; k < VEC; k++) q[VEC * i + k] = !bad && a64 > 0.0 ? rounded(VEC * i + k) : 0;
     }
+    if (MODE == BULK && ++s == stages) s = 0, phase ^= 1;
+  }
+    if (MODE == BULK && tid == 0 && *(volatile uint32_t *)&arrivals.abort_flag) // copies under way are given time to land
+        for (const uint64_t t0 = now_ns(); now_ns() - t0 < 200000;) {}
 }
 
 constexpr size_t STAGE_MOST = 200 << 10;
+
+// What a kernel may use of an SM's shared memory beyond what it may unasked (48 KB with its own arrays): asked for once per device.
+template <typename K> cudaError_t allow(fq_device *dev, K kernel, size_t bytes, std::atomic<uint64_t> &asked) {
+    if (bytes <= (40 << 10)) return cudaSuccess;
+    const uint64_t bit = 1ull << (dev->ordinal & 63);
+    if ((asked.load(std::memory_order_relaxed) & bit) && dev->ordinal <= 63) return cudaSuccess;
+    if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)STAGE_MOST)) return e;
+    asked.fetch_or(bit, std::memory_order_relaxed);
+    return cudaSuccess;
+}
 
 template <int OP, typename T, int VEC, int NT>
 cudaError_t launch_nt(fq_device *dev, const T *x, const T *r, const float *w, uint32_t n, float eps, uint32_t rows, T *h, int8_t *q, float *scales) {
     const size_t bytes = (size_t)n * 4 * (NT == 32 ? 8 : 1);
     const dim3 grid(NT == 32 ? (rows + 7) / 8 : rows), block(NT == 32 ? 256 : NT);
-    if (bytes > STAGE_MOST) return launch_pdl(k_rows_i8<OP, T, VEC, NT, false>, grid, block, 0, dev->stream, x, r, w, n, eps, rows, h, q, scales);
-    auto kernel = k_rows_i8<OP, T, VEC, NT, true>;
-    if (bytes > (40 << 10)) { // beyond what a kernel may use unasked (48 KB with its own arrays): asked for once per device
-        static std::atomic<uint64_t> asked{0};
-        const uint64_t bit = 1ull << (dev->ordinal & 63);
-        if (!(asked.load(std::memory_order_relaxed) & bit) || dev->ordinal > 63) {
-            if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)STAGE_MOST)) return e;
-            asked.fetch_or(bit, std::memory_order_relaxed);
+    const double inv_n = 1.0 / n;
+    if constexpr (NT != 32 && VEC * sizeof(T) == 16) {
+        // Two stages where two blocks of them fit an SM; one, and a block for every row, where three of those do.
+        const size_t stage = 2 * (size_t)n * sizeof(T);
+        const uint32_t stages = 2 * stage <= (100 << 10) ? 2 : 1;
+        if (stages * stage <= (74 << 10) || stages == 2) {
+            static std::atomic<uint64_t> asked{0};
+            auto kernel = k_rows_i8<OP, T, VEC, NT, BULK>;
+            if (const cudaError_t e = allow(dev, kernel, stages * stage, asked)) return e;
+            const uint32_t per_sm = (uint32_t)std::min<size_t>(1280 / NT, (224 << 10) / (stages * stage + 2048));
+            const dim3 walkers(stages == 1 ? rows : std::min(rows, per_sm * (uint32_t)dev->sm_count));
+            return launch_pdl(kernel, walkers, block, stages * stage, dev->stream, x, r, w, n, eps, rows, h, q, scales, inv_n, stages, dev->status_dev);
         }
     }
-    return launch_pdl(kernel, grid, block, bytes, dev->stream, x, r, w, n, eps, rows, h, q, scales);
+    if (bytes > STAGE_MOST)
+        return launch_pdl(k_rows_i8<OP, T, VEC, NT, DIRECT>, grid, block, 0, dev->stream, x, r, w, n, eps, rows, h, q, scales, inv_n, 1u, dev->status_dev);
+    static std::atomic<uint64_t> asked{0};
+    auto kernel = k_rows_i8<OP, T, VEC, NT, KEPT>;
+    if (const cudaError_t e = allow(dev, kernel, bytes, asked)) return e;
+    return launch_pdl(kernel, grid, block, bytes, dev->stream, x, r, w, n, eps, rows, h, q, scales, inv_n, 1u, dev->status_dev);
 }
 
 template <int OP, typename T, int VEC>

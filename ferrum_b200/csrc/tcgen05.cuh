@@ -59,6 +59,13 @@ __device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *map, i
                  : "memory");
 }
 
+// A run of bytes (a multiple of 16, from and to 16-byte boundaries) without a tensor map.
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
+
 // One lane of a converged warp.  The branches that issue TMA and MMA instructions are taken by it, not by `lane == 0`: the
 // compiler then knows that a single thread runs them and feeds their uniform operands without a loop over lanes (the
 // seven projections of a 27B-class layer, 2048 rows: 1437 -> 1290 us; in a bare loop of MMAs the branch costs 53 cycles
