@@ -27,7 +27,7 @@ using namespace fqk;
 using namespace fqtc;
 
 struct Arrivals { // of a block's bulk copies
-    uint64_t full[2];
+    uint64_t full;
     uint32_t abort_flag;
 };
 
@@ -149,52 +149,47 @@ template <int OP> constexpr float MOST_2 = OP == GLU ? 1048576.f : 1e37f;
 enum Mode {
     DIRECT, // nowhere: v is computed again from memory (rows longer than shared memory)
     KEPT,   // v in shared memory, read from memory by the threads
-    BULK    // bulk copies bring the inputs to shared memory, where v takes their place
+    BULK    // bulk copies bring the inputs to shared memory, where v takes their place (bf16: a group's 16 bytes of each)
 };
 
-// NT threads per row: a block, or one of its eight warps.  With BULK blocks walk the rows, `stages` of them on their way or in
-// work at a time; a stage is the row of x and, of the same size, the row of r or room for the other half of v.
+// NT threads per row: a block, or one of its eight warps.
 template <int OP, typename T, int VEC, int NT, int MODE>
-__global__ void __launch_bounds__(NT == 32 ? 256 : NT, NT == 32 ? 5 : 1280 / NT)
-k_rows_i8(const T *x0, const T *r0, const float *w, uint32_t n, float eps, uint32_t rows, T *h0, int8_t *q0, float *scales, double inv_n, uint32_t stages, int *status) {
+__global__ void __launch_bounds__(NT == 32 ? 256 : NT, NT == 512 ? 3 : NT == 32 ? 5 : 1280 / NT)
+k_rows_i8(const T *x, const T *r, const float *w, uint32_t n, float eps, uint32_t rows, T *h, int8_t *q, float *scales, double inv_n, int *status) {
     constexpr bool IS_NORM = OP == NORM || OP == ADD_NORM, TWO = OP == ADD_NORM || OP == GLU, ONE_WARP = NT == 32;
     constexpr int W = NT / 32;
     extern __shared__ float4 stage[];
-    __shared__ double all_ss[2][W]; // rows alternate between two of each
+    __shared__ double part_ss[W];
     __shared__ uint32_t part_max[W], part_2[W];
-    __shared__ unsigned long long all_largest[2];
+    __shared__ unsigned long long largest;
     __shared__ Arrivals arrivals;
     pdl_trigger();
     const uint32_t lane = threadIdx.x & 31, warp = ONE_WARP ? 0 : threadIdx.x >> 5, tid = ONE_WARP ? lane : threadIdx.x;
-    const uint32_t first = ONE_WARP ? blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x, groups = n / VEC, half = n * (uint32_t)sizeof(T);
-    if (!ONE_WARP && tid == 0) all_largest[0] = all_largest[1] = 0;
+    const uint32_t row = ONE_WARP ? blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x, groups = n / VEC, half = n * (uint32_t)sizeof(T);
+    // Of group i, BULK: the 16 bytes at i and at `half` + i; KEPT: VEC floats.
+    uint8_t *const kept = reinterpret_cast<uint8_t *>(stage) + (ONE_WARP ? (threadIdx.x >> 5) * n * 4 : 0);
+    if (!ONE_WARP && tid == 0) largest = 0;
     if (MODE == BULK && tid == 0) {
-        for (uint32_t s = 0; s < stages; s++) mbar_init(&arrivals.full[s], 1);
+        mbar_init(&arrivals.full, 1);
         arrivals.abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     pdl_wait();
-    if (first >= rows) return; // whole warps
-    uint8_t *const base = reinterpret_cast<uint8_t *>(stage) + (ONE_WARP ? (threadIdx.x >> 5) * n * 4 : 0);
-    auto ask = [&](uint32_t row, uint32_t s) { // one thread
-        mbar_expect_tx(&arrivals.full[s], TWO ? 2 * half : half);
-        bulk_load(base + s * 2 * half, x0 + (size_t)row * n, half, &arrivals.full[s]);
-        if constexpr (TWO) bulk_load(base + s * 2 * half + half, r0 + (size_t)row * n, half, &arrivals.full[s]);
-    };
-    if constexpr (MODE == BULK) {
-        __syncthreads();
-        if (tid == 0)
-            for (uint32_t s = 0; s < stages && first + s * gridDim.x < rows; s++) ask(first + s * gridDim.x, s);
-    }
-    uint32_t s = 0, phase = 0, parity = 0;
-  for (uint32_t row = first; row < rows; row += MODE == BULK ? gridDim.x : rows, parity ^= 1) {
-    const T *const x = x0 + (size_t)row * n, *const r = TWO ? r0 + (size_t)row * n : nullptr;
-    T *const h = OP == ADD_NORM ? h0 + (size_t)row * n : nullptr;
-    int8_t *const q = q0 + (size_t)row * n;
-    double *const part_ss = all_ss[parity];
-    uint8_t *const kept = base + s * 2 * half; // of group i the VEC * sizeof(T) bytes at i and the same at `half` + i: v, its halves
+    if (row >= rows) return; // whole warps
+    x += (size_t)row * n;
+    if constexpr (TWO) r += (size_t)row * n;
+    if constexpr (OP == ADD_NORM) h += (size_t)row * n;
+    q += (size_t)row * n;
     bool late = false;
-    if constexpr (MODE == BULK) late = !mbar_wait(&arrivals.full[s], phase, &arrivals, status);
+    if constexpr (MODE == BULK) {
+        if (tid == 0) {
+            mbar_expect_tx(&arrivals.full, TWO ? 2 * half : half);
+            bulk_load(kept, x, half, &arrivals.full);
+            if constexpr (TWO) bulk_load(kept + half, r, half, &arrivals.full);
+        }
+        __syncthreads();
+        late = !mbar_wait(&arrivals.full, 0, &arrivals, status);
+    }
 
     auto product = [](const Vec<VEC> &a, const Vec<VEC> &b) {
         Vec<VEC> v;
@@ -208,8 +203,7 @@ k_rows_i8(const T *x0, const T *r0, const float *w, uint32_t n, float eps, uint3
         else if constexpr (MODE == BULK && VEC == 8) {
             const Vec<4> lo = load<4>(reinterpret_cast<const float *>(kept) + 4 * i), hi = load<4>(reinterpret_cast<const float *>(kept + half) + 4 * i);
             return Vec<VEC>{lo.p[0], lo.p[1], hi.p[0], hi.p[1]};
-        } else if constexpr (MODE == BULK) return load<VEC>(reinterpret_cast<const float *>(kept) + VEC * i);
-        else if constexpr (OP == PLAIN) return Vec<VEC>(floats(fetch<VEC>(x + VEC * i)));
+        } else if constexpr (OP == PLAIN) return Vec<VEC>(floats(fetch<VEC>(x + VEC * i)));
         else if constexpr (OP == GLU) return product(floats(fetch<VEC>(x + VEC * i)), floats(fetch<VEC>(r + VEC * i)));
         else return product(floats(fetch<VEC>((OP == ADD_NORM ? (const T *)h : x) + VEC * i)), load<VEC>(w + VEC * i));
     };
@@ -247,13 +241,11 @@ k_rows_i8(const T *x0, const T *r0, const float *w, uint32_t n, float eps, uint3
         if constexpr (MODE == BULK && VEC == 8) {
             store<4>(reinterpret_cast<float *>(kept) + 4 * i, Vec<4>{v.p[0], v.p[1]});
             store<4>(reinterpret_cast<float *>(kept + half) + 4 * i, Vec<4>{v.p[2], v.p[3]});
-        } else if constexpr (MODE == BULK) {
-            store<VEC>(reinterpret_cast<float *>(kept) + at, v);
         }
     };
     if constexpr (MODE == BULK) {
         using In = decltype(fetch<VEC>(x));
-        static_assert(sizeof(In) == 16, "a group of a stage is one load");
+        static_assert(sizeof(In) == 16 && VEC == 8, "a group is 16 bytes of each input, and 32 of v");
 #pragma unroll 2
         for (uint32_t i = tid; i < groups; i += NT)
             take(i, reinterpret_cast<const In *>(kept)[i], reinterpret_cast<const In *>(kept + (TWO ? half : 0))[i]);
@@ -283,16 +275,13 @@ k_rows_i8(const T *x0, const T *r0, const float *w, uint32_t n, float eps, uint3
             part_max[warp] = most;
             part_2[warp] = most_2;
         }
-        late = __syncthreads_or(late);
-        if (late) break; // a copy did not come: the status says so
-        if (MODE == BULK && tid == 0) {
-            all_largest[parity ^ 1] = 0;
-            // Everyone is past the row before: the next row that takes its stage may come (its values were read and written here).
-            const uint32_t before = (s + stages - 1) % stages;
-            if (row != first && row + (size_t)(stages - 1) * gridDim.x < rows) {
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                ask(row + (stages - 1) * gridDim.x, before);
+        if constexpr (MODE == BULK) {
+            if (__syncthreads_or(late)) { // a copy did not come, and the status says so: time for it to land before the memory is another's
+                for (const uint64_t t0 = now_ns(); now_ns() - t0 < 200000;) {}
+                return;
             }
+        } else {
+            __syncthreads();
         }
         most = __reduce_max_sync(0xffffffffu, part_max[lane % W]);
         if constexpr (OP != PLAIN) most_2 = __reduce_max_sync(0xffffffffu, part_2[lane % W]);
@@ -313,7 +302,7 @@ k_rows_i8(const T *x0, const T *r0, const float *w, uint32_t n, float eps, uint3
                 for (int k = 0; k < VEC / 2; k++) which |= (fabsf(v.p[k].x) >= floor ? 1u : 0u) << (2 * k) | (fabsf(v.p[k].y) >= floor ? 2u : 0u) << (2 * k);
                 for (; which; which &= which - 1) a64 = fmax(a64, fabs(exact(VEC * i + __ffs(which) - 1)));
             }
-        if (!ONE_WARP && a64 > 0.0) atomicMax(&all_largest[parity], (unsigned long long)__double_as_longlong(a64));
+        if (!ONE_WARP && a64 > 0.0) atomicMax(&largest, (unsigned long long)__double_as_longlong(a64));
     } else {
         ss = 0.0;
         for (uint32_t i = tid; i < groups; i += NT)
@@ -327,7 +316,7 @@ k_rows_i8(const T *x0, const T *r0, const float *w, uint32_t n, float eps, uint3
                     ss = fma(a, a, ss);
                 }
             }
-        if (!ONE_WARP && a64 > 0.0) atomicMax(&all_largest[parity], (unsigned long long)__double_as_longlong(a64));
+        if (!ONE_WARP && a64 > 0.0) atomicMax(&largest, (unsigned long long)__double_as_longlong(a64));
         if constexpr (IS_NORM) {
 #pragma unroll
             for (int off = 16; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
@@ -340,6 +329,15 @@ k_rows_i8(const T *x0, const T *r0, const float *w, uint32_t n, float eps, uint3
     auto rest_of = [&](const float2 &v, const float2 &whole) { return __ffma2_rn(v, f, __fadd2_rn(minus(whole), magic)); };
     auto low_bytes = [](const float2 &a, const float2 &b) {
         return __byte_perm(__byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040), __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040), 0x5410);
+    };
+    // A value of a row as it is, v, against the border b that its quotient is next to: 127 v - b a from products and what their
+    // roundings took (where it decides the products differ by little, and exactly).
+    auto settle = [&](float v, int8_t *to, float whole) {
+        const float a = __uint_as_float(most), near = whole - magic.x, rest = fmaf(v, f.x, -near);
+        const float b = near + copysignf(0.5f, rest), p = 127.f * v, m = b * a;
+        const float over = copysignf(1.f, rest) * ((p - m) + (fmaf(127.f, v, -p) - fmaf(b, a, -m)));
+        const bool odd = __float_as_uint(whole) & 1;
+        if (fabsf(rest) > 0.25f && (over > 0.f || (over == 0.f && odd))) *to = (int8_t)(near + copysignf(1.f, rest));
     };
     if (fast) { // while the largest value is taken in 64 bits elsewhere
         uint32_t at = 0;
@@ -354,7 +352,17 @@ k_rows_i8(const T *x0, const T *r0, const float *w, uint32_t n, float eps, uint3
             }
             if constexpr (VEC == 8) *reinterpret_cast<uint2 *>(q + VEC * i) = make_uint2(low_bytes(whole.p[0], whole.p[1]), low_bytes(whole.p[2], whole.p[3]));
             else *reinterpret_cast<uint32_t *>(q + VEC * i) = low_bytes(whole.p[0], whole.p[1]);
-            if (max_abs(0.f, rest) > 0.5f - 128 * OFF<OP>) near |= 1u << (at & 31);
+            if (max_abs(0.f, rest) > 0.5f - 128 * OFF<OP>) {
+                if constexpr (OP == PLAIN) { // v and a are what they are, and bf16 rows hold many halves of a: 63.5
+#pragma unroll
+                    for (int k = 0; k < VEC / 2; k++) {
+                        settle(v.p[k].x, q + VEC * i + 2 * k, whole.p[k].x);
+                        settle(v.p[k].y, q + VEC * i + 2 * k + 1, whole.p[k].y);
+                    }
+                } else {
+                    near |= 1u << (at & 31);
+                }
+            }
         }
     }
     if constexpr (ONE_WARP) {
@@ -363,7 +371,7 @@ k_rows_i8(const T *x0, const T *r0, const float *w, uint32_t n, float eps, uint3
         for (int off = 16; off > 0; off >>= 1) a64 = fmax(a64, __shfl_xor_sync(0xffffffffu, a64, off));
     } else {
         bad = __syncthreads_or(bad);
-        a64 = __longlong_as_double((long long)all_largest[parity]);
+        a64 = __longlong_as_double((long long)largest);
     }
     if (tid == NT - 1) { // not the first warp, which may have one group more of the row than the last
         double c = 1.0;
@@ -383,7 +391,12 @@ k_rows_i8(const T *x0, const T *r0, const float *w, uint32_t n, float eps, uint3
         scales[row] = bad ? __int_as_float(0x7fc00000) : (float)(a64 * c * (1.0 / 127.0));
     }
 
-    auto rounded = [&](uint32_t i) { return (int8_t)__double2int_rn(exact(i) * 127.0 / a64); };
+    // 127 v / a rounded, from the whole number next to it or nearly so: 127 v is compared with its borders times a.
+    auto rounded = [&](double v, int near) {
+        const double t = 127.0 * v, up = ((double)near + 0.5) * a64, down = ((double)near - 0.5) * a64;
+        if (t > up || (t == up && (near & 1))) return (int8_t)(near + 1);
+        return (int8_t)(t < down || (t == down && (near & 1)) ? near - 1 : near);
+    };
     if (fast) {
         // Values that may be on the wrong side of a border, by their own size (bit b of `near`: groups b, b + 32, ...).
         while (near) {
@@ -391,28 +404,23 @@ k_rows_i8(const T *x0, const T *r0, const float *w, uint32_t n, float eps, uint3
             near &= near - 1;
             for (uint32_t i = tid + b * NT; i < groups; i += 32 * NT) {
                 const Vec<VEC> v = again(i);
-                uint32_t which = 0;
+                auto look = [&](uint32_t k, float e) {
+                    const float whole = fmaf(e, f.x, magic.x), rest = fmaf(e, f.x, magic.x - whole);
+                    if (fabsf(rest) > 0.5f - (fabsf(e * f.x) + 0.5f) * OFF<OP>)
+                        q[VEC * i + k] = rounded(exact(VEC * i + k), (int8_t)__float_as_uint(whole));
+                };
 #pragma unroll
                 for (int k = 0; k < VEC / 2; k++) {
-                    const float2 rest = rest_of(v.p[k], whole_of(v.p[k]));
-                    if (fabsf(rest.x) > 0.5f - (fabsf(v.p[k].x * f.x) + 0.5f) * OFF<OP>) which |= 1u << (2 * k);
-                    if (fabsf(rest.y) > 0.5f - (fabsf(v.p[k].y * f.x) + 0.5f) * OFF<OP>) which |= 2u << (2 * k);
-                }
-                for (; which; which &= which - 1) {
-                    const uint32_t at = VEC * i + __ffs(which) - 1;
-                    q[at] = rounded(at);
+                    look(2 * k, v.p[k].x);
+                    look(2 * k + 1, v.p[k].y);
                 }
             }
         }
     } else {
         for (uint32_t i = tid; i < groups; i += NT)
 #pragma unroll 1
-            for (uint32_t k = 0; k < VEC; k++) q[VEC * i + k] = !bad && a64 > 0.0 ? rounded(VEC * i + k) : 0;
+            for (uint32_t k = 0; k < VEC; k++) q[VEC * i + k] = !bad && a64 > 0.0 ? (int8_t)__double2int_rn(exact(VEC * i + k) * 127.0 / a64) : 0;
     }
-    if (MODE == BULK && ++s == stages) s = 0, phase ^= 1;
-  }
-    if (MODE == BULK && tid == 0 && *(volatile uint32_t *)&arrivals.abort_flag) // copies under way are given time to land
-        for (const uint64_t t0 = now_ns(); now_ns() - t0 < 200000;) {}
 }
 
 constexpr size_t STAGE_MOST = 200 << 10;
@@ -432,25 +440,19 @@ cudaError_t launch_nt(fq_device *dev, const T *x, const T *r, const float *w, ui
     const size_t bytes = (size_t)n * 4 * (NT == 32 ? 8 : 1);
     const dim3 grid(NT == 32 ? (rows + 7) / 8 : rows), block(NT == 32 ? 256 : NT);
     const double inv_n = 1.0 / n;
-    if constexpr (NT != 32 && VEC * sizeof(T) == 16) {
-        // Two stages where two blocks of them fit an SM; one, and a block for every row, where three of those do.
-        const size_t stage = 2 * (size_t)n * sizeof(T);
-        const uint32_t stages = 2 * stage <= (100 << 10) ? 2 : 1;
-        if (stages * stage <= (74 << 10) || stages == 2) {
+    if constexpr (NT != 32 && VEC == 8)
+        if (bytes <= (74 << 10)) { // three blocks an SM
             static std::atomic<uint64_t> asked{0};
             auto kernel = k_rows_i8<OP, T, VEC, NT, BULK>;
-            if (const cudaError_t e = allow(dev, kernel, stages * stage, asked)) return e;
-            const uint32_t per_sm = (uint32_t)std::min<size_t>(1280 / NT, (224 << 10) / (stages * stage + 2048));
-            const dim3 walkers(stages == 1 ? rows : std::min(rows, per_sm * (uint32_t)dev->sm_count));
-            return launch_pdl(kernel, walkers, block, stages * stage, dev->stream, x, r, w, n, eps, rows, h, q, scales, inv_n, stages, dev->status_dev);
+            if (const cudaError_t e = allow(dev, kernel, bytes, asked)) return e;
+            return launch_pdl(kernel, grid, block, bytes, dev->stream, x, r, w, n, eps, rows, h, q, scales, inv_n, dev->status_dev);
         }
-    }
     if (bytes > STAGE_MOST)
-        return launch_pdl(k_rows_i8<OP, T, VEC, NT, DIRECT>, grid, block, 0, dev->stream, x, r, w, n, eps, rows, h, q, scales, inv_n, 1u, dev->status_dev);
+        return launch_pdl(k_rows_i8<OP, T, VEC, NT, DIRECT>, grid, block, 0, dev->stream, x, r, w, n, eps, rows, h, q, scales, inv_n, dev->status_dev);
     static std::atomic<uint64_t> asked{0};
     auto kernel = k_rows_i8<OP, T, VEC, NT, KEPT>;
     if (const cudaError_t e = allow(dev, kernel, bytes, asked)) return e;
-    return launch_pdl(kernel, grid, block, bytes, dev->stream, x, r, w, n, eps, rows, h, q, scales, inv_n, 1u, dev->status_dev);
+    return launch_pdl(kernel, grid, block, bytes, dev->stream, x, r, w, n, eps, rows, h, q, scales, inv_n, dev->status_dev);
 }
 
 template <int OP, typename T, int VEC>
@@ -459,8 +461,11 @@ cudaError_t launch_vec(fq_device *dev, const void *x, const void *r, const float
     const bool few = rows <= 2 * (uint32_t)dev->sm_count;
     const uint32_t groups = n / VEC;
     if (n <= 1024) return launch_nt<OP, T, VEC, 32>(dev, tx, tr, w, n, eps, rows, (T *)h, q, scales);
-    if (groups > (few ? 512 : 2600)) return launch_nt<OP, T, VEC, 512>(dev, tx, tr, w, n, eps, rows, (T *)h, q, scales);
-    if (groups > (few ? 256 : 800)) return launch_nt<OP, T, VEC, 256>(dev, tx, tr, w, n, eps, rows, (T *)h, q, scales);
+    // With many rows the threads that a row's sums are joined over cost more than the time a row waits for itself; a few rows wait.
+    // us with 128 / 256 / 512 threads: add_rmsnorm bf16 2048 x 5120 21.1 / 19.5 / -, gated unit 14.8 / 16.4 / -, 1021 x 17408 - /
+    // 24.5 / 22.2; one row of 5120 F32 with 256 / 512 XXX / 3.7.
+    if (groups > (few ? 512 : 1600)) return launch_nt<OP, T, VEC, 512>(dev, tx, tr, w, n, eps, rows, (T *)h, q, scales);
+    if (groups > (few ? 256 : OP == ADD_NORM ? 400 : 800)) return launch_nt<OP, T, VEC, 256>(dev, tx, tr, w, n, eps, rows, (T *)h, q, scales);
     return launch_nt<OP, T, VEC, 128>(dev, tx, tr, w, n, eps, rows, (T *)h, q, scales);
 }
 
