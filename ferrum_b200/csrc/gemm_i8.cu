@@ -143,6 +143,26 @@ __device__ __forceinline__ void store_tile(const Job &J, const Target &T, uint32
     else store_rows(static_cast<float *>(T.y) + at, T.rows, acc, live, row < T.rows, ws, xs);
 }
 
+// The same of partial sums in shared memory, [token][row]: this block's and, `stride` apart, those of the others.
+template <typename YT>
+__device__ __forceinline__ void store_sums(YT *y, uint32_t rows, uint32_t tokens, const int *sums, const int *others, uint32_t blocks, uint32_t stride, const float *xs, float ws) {
+    constexpr uint32_t AHEAD = 8; // tokens whose loads are under way together (one at a time took 150 clocks each)
+    for (uint32_t c0 = 0; c0 < tokens; c0 += AHEAD) {
+        int v[AHEAD];
+#pragma unroll
+        for (uint32_t c = 0; c < AHEAD; c++) v[c] = c0 + c < tokens ? sums[(c0 + c) * BM] : 0;
+        for (uint32_t from = 0; from < blocks; from++)
+#pragma unroll
+            for (uint32_t c = 0; c < AHEAD; c++)
+                if (c0 + c < tokens) v[c] += others[from * stride + (c0 + c) * BM];
+#pragma unroll
+        for (uint32_t c = 0; c < AHEAD; c++) {
+            if (c0 + c < tokens) put(y, (float)v[c] * xs[c0 + c] * ws);
+            y += rows;
+        }
+    }
+}
+
 template <bool SLICED>
 __global__ void __launch_bounds__(THREADS)
 k_gemm_i8(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ Job J, int *status) {
@@ -291,15 +311,11 @@ k_gemm_i8(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ Job 
                     const uint32_t from = slice < to ? slice : slice - 1;
                     bulk_send(cluster_address(smem_u32(ring), to) + (J.bn + from * share) * BM * 4, ring + first * BM * 4, n * BM * 4, cluster_address(smem_u32(&ctl.received), to));
                 }
-            if (mine_end > mine && mbar_wait(&ctl.received, 0, &ctl, status) && row < T.rows)
-                for (uint32_t c = mine; c < mine_end; c++) {
-                    int sum = sums[c * BM];
-                    for (uint32_t from = 0; from + 1 < J.slices; from++) sum += others[(from * share + c - mine) * BM];
-                    const float f = (float)sum * xs[quarter][c] * ws;
-                    const size_t at = (size_t)(p.m0 + c) * T.rows + row;
-                    if (J.bf16) put(static_cast<__nv_bfloat16 *>(T.y) + at, f);
-                    else put(static_cast<float *>(T.y) + at, f);
-                }
+            if (mine_end > mine && mbar_wait(&ctl.received, 0, &ctl, status) && row < T.rows) {
+                const size_t at = (size_t)(p.m0 + mine) * T.rows + row;
+                if (J.bf16) store_sums(static_cast<__nv_bfloat16 *>(T.y) + at, T.rows, mine_end - mine, sums + mine * BM, others, J.slices - 1, share * BM, xs[quarter] + mine, ws);
+                else store_sums(static_cast<float *>(T.y) + at, T.rows, mine_end - mine, sums + mine * BM, others, J.slices - 1, share * BM, xs[quarter] + mine, ws);
+            }
         }
         __syncwarp();
         cluster_sync(); // what a block sent has been received
@@ -465,12 +481,20 @@ __global__ void __launch_bounds__(256) k_tile_i8(const uint8_t *__restrict__ src
     *reinterpret_cast<uint4 *>(dst + (tile << 14) + r * 128 + chunk * 16) = v;
 }
 
-// How a product is cut: tokens of a tile, the blocks among which an item's K is shared, blocks per SM, pairs or single blocks.
+// How a product is cut: tokens of a tile, the blocks among which an item's K is shared, pairs or single blocks.
 struct Plan {
-    uint32_t bn, token_tiles, slices, per, stages, per_sm;
+    uint32_t bn, token_tiles, slices, per, stages;
     bool pair;
 };
-uint32_t ring_bytes(const Plan &p) { return p.stages * (TILE_BYTES + (p.pair ? p.bn / 2 : p.bn) * BK); }
+uint32_t stage_bytes(const Plan &p) { return TILE_BYTES + (p.pair ? p.bn / 2 : p.bn) * BK; }
+// By an estimate of clocks, one block per SM (two with half the ring each were slower wherever they differed):
+//   - a k-block takes its four MMAs (40 / 48 / 64 / 128 clocks each at N = 32 / 64 / 128 / 256, and 1.3 times that with the
+//     waits between them), or as long as its bytes need: one
+//     SM streams weights at 57 bytes a clock, L2 feeds all of them 6500 a clock; the first ring of it comes at once;
+//   - HBM delivers 3440 bytes of weights a clock;
+//   - a cluster's exchange takes 1300 clocks and 55 a token; a pair's start 1000.
+// us, estimated best against the other (rows x cols, tokens): 5120 x 17408, 1: three slices 16.4, one 21.1; 8192 x 5120, 1: one
+// 9.1, two 9.9, 64: one 10.8, two 13.2; 34816 x 5120, 2048: pairs 224, single blocks 335.
 Plan plan(const fq_device *dev, const fq_matrix *const *w, uint32_t count, uint32_t k_blocks, uint32_t m) {
     const uint32_t sms = (uint32_t)dev->sm_count;
     uint32_t tiles = 0, pairs = 0;
@@ -478,47 +502,36 @@ Plan plan(const fq_device *dev, const fq_matrix *const *w, uint32_t count, uint3
         tiles += (uint32_t)((w[i]->rows + BM - 1) / BM);
         pairs += (uint32_t)((w[i]->rows + 2 * BM - 1) / (2 * BM));
     }
+    const double hbm = (double)tiles * k_blocks * TILE_BYTES / 3440.0;
     Plan p{};
     double best = 0.0;
-    auto round16 = [](uint32_t v, uint32_t to) { return (v + to - 1) / to * to; };
     auto consider = [&](uint32_t token_tiles, bool pair, uint32_t slices) {
+        const uint32_t step = pair ? 32 : 16;
         Plan c{};
         c.pair = pair;
-        c.bn = round16((m + token_tiles - 1) / token_tiles, pair ? 32 : 16);
+        c.bn = ((m + token_tiles - 1) / token_tiles + step - 1) / step * step;
         if (c.bn > 256) return;
         c.token_tiles = (m + c.bn - 1) / c.bn;
-        c.per_sm = m <= 64 ? 2 : 1;
-        const uint32_t items = (pair ? pairs : tiles) * c.token_tiles, slots = pair ? sms / 2 : sms * c.per_sm;
         c.per = (k_blocks + slices - 1) / slices;
         c.slices = (k_blocks + c.per - 1) / c.per; // no slice is left without work
-        c.stages = std::min((SMEM_MAX / c.per_sm - 8192) / (TILE_BYTES + (pair ? c.bn / 2 : c.bn) * BK), MAX_STAGES);
+        c.stages = std::min((SMEM_MAX - 8192) / stage_bytes(c), MAX_STAGES);
+        const uint32_t items = (pair ? pairs : tiles) * c.token_tiles, slots = pair ? sms / 2 : sms;
         if (c.slices > 1) { // all at once, and the sums fit where the ring was
-            if (items > dev->i8_clusters[c.per_sm - 1][c.slices]) return;
-            if ((c.bn + (c.slices - 1) * ((c.bn + c.slices - 1) / c.slices)) * BM * 4 > ring_bytes(c)) return;
+            if (items > dev->i8_clusters[c.slices]) return;
+            if ((c.bn + (c.slices - 1) * ((c.bn + c.slices - 1) / c.slices)) * BM * 4 > c.stages * stage_bytes(c)) return;
         }
-        // Clocks of a k-block on an SM: its MMAs (measured, profiles/tcgen05_mma_rate.md), or what it takes in at 44 bytes a clock,
-        // the rate at which all SMs together are fed from L2.
-        const double mma = 4.0 * std::max(32.0 + c.bn / 4.0, c.bn / 2.0), feed = (TILE_BYTES + (pair ? c.bn / 2 : c.bn) * BK) / 44.0;
-        const double rounds = (items + slots - 1) / slots;
-        const double cost = rounds * (c.per * std::max(mma, feed) + 4.0 * c.bn) + (c.slices > 1 ? 2000.0 + 8.0 * c.bn : 0.0) + (pair ? 1000.0 : 0.0);
+        const double active = std::min(items * c.slices, slots) * (pair ? 2.0 : 1.0), mma = 5.2 * std::max(32.0 + c.bn / 4.0, c.bn / 2.0);
+        const double feed = std::max(TILE_BYTES / 57.0 + (stage_bytes(c) - TILE_BYTES) / 300.0, stage_bytes(c) * active / 6500.0);
+        const double rounds = (items + slots - 1) / slots, ring = std::min(c.per, 8u) * std::max(0.0, feed - mma);
+        const double cost = std::max(hbm, rounds * c.per * std::max(mma, feed) - ring) + 6.0 * c.bn + (c.slices > 1 ? 1300.0 + 55.0 * c.bn : 0.0) + (pair ? 1000.0 : 0.0);
         if (p.bn == 0 || cost < best) {
             best = cost;
             p = c;
         }
     };
-    if (m <= 64) { // as much of the weights under way as the machine holds
-        for (uint32_t slices = 1; slices <= std::min(MAX_SLICES, k_blocks); slices++) {
-            best = 0.0;
-            const Plan before = p;
-            p.bn = 0;
-            consider(1, false, slices);
-            if (p.bn == 0) p = before;
-        }
-    } else {
-        for (uint32_t t = (m + 255) / 256; t <= (m + 255) / 256 + 7 && t <= (m + 15) / 16; t++) {
-            for (uint32_t slices = 1; slices <= std::min(MAX_SLICES, k_blocks); slices++) consider(t, false, slices);
-            consider(t, true, 1);
-        }
+    for (uint32_t t = (m + 255) / 256; t <= (m + 255) / 256 + 7 && t <= (m + 15) / 16; t++) {
+        for (uint32_t slices = 1; slices <= std::min(MAX_SLICES, k_blocks) && (slices == 1 || tiles * t * slices <= sms); slices++) consider(t, false, slices);
+        consider(t, true, 1);
     }
     return p;
 }
@@ -526,25 +539,24 @@ Plan plan(const fq_device *dev, const fq_matrix *const *w, uint32_t count, uint3
 // Once per handle: the kernels may use all of an SM's shared memory, and how many clusters of each size run at once (a cluster's
 // blocks share a GPC, so fewer than blocks would).
 cudaError_t prepare_device(fq_device *dev) {
-    if (dev->i8_clusters[0][1]) return cudaSuccess;
+    if (dev->i8_clusters[1]) return cudaSuccess;
     for (const void *kernel : {(const void *)k_gemm_i8<false>, (const void *)k_gemm_i8<true>, (const void *)k_gemm_i8_pair})
         if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(SMEM_MAX - 6144))) return e;
-    for (uint32_t per_sm = 2; per_sm >= 1; per_sm--)
-        for (uint32_t slices = MAX_SLICES; slices >= 1; slices--) {
-            cudaLaunchConfig_t cfg{};
-            cfg.gridDim = dim3(slices * (uint32_t)dev->sm_count);
-            cfg.blockDim = dim3(THREADS);
-            cfg.dynamicSmemBytes = SMEM_MAX / per_sm - 8192 + 1024;
-            cudaLaunchAttribute attr[1];
-            attr[0].id = cudaLaunchAttributeClusterDimension;
-            attr[0].val.clusterDim.x = slices;
-            attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-            cfg.attrs = attr;
-            cfg.numAttrs = 1;
-            int clusters = 0;
-            if (const cudaError_t e = cudaOccupancyMaxActiveClusters(&clusters, k_gemm_i8<true>, &cfg)) return e;
-            dev->i8_clusters[per_sm - 1][slices] = (uint16_t)clusters; // [0][1], the last, is never 0
-        }
+    for (uint32_t slices = MAX_SLICES; slices >= 1; slices--) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(slices * (uint32_t)dev->sm_count);
+        cfg.blockDim = dim3(THREADS);
+        cfg.dynamicSmemBytes = SMEM_MAX - 8192 + 1024;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = slices;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        int clusters = 0;
+        if (const cudaError_t e = cudaOccupancyMaxActiveClusters(&clusters, k_gemm_i8<true>, &cfg)) return e;
+        dev->i8_clusters[slices] = (uint16_t)clusters; // [1], the last, is never 0
+    }
     return cudaSuccess;
 }
 
@@ -587,9 +599,9 @@ int launch(fq_device *dev, const fq_matrix *const *w, uint32_t count, const int8
     J.box_bytes = box_rows * BK;
     cudaLaunchConfig_t cfg{};
     const uint32_t sms = (uint32_t)dev->sm_count;
-    cfg.gridDim = dim3(p.pair ? 2 * std::min(J.items, sms / 2) : p.slices > 1 ? J.items * p.slices : std::min(J.items, sms * p.per_sm));
+    cfg.gridDim = dim3(p.pair ? 2 * std::min(J.items, sms / 2) : p.slices > 1 ? J.items * p.slices : std::min(J.items, sms));
     cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = 1024 + ring_bytes(p);
+    cfg.dynamicSmemBytes = 1024 + p.stages * stage_bytes(p);
     cfg.stream = dev->stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

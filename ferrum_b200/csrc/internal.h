@@ -74,9 +74,8 @@ struct fq_device {
     // Split-K workspace of the prefill GEMM: partial fp32 tiles and one arrival counter per tile.
     float *gemm_ws = nullptr;
     size_t gemm_ws_bytes = 0;
-    // Clusters of 1..8 blocks of the 8-bit projection kernel that run at once, with one and with two blocks an SM
-    // (filled when the first such matrix is made).
-    uint16_t i8_clusters[2][9] = {};
+    // Clusters of 1..8 blocks of the 8-bit projection kernel that run at once (filled when the first such matrix is made).
+    uint16_t i8_clusters[9] = {};
     // One word in mapped pinned host memory that kernels set when a bounded wait gives up.
     volatile int *status_host = nullptr;
     int *status_dev = nullptr;
