@@ -15,9 +15,9 @@
 // than 20 / b above it (a term is 2^20 at most, far from fp32's end; a running maximum would rescale every few values).  Dividing by b as
 // it is keeps its own rounding out of z.
 //
-// The most likely tokens: while the row is read, every thread notes the largest of each 16 or 32 logits it takes in.  Of the
-// block's threads the k-th largest maximum is a bound that k tokens reach and few more do, so at the end only the few pieces that
-// reach it are read again, and what they hold is put in order by counting (what a piece could hold was looked at as it came
+// The most likely tokens: while the row is read, every thread notes the largest of each 16 to 64 logits it takes in.  Of the
+// block's threads the k-th largest maximum (of the best of every warp) is a bound that k tokens reach and few more do, so at
+// the end only the few pieces that reach it are read again, and what they hold is put in order by counting (what a piece could hold was looked at as it came
 // by, against a bound that rose slowly, in the first version: 20 to 90 us more for 8 to 32 alternatives of 1021 rows).
 // Keys (value, index) are unique, of equal values the lower index is larger, so nothing depends on the order of threads.
 #include <algorithm>
@@ -32,8 +32,7 @@ namespace {
 using namespace fqk;
 
 constexpr uint32_t MAX_TOP = 32, MAX_CLUSTER = 8;
-constexpr int UNROLL = 4;        // 16-byte loads of a thread in flight
-constexpr uint32_t FIRSTS = 64;  // thread maxima that the bound is taken from
+constexpr int UNROLL = 4; // 16-byte loads of a thread in flight
 template <int NT> constexpr uint32_t NOTES = 40 * 256 / NT; // maxima that a thread notes (more tiles than these share one)
 constexpr uint32_t POOL = 512;   // pieces read again, and values kept of them
 constexpr float LOG2E = 1.44269502f; // b: log2(e) rounded to fp32
@@ -166,18 +165,6 @@ __device__ __forceinline__ Sums join_warp(Sums a, int lanes = 32) {
     }
     return a;
 }
-// The best 32 of two sorted lists (descending by lane), sorted.
-__device__ __forceinline__ uint64_t merge_lists(uint64_t a, const uint64_t *b, uint32_t lane) {
-    const uint64_t o = b[31 - lane];
-    uint64_t c = a > o ? a : o;
-#pragma unroll 1
-    for (int off = 16; off > 0; off >>= 1) {
-        const uint64_t other = __shfl_xor_sync(0xffffffffu, c, off);
-        if ((other > c) == ((lane & off) == 0)) c = other;
-    }
-    return c;
-}
-
 // A row of logits around numbers beyond MOST: by one warp, in 64 bits about its largest.
 template <typename T> __device__ __noinline__ void sum_64(const T *l, uint32_t n, uint32_t lane, double &z, double &entropy) {
     double mx = -INFINITY, s = 0.0, t = 0.0;
@@ -208,11 +195,31 @@ __device__ __forceinline__ uint32_t cluster_address(const void *p, uint32_t rank
 __device__ __forceinline__ void store_cluster(uint32_t to, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to), "r"(v) : "memory"); }
 
 template <bool TOP> struct Best { // shared memory of best_of
-    uint4 firsts[FIRSTS / 4];
-    uint64_t keys[POOL + MAX_TOP], out[MAX_TOP];
+    alignas(16) uint64_t keys[POOL + MAX_TOP];
+    alignas(16) uint32_t maxima[64];
+    uint64_t out[MAX_TOP];
     uint32_t work[POOL], wanted, found, bound, before[32];
 };
 template <> struct Best<false> {};
+
+// The first `total` keys of the pool in order, the best MAX_TOP of them in S.out.
+template <int NT> __device__ __forceinline__ void order_pool(Best<true> &S, uint32_t total) {
+    const uint32_t tid = threadIdx.x;
+    if (tid < MAX_TOP) S.out[tid] = 0;
+    if (tid == 0) S.keys[total] = 0; // they are read by twos
+    __syncthreads();
+    for (uint32_t i = tid; i < total; i += NT) {
+        const uint64_t mine = S.keys[i];
+        uint32_t higher = 0;
+#pragma unroll 8
+        for (uint32_t o = 0; o < total; o += 2) {
+            const ulonglong2 two = *reinterpret_cast<const ulonglong2 *>(S.keys + o);
+            higher += (two.x > mine) + (two.y > mine);
+        }
+        if (higher < MAX_TOP) S.out[higher] = mine;
+    }
+    __syncthreads();
+}
 
 // The k best (value, index) keys of the block's pieces [begin, end), sorted, in the lanes of its first warp (0 where there are
 // fewer); all threads call it, after what they noted (`noted` times, the largest `most`).
@@ -221,42 +228,38 @@ __device__ __forceinline__ uint64_t best_of(Best<true> &S, const float *notes, u
                                             uint32_t skip, uint32_t begin, uint32_t end, uint32_t k) {
     constexpr uint32_t W = NT / 32, V = PER_LOAD<T>, TILE = UNROLL * NT;
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    uint32_t *firsts = reinterpret_cast<uint32_t *>(S.firsts);
     // This thread's first piece of a note; the threads that have one come first.
     auto piece_of = [&](uint32_t note, uint32_t thread) { return begin + note * shared_by * TILE + thread; };
     uint32_t best = order_of(most); // a logit of the thread, or 0
-    const uint32_t warps = min(W, (end - begin + 31) / 32); // with something to read
-    const uint32_t m = min(min(32u, FIRSTS / max(warps, 1u)), 2 * k / max(warps, 1u) + 2); // maxima of every warp, m * warps >= k
+    // The largest maxima of every warp whose threads all have logits, 32 or (from 17 alternatives on) 64 of them, k at least.
+    const uint32_t warps = max(1u, min(W, (end - begin) / 32)), m = min(32u, (k > 16 ? 64 : 32) / warps);
     if (warp < warps) {
         uint32_t high = __reduce_max_sync(0xffffffffu, best);
 #pragma unroll 1
         for (uint32_t i = 0; i < m; i++) {
-            if (lane == 0) firsts[warp * m + i] = high;
+            if (lane == 0) S.maxima[warp * m + i] = high;
             const uint32_t holders = __ballot_sync(0xffffffffu, best == high);
             if (lane == (uint32_t)__ffs(holders) - 1) best = 0;
             high = __reduce_max_sync(0xffffffffu, best);
         }
     }
-    for (uint32_t i = m * warps + tid; i < FIRSTS; i += NT) firsts[i] = 0;
-    if (tid == 0) {
-        S.wanted = S.found = 0;
-        S.bound = 0xFFFFFFFFu;
-    }
+    for (uint32_t i = m * warps + tid; i < 64; i += NT) S.maxima[i] = 0;
+    if (tid == 0) S.wanted = S.found = 0;
     __syncthreads();
     // The bound: the least of those that fewer than k are above.  0, below everything, where there are fewer than k.
-    if (tid < FIRSTS) {
-        const uint32_t mine = firsts[tid];
+    if (warp < 2) {
+        const uint32_t mine = S.maxima[tid], last = k > 16 ? 64 : 32;
         uint32_t higher = 0;
 #pragma unroll 4
-        for (uint32_t i = 0; i < FIRSTS / 4; i++) {
-            const uint4 f = S.firsts[i];
+        for (uint32_t i = 0; i < last; i += 4) {
+            const uint4 f = *reinterpret_cast<const uint4 *>(S.maxima + i);
             higher += (f.x > mine) + (f.y > mine) + (f.z > mine) + (f.w > mine);
         }
-        const uint32_t mine_or_more = __reduce_min_sync(0xffffffffu, higher < k ? mine : 0xFFFFFFFFu);
-        if (lane == 0) atomicMin(&S.bound, mine_or_more);
+        const uint32_t reached = __reduce_min_sync(0xffffffffu, higher < k && tid < last ? mine : 0xFFFFFFFFu);
+        if (lane == 0) S.before[warp] = reached;
     }
     __syncthreads();
-    uint32_t least = S.bound;
+    uint32_t least = min(S.before[0], S.before[1]);
     auto load = [&](uint32_t j) { return j * V - skip <= n && n - (j * V - skip) >= V ? __ldcg(aligned + j) : ends(l, n, j * V - skip); };
     auto order_at = [&](const uint4 &p, uint32_t i) {
         const uint32_t w = word(p, sizeof(T) == 2 ? i / 2 : i);
@@ -268,27 +271,31 @@ __device__ __forceinline__ uint64_t best_of(Best<true> &S, const float *notes, u
     uint32_t total;
     for (;;) {
         const float reach = value_of(least);
-        if (!(most < reach)) {
-            const uint32_t last = piece_of(noted - 1, tid) < end ? noted : noted - 1;
-#pragma unroll 4
-            for (uint32_t i = 0; i < last; i++) {
+        if (__any_sync(0xffffffffu, !(most < reach)))
+#pragma unroll 2
+            for (uint32_t i = 0; i < noted; i++) {
                 const float v = notes[i * NT + tid];
-                if (least == 0 ? !above || v == v : above ? v > reach : v >= reach) {
-                    const uint32_t at = atomicAdd(&S.wanted, 1u);
-                    if (at < POOL) S.work[at] = i * NT + tid;
-                }
+                const bool want = piece_of(i, tid) < end && (least == 0 ? !above || v == v : above ? v > reach : v >= reach);
+                const uint32_t which = __ballot_sync(0xffffffffu, want);
+                if (which == 0) continue;
+                uint32_t at = 0;
+                if (lane == 0) at = atomicAdd(&S.wanted, __popc(which));
+                at = __shfl_sync(0xffffffffu, at, 0) + __popc(which & ((1u << lane) - 1));
+                if (want && at < POOL) S.work[at] = i * NT + tid;
             }
-        }
         __syncthreads();
         const uint32_t wanted = S.wanted, per = UNROLL * shared_by;
         for (uint32_t i = tid; i < min(wanted, POOL) * per; i += NT) {
             const uint32_t entry = S.work[i / per], j = piece_of(entry / NT, entry % NT) + i % per * NT;
             if (j >= end) continue;
             const uint4 p = load(j);
-#pragma unroll 1
+#pragma unroll
             for (uint32_t e = 0; e < V; e++) {
-                const uint32_t order = order_at(p, e), at = j * V - skip + e;
-                if (at < n && (above ? order > least : order >= least)) {
+                const uint32_t w = word(p, sizeof(T) == 2 ? e / 2 : e), at = j * V - skip + e;
+                const float v = sizeof(T) == 4 ? __uint_as_float(w) : (e & 1) ? high_half(w) : low_half(w);
+                if (v < reach || at >= n) continue;
+                const uint32_t order = order_of(v);
+                if (above ? order > least : order >= least) {
                     const uint32_t to = atomicAdd(&S.found, 1u);
                     if (to < POOL) S.keys[to] = key_of(order, at);
                 }
@@ -341,22 +348,13 @@ __device__ __forceinline__ uint64_t best_of(Best<true> &S, const float *notes, u
             total = min(total, max(k, 1u));
             __syncthreads();
         }
-    if (tid < MAX_TOP) S.out[tid] = 0;
-    __syncthreads();
-    for (uint32_t i = tid; i < total; i += NT) {
-        const uint64_t mine = S.keys[i];
-        uint32_t higher = 0;
-#pragma unroll 4
-        for (uint32_t o = 0; o < total; o++) higher += S.keys[o] > mine;
-        if (higher < MAX_TOP) S.out[higher] = mine;
-    }
-    __syncthreads();
+    order_pool<NT>(S, total);
     return S.out[lane];
 }
 
 // Block `rank` of the `parts` of row blockIdx.x / parts.
 template <typename T, int NT, bool TOP>
-__global__ void __launch_bounds__(NT, 1024 / NT)
+__global__ void __launch_bounds__(NT, NT == 512 ? 1 : 1024 / NT)
 k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids, uint32_t k, uint32_t parts, Outputs out) {
     constexpr int W = NT / 32, V = PER_LOAD<T>;
     extern __shared__ float notes[]; // [NOTES or fewer][NT]: the largest of a thread's logits in a tile; NaN: it has no number there
@@ -440,7 +438,7 @@ k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids
             }
         }
         if (!(highest <= given)) {
-            if constexpr (sizeof(T) == 2) { // ones added in bf16: 4 * UNROLL at most
+            if constexpr (sizeof(T) == 2) { // ones added in bf16, 32 at most
                 const __nv_bfloat162 g = __float2bfloat162_rn(given);
                 __nv_bfloat162 above = __float2bfloat162_rn(0.f);
 #pragma unroll
@@ -526,20 +524,35 @@ k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids
             count = __reduce_add_sync(0xffffffffu, lane < parts ? all_counts[lane] : 0u);
             flags = __reduce_or_sync(0xffffffffu, lane < parts ? all_bads[lane] : 0u);
         }
-        if constexpr (TOP)
-#pragma unroll 1
-            for (uint32_t half = parts / 2; half > 0; half /= 2) { // (parts is a power of two)
-                if (warp < half) all_lists[warp][lane] = list = merge_lists(all_lists[warp][lane], all_lists[warp + half], lane);
-                __syncthreads();
+        if constexpr (TOP) { // what reaches the largest of the lists' k-th keys, put in order by counting
+            uint64_t kth = lane < parts ? all_lists[lane][k - 1] : 0;
+#pragma unroll
+            for (int off = MAX_CLUSTER / 2; off > 0; off /= 2) kth = max(kth, __shfl_xor_sync(0xffffffffu, kth, off));
+            kth = __shfl_sync(0xffffffffu, kth, 0);
+            if (tid == 0) top.found = 0;
+            __syncthreads();
+            for (uint32_t p = warp; p < parts; p += W) {
+                const uint64_t key = all_lists[p][lane];
+                const uint32_t reach = __ballot_sync(0xffffffffu, key != 0 && key >= kth); // a list's first ones
+                uint32_t at = 0;
+                if (lane == 0) at = atomicAdd(&top.found, __popc(reach));
+                at = __shfl_sync(0xffffffffu, at, 0);
+                if (reach >> lane & 1) top.keys[at + lane] = key;
             }
+            __syncthreads();
+            order_pool<NT>(top, top.found);
+            list = top.out[lane];
+        }
     }
     if (warp != 0) return;
     double z, entropy;
     if ((flags & 1) || !(flags & 4)) z = entropy = NAN;
     else if ((flags & 2) || a.c < -MOST * LOG2E) sum_64(l, n, lane, z, entropy); // (the pivot is the row's largest or near it)
     else {
-        const double log2_s = log2((double)a.s);
-        z = ((double)a.c + log2_s) / (double)LOG2E;
+        // log2 S from its exponent and, within 2^-24, its mantissa.
+        const uint32_t bits = __float_as_uint(a.s);
+        const double log2_s = (double)((int)(bits >> 23) - 127) + (double)log2f(__uint_as_float((bits & 0x7FFFFFu) | 0x3F800000u));
+        z = ((double)a.c + log2_s) * (1.0 / (double)LOG2E);
         entropy = 0.69314718055994531 * (log2_s - (double)a.t / (double)a.s);
     }
     if (lane == 0) {

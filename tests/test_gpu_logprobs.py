@@ -30,24 +30,28 @@ def run(d, l, n, ids, k, stride=None):
 
 
 def check(l, ids, k, got):
-    """`l`: [rows, n] float64 of exactly the logits that were passed."""
+    """`l`: [rows, n] float64 of exactly the logits that were passed; the same in 64 bits by torch, on the device for its speed."""
     lp, rk, en, tp, ti = got
     rows, n = l.shape
-    with np.errstate(all="ignore"):
-        mx = l.max(axis=1)
-        e = np.exp(l - mx[:, None])
-        s = e.sum(axis=1)
-        z = mx + np.log(s)
-        p = e / s[:, None]
-        entropy = -np.where(p > 0, p * (l - z[:, None]), 0).sum(axis=1)
-        z, entropy = np.where(np.isfinite(mx), z, np.nan), np.where(np.isfinite(mx), entropy, np.nan)
-        inside = np.asarray(ids) < n
-        given = np.where(inside, l[np.arange(rows), np.where(inside, ids, 0)], np.nan)
-        want = given - z
-        rank = np.where(inside, 1 + (l > given[:, None]).sum(axis=1), 0)
-    order = np.argsort(np.where(np.isnan(l), np.inf, -l), axis=1, kind="stable")
-    # NaN goes behind -infinity, which the key above cannot say: only rows without NaN are compared by it.
-    clean = ~np.isnan(l).any(axis=1)
+    x = torch.from_numpy(np.ascontiguousarray(l)).cuda()
+    id_ = torch.from_numpy(np.asarray(ids, np.int64)).cuda()
+    mx = x.max(dim=1).values  # NaN where a row holds one
+    e = (x - mx[:, None]).exp()
+    s = e.sum(dim=1)
+    z = mx + s.log()
+    p = e / s[:, None]
+    entropy = -torch.where(p > 0, p * (x - z[:, None]), 0.0).sum(dim=1)
+    z, entropy = z.where(mx.isfinite(), float("nan")), entropy.where(mx.isfinite(), float("nan"))
+    inside = id_ < n
+    given = x.gather(1, id_.where(inside, 0)[:, None])[:, 0].where(inside, float("nan"))
+    want = given - z
+    rank = (1 + (x > given[:, None]).sum(dim=1)).where(inside, 0)
+    want, rank, entropy, z = (t.cpu().numpy() for t in (want, rank, entropy, z))
+    if k:
+        # NaN goes behind -infinity, which the order below cannot say: only rows without NaN are compared by it.
+        clean = ~x.isnan().any(dim=1).cpu().numpy()
+        order = torch.sort(x + 0.0, dim=1, descending=True, stable=True).indices[:, :k].cpu().numpy()
+        top = x.gather(1, torch.from_numpy(ti.astype(np.int64)).cuda()).cpu().numpy()
     # Sums: a term exp(d) carries the roundings of d (|d| * 2^-24 twice), 2^-22 of the exponential, and the additions of a
     # thread's share (n / 256 at the most) and of a tree; far terms weigh nothing, so |d| is taken at 100.  The entropy's
     # second sum has one rounding more in terms of at most |d| times the first's.
@@ -61,8 +65,7 @@ def check(l, ids, k, got):
     assert near(en, entropy, off(entropy) * (1 + span)), (en, entropy)
     assert np.array_equal(rk, rank), (rk, rank)
     if k:
-        assert np.array_equal(ti[clean], order[clean, :k])
-        top = l[np.arange(rows)[:, None], ti]
+        assert np.array_equal(ti[clean], order[clean])
         with np.errstate(all="ignore"):
             want = top - z[:, None]
         assert near(tp, want, off(want))
@@ -181,6 +184,56 @@ def test_padded_and_unaligned_rows(device, n, stride, first, dtype):
     check(l.double().numpy(), ids, 16, run(device, buf, n, ids, 16, stride))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,n", [(1, 700001), (19, 1400003), (700, 50003)])
+def test_rows_of_more_pieces_than_are_noted(device, rows, n, dtype):
+    """A block notes 40 (20, 80) maxima a thread; longer rows share them, and a row of many that no cluster cuts is long early."""
+    rng = np.random.default_rng(n)
+    l = torch.randn(rows, n, generator=torch.Generator(device="cuda").manual_seed(n), device="cuda").mul_(2.5).to(dtype)
+    l[rows // 2, -9:] += 9  # in the last, shorter piece
+    ids = rng.integers(0, n, rows)
+    got = run(device, l.view(-1), n, ids, 32)
+    some = np.unique(np.r_[0, rows // 2, rows - 1, rng.integers(0, rows, 4)])
+    check(l[torch.from_numpy(some).cuda()].double().cpu().numpy(), ids[some], 32, [g[some] for g in got])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [40, 5000, 60000])
+def test_alternatives_where_few_tokens_are_numbers(device, n, dtype):
+    """Rows of NaN but for a few tokens, fewer than are asked for: numbers in their order, then NaN by id."""
+    rng, k = np.random.default_rng(n), 32
+    for numbers in (0, 1, 5, 31, 33):
+        l = np.full((3, n), np.nan)
+        for r in range(3):
+            l[r, rng.choice(n, numbers, replace=False)] = rng.standard_normal(numbers)
+        t = torch.from_numpy(l).to(dtype)
+        got = run(device, t.cuda().view(-1), n, [0, 1, n - 1], k)
+        x = t.double().numpy()
+        assert np.array_equal(got[4], np.argsort(np.where(np.isnan(x), np.inf, -x), axis=1, kind="stable")[:, :k])
+        assert all(np.isnan(got[i]).all() for i in (0, 2, 3))
+        with np.errstate(all="ignore"):
+            assert np.array_equal(got[1], 1 + (x > x[[0, 1, 2], [0, 1, n - 1]][:, None]).sum(1))
+
+
+@pytest.mark.parametrize("rows", [1, 60])
+def test_more_best_tokens_than_are_kept(device, rows):
+    """Hundreds to thousands of logits above every thread's typical one: in few pieces, in all pieces, equal or growing."""
+    n, rng = 50000, np.random.default_rng(7)
+    base = rng.standard_normal(n)
+    cases = []
+    for count in (300, 513, 4000):
+        for kind in range(4):
+            x = base.copy()
+            at = np.arange(1000, 1000 + count) if kind % 2 else rng.choice(n, count, replace=False)
+            x[at] = 10 if kind < 2 else 10 + np.arange(count) / 8.0
+            cases.append(x)
+    for x in cases:
+        l = torch.from_numpy(np.tile(x, (rows, 1))).float()
+        for k in (1, 17, 32):
+            ids = rng.integers(0, n, rows)
+            check(l.double().numpy(), ids, k, run(device, l.cuda().view(-1), n, ids, k))
+
+
 def test_padding_rows_and_unwanted_outputs(device):
     """Ids that name no token, the same id in every row, and each output alone with the same values."""
     s, rng, n = S(), np.random.default_rng(4), 5000
@@ -209,6 +262,30 @@ def test_repeated_calls_give_the_same_bits(device):
         first = run(device, l, n, ids, 32)
         for _ in range(3):
             assert all(np.array_equal(a, b) for a, b in zip(first, run(device, l, n, ids, 32)))
+
+
+def test_captured_and_replayed(device):
+    """Two captured graphs of the same logits on one handle, replayed in turn with new logits, give what direct calls give."""
+    s, n, rows, k = S(), 32000, 5, 20
+    rng = np.random.default_rng(12)
+    l, ids = torch.zeros(rows, n, device="cuda"), torch.from_numpy(rng.integers(0, n, rows).astype(np.int32)).cuda()
+    out = [[torch.zeros(shape, dtype=t, device="cuda") for shape, t in ((rows, F32), (rows, torch.int32), (rows, F32), ((rows, k), F32), ((rows, k), torch.int32))] for _ in range(3)]
+    call = lambda o: s.token_logprobs(device, l, n, rows, ids, o[0], o[1], o[2], k, o[3], o[4])
+    torch.cuda.synchronize()
+    graphs = []
+    for o in out[:2]:
+        device.capture_begin()
+        call(o)
+        graphs.append(device.capture_end())
+    for step in range(3):
+        l.copy_(torch.from_numpy(logits(rng, rows, n)).float())
+        torch.cuda.synchronize()
+        for g in graphs:
+            g.launch()
+        call(out[2])
+        device.synchronize()
+        for o in out[:2]:
+            assert all(torch.equal(a, b) for a, b in zip(o, out[2]))
 
 
 def test_refused_calls(device):
