@@ -597,9 +597,14 @@ cudaError_t launch_shape(fq_device *dev, const T *logits, uint32_t n, size_t str
 template <typename T>
 cudaError_t launch_rows(fq_device *dev, const T *logits, uint32_t n, size_t stride, uint32_t rows, const uint32_t *ids, uint32_t k, const Outputs &out) {
     const uint32_t sms = (uint32_t)dev->sm_count;
-    const bool wide = rows * MAX_CLUSTER <= sms && n > 8192; // a few rows: as many threads as there can be
+    // A row is cut while four blocks an SM hold all parts and a part keeps 4096 logits.  us with two / four / eight blocks an SM:
+    // 64 rows of 151936 F32 without alternatives 14.3 / 10.9 / 10.9, 100 rows 23.5 / 16.2 / 18.0, 200 rows of 32000 bf16 8.0 / 6.5 / 7.7.
     uint32_t parts = 1;
-    while (parts < MAX_CLUSTER && (wide || rows * (2 * parts) <= 4 * sms) && n / (2 * parts) >= 4096) parts *= 2;
+    while (parts < MAX_CLUSTER && rows * (2 * parts) <= 4 * sms && n / (2 * parts) >= 4096) parts *= 2;
+    // Blocks that leave half the SMs empty have 512 threads (with 20 alternatives, us with 256 / 512: one row of 151936 F32 10.1 /
+    // 9.0, 16 of 32000 8.2 / 7.7; but 18 of 151936 bf16, more clusters of eight such blocks than run at once, 12.6 / 17.4); those of
+    // short rows 128, which their joins cost less (128 / 256: 2000 rows of 8192 bf16 19.6 / 26.6, 512 of 4096 9.2 / 9.6).
+    const bool wide = rows * parts <= sms / 2 && n > 8192;
     auto go = [&](auto top) {
         constexpr bool TOP = decltype(top)::value;
         if (wide) return launch_shape<T, 512, TOP>(dev, logits, n, stride, rows, ids, k, parts, out);

@@ -78,7 +78,7 @@ def logits(rng, rows, n):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("rows", [1, 5, 130, 700])
+@pytest.mark.parametrize("rows", [1, 5, 18, 130, 700])
 @pytest.mark.parametrize("n", [1, 2, 3, 7, 31, 33, 128, 1000, 4099, 32000, 50257, 151936])
 def test_rows_of_every_length(device, n, rows, dtype):
     if n > 40000 and rows > 130:
