@@ -17,11 +17,12 @@
 // Blocks walk (row tile, token tile) items.  Where there are fewer items than blocks the machine holds, a cluster of up to
 // eight blocks cuts an item's K and adds the partial sums (whole numbers, so in any order) through distributed shared memory:
 // block r of the cluster collects and stores the tokens of its share, which the others send as one bulk copy each (value by
-// value, remote stores took 45 instead of XXX us for q|k|v of 128 rows).  All waits are bounded (tcgen05.cuh).
+// value, remote stores took 45 us for q|k|v of 128 rows where these took 24).  All waits are bounded (tcgen05.cuh).
 #include <algorithm>
 #include <cmath>
 #include <cstring>
-#include <vector>
+#include <memory>
+#include <new>
 
 #include "gemv_common.cuh"
 #include "internal.h"
@@ -641,13 +642,15 @@ extern "C" int fq_matrix_create_i8(fq_device *dev, uint64_t rows, uint64_t cols,
         if (attr.type == cudaMemoryTypeDevice && attr.device != dev->ordinal) return fq_fail(dev, FQ_ERR_DEVICE, "the payload is on device %d", attr.device);
         on_device = attr.type == cudaMemoryTypeDevice;
     }
-    std::vector<float> host(rows);
-    cudaError_t e = cudaMemcpyAsync(host.data(), scales, rows * 4, cudaMemcpyDefault, dev->stream);
+    const std::unique_ptr<float[]> host(new (std::nothrow) float[rows]);
+    if (!host) return fq_fail(dev, FQ_ERR_CUDA, "no host memory for %llu scales", (unsigned long long)rows);
+    cudaError_t e = cudaMemcpyAsync(host.get(), scales, rows * 4, cudaMemcpyDefault, dev->stream);
     if (e == cudaSuccess) e = cudaStreamSynchronize(dev->stream);
     if (e != cudaSuccess) return fq_check_cuda(dev, e, "weight scales");
     for (uint64_t r = 0; r < rows; r++)
         if (!std::isfinite(host[r])) return fq_fail(dev, FQ_ERR_WEIGHT, "the scale of row %llu is not finite", (unsigned long long)r);
-    fq_matrix *w = new fq_matrix();
+    fq_matrix *w = new (std::nothrow) fq_matrix();
+    if (!w) return fq_fail(dev, FQ_ERR_CUDA, "no host memory for a matrix");
     w->dev = dev;
     w->format = FQ_I8;
     w->rows = rows;
@@ -673,7 +676,7 @@ extern "C" int fq_matrix_create_i8(fq_device *dev, uint64_t rows, uint64_t cols,
         k_tile_i8<<<(unsigned)(tiles * 4), 256, 0, dev->stream>>>(src, rows, cols, k_blocks, w->data);
         e = cudaGetLastError();
     }
-    if (e == cudaSuccess) e = cudaMemcpyAsync(w->scales, host.data(), rows * 4, cudaMemcpyHostToDevice, dev->stream);
+    if (e == cudaSuccess) e = cudaMemcpyAsync(w->scales, host.get(), rows * 4, cudaMemcpyHostToDevice, dev->stream);
     if (e == cudaSuccess) e = cudaStreamSynchronize(dev->stream);
     if (staged) cudaFree(staged);
     int rc = fq_check_cuda(dev, e, "weight upload");
@@ -705,7 +708,7 @@ extern "C" int fq_project_many_i8(fq_device *dev, const fq_matrix *const *w, siz
         if (m > 0x7fffffffu / 8) return fq_fail(dev, FQ_ERR_SHAPE, "too many activation rows");
         const size_t yb = m * w[i]->rows * fq_dtype_size(y_dtype);
         if (int rc = fq_check_binding(dev, x, x_elems, "x")) return rc;
-        if (int rc = fq_check_binding(dev, x_scales, m * 4, "x_scales")) return rc;
+        if (int rc = fq_check_binding(dev, x_scales, m * 4, "x_scales", 4)) return rc;
         if (int rc = fq_check_binding(dev, y[i], yb, "y")) return rc;
         if (int rc = fq_check_no_alias(dev, y[i], yb, x, x_elems, "y")) return rc;
         if (int rc = fq_check_no_alias(dev, y[i], yb, x_scales, m * 4, "y")) return rc;

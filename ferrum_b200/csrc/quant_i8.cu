@@ -388,7 +388,7 @@ k_rows_i8(const T *x, const T *r, const float *w, uint32_t n, float eps, uint32_
                 c = 1.0 / sqrt(mean);
             }
         }
-        scales[row] = bad ? __int_as_float(0x7fc00000) : (float)(a64 * c * (1.0 / 127.0));
+        scales[row] = bad ? __int_as_float(0x7fc00000) : a64 > 0.0 ? (float)(a64 * c * (1.0 / 127.0)) : 0.f; // (c of zeros without eps is infinite)
     }
 
     // 127 v / a rounded, from the whole number next to it or nearly so: 127 v is compared with its borders times a.
@@ -463,7 +463,7 @@ cudaError_t launch_vec(fq_device *dev, const void *x, const void *r, const float
     if (n <= 1024) return launch_nt<OP, T, VEC, 32>(dev, tx, tr, w, n, eps, rows, (T *)h, q, scales);
     // With many rows the threads that a row's sums are joined over cost more than the time a row waits for itself; a few rows wait.
     // us with 128 / 256 / 512 threads: add_rmsnorm bf16 2048 x 5120 21.1 / 19.5 / -, gated unit 14.8 / 16.4 / -, 1021 x 17408 - /
-    // 24.5 / 22.2; one row of 5120 F32 with 256 / 512 XXX / 3.7.
+    // 24.5 / 22.2; add_rmsnorm F32 of one row of 5120 - / 4.1 / 3.5, of 200 - / 6.5 / 5.3.
     if (groups > (few ? 512 : 1600)) return launch_nt<OP, T, VEC, 512>(dev, tx, tr, w, n, eps, rows, (T *)h, q, scales);
     if (groups > (few ? 256 : OP == ADD_NORM ? 400 : 800)) return launch_nt<OP, T, VEC, 256>(dev, tx, tr, w, n, eps, rows, (T *)h, q, scales);
     return launch_nt<OP, T, VEC, 128>(dev, tx, tr, w, n, eps, rows, (T *)h, q, scales);
@@ -492,7 +492,7 @@ int check_rows(fq_device *dev, const void *x, const void *r, int dtype, const fl
     if (norm)
         if (int rc = fq_check_binding(dev, w, (size_t)n * 4, "w")) return rc;
     if (int rc = fq_check_binding(dev, q, count, "q")) return rc;
-    if (int rc = fq_check_binding(dev, scales, (size_t)rows * 4, "scales")) return rc;
+    if (int rc = fq_check_binding(dev, scales, (size_t)rows * 4, "scales", 4)) return rc;
     const struct { const void *p; size_t bytes; } in[3] = {{x, bytes}, {r, bytes}, {w, (size_t)n * 4}};
     for (const auto &i : in) {
         if (int rc = fq_check_no_alias(dev, q, count, i.p, i.bytes, "q")) return rc;

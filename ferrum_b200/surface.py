@@ -507,10 +507,13 @@ def _want(t: Optional[torch.Tensor], dtype: torch.dtype, count: int, name: str) 
         raise ShapeError(f"{name} of {t.numel()} values for {count}")
 
 
+_MOST = 0x7fffffff  # rows, and values of a row: the C interface has 32 bits for them
+
+
 def _rows_i8(x: torch.Tensor, rows: int, q: torch.Tensor, scales: torch.Tensor) -> int:
     """Checks the outputs of ``rows`` rows in 8 bits; the length of a row."""
     n = x.numel() // rows if rows > 0 else 0
-    if rows <= 0 or n * rows != x.numel():
+    if not 0 < rows <= _MOST or n * rows != x.numel() or n > _MOST:
         raise ShapeError(f"{x.numel()} values as {rows} rows")
     _want(q, torch.int8, x.numel(), "q")
     _want(scales, torch.float32, rows, "scales")
@@ -581,9 +584,9 @@ def token_logprobs(d: Device, logits: torch.Tensor, n: int, rows: int, ids: Opti
     default), the rows' entropy, and their k most likely tokens.  Outputs that are None are not computed."""
     _need(d, logits, ids, logprobs, ranks, entropy, top_logprobs, top_ids)
     stride = n if stride is None else stride
-    if n <= 0 or rows <= 0 or stride < n or logits.numel() < (rows - 1) * stride + n:
+    if not 0 < n <= _MOST or not 0 < rows <= _MOST or stride < n or logits.numel() < (rows - 1) * stride + n:
         raise ShapeError(f"{logits.numel()} values as {rows} rows of {n} logits, {stride} apart")
-    if k < 0:
+    if not 0 <= k <= n:
         raise ParameterError(f"{k} alternatives")
     for t, dtype, count, name in ((ids, torch.int32, rows, "ids"), (logprobs, torch.float32, rows, "logprobs"), (ranks, torch.int32, rows, "ranks"),
                                   (entropy, torch.float32, rows, "entropy"), (top_logprobs, torch.float32, rows * k, "top_logprobs"),

@@ -259,8 +259,8 @@ int fq_topk_blocks(fq_device *dev, const float *x, uint32_t n, uint32_t rows, fl
  *                       h may be x or r itself
  *   fq_glu_i8           v = silu(gate) * up
  * The row inputs are F32 or BF16, `rows` rows of n values (a multiple of 4); w is F32.  A row of zeros has scale 0.  A row
- * with an infinity or a NaN among its inputs or its v (for the norms: among h * w) has scale NaN and q = 0, which makes NaN of everything
- * projected from it and of nothing else. */
+ * with an infinity or a NaN among its inputs or its v (for the norms: among h * w) has scale NaN and q = 0, which makes NaN of
+ * everything projected from it and of nothing else.  Scales may start at any 4 bytes (those of later rows of a batch do). */
 int fq_quantize_i8(fq_device *dev, const void *x, int x_dtype, uint32_t n, uint32_t rows, int8_t *q, float *scales);
 int fq_rmsnorm_i8(fq_device *dev, const void *x, int x_dtype, const float *w, uint32_t n, float eps, uint32_t rows, int8_t *q, float *scales);
 int fq_add_rmsnorm_i8(fq_device *dev, const void *x, const void *r, int x_dtype, const float *w, uint32_t n, float eps, uint32_t rows, void *h,
@@ -273,7 +273,7 @@ int fq_glu_i8(fq_device *dev, const void *gate, const void *up, int dtype, uint3
 int fq_matrix_create_i8(fq_device *dev, uint64_t rows, uint64_t cols, const int8_t *values, const float *scales, fq_matrix **out);
 /* y[t][o] = (sum_k x[t][k] w[o][k]) * x_scales[t] * w_scale[o] for m rows of 8-bit integers.  The sum is exact at every
  * width; it is rounded to fp32 once, multiplied by the token's scale, then by the row's, and stored as F32 or BF16 (RNE).
- * x_elems must be m * cols and y_elems m * rows.  `fq_project_many_i8` is up to eight matrices of one width that share x
+ * x_elems must be m * cols and y_elems m * rows; x_scales may start at any 4 bytes.  `fq_project_many_i8` is up to eight matrices of one width that share x
  * (q|k|v, gate|up) in one launch; y[i] receives m * rows_i values. */
 int fq_project_i8(fq_device *dev, const fq_matrix *w, const int8_t *x, size_t x_elems, const float *x_scales, size_t m, void *y, int y_dtype,
                   size_t y_elems);

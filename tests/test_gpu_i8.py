@@ -325,6 +325,103 @@ def test_refused_calls(device):
     assert d.counters().dispatches == before, "a refused call enqueues nothing"
 
 
+@pytest.mark.parametrize("op", OPS)
+def test_rows_of_zeros_without_eps(device, op):
+    """Nothing divides by nothing: scale 0 and whole numbers 0, beside a row that has values."""
+    for n in (64, 5120, 60000):
+        x = torch.zeros(3, n, device="cuda")
+        x[1] = 1
+        q, s = torch.full((3, n), 9, dtype=torch.int8, device="cuda"), torch.full((3,), 9.0, device="cuda")
+        w = torch.ones(n, device="cuda")
+        torch.cuda.synchronize()
+        if op == "quantize":
+            S().quantize_i8(device, x, 3, q, s)
+        elif op == "rmsnorm":
+            S().rmsnorm_i8(device, x, w, 0.0, 3, q, s)
+        elif op == "add":
+            S().add_rmsnorm_i8(device, x, torch.zeros_like(x), w, 0.0, 3, torch.empty_like(x), q, s)
+        else:
+            S().glu_i8(device, x, x, 3, q, s)
+        device.synchronize()
+        assert not q[[0, 2]].any() and not s[[0, 2]].any() and torch.all(q[1] == 127) and s[1] > 0
+
+
+@pytest.mark.parametrize("first", [1, 2, 3])
+def test_later_rows_of_a_batch(device, first):
+    """A call on some rows of larger arrays: scales begin at any 4 bytes, and what lies around the rows stays as it was."""
+    rng = np.random.default_rng(first)
+    w, wq, ws = matrix(rng, device, 200, 272)
+    x = gpu(rng.standard_normal((9, 272)))
+    q, sc, y = torch.full((9, 272), 5, dtype=torch.int8, device="cuda"), torch.full((9,), 5.0, device="cuda"), torch.full((9, 200), 5.0, device="cuda")
+    part = slice(first, first + 4)
+    S().quantize_i8(device, x[part], 4, q[part], sc[part])
+    S().project_i8(device, w, q[part], sc[part], 4, y[part])
+    device.synchronize()
+    check_rows("quantize", x[part], None, None, q[part].cpu().numpy(), sc[part].cpu().numpy())
+    assert same(y[part], expect(q[part].cpu().numpy(), sc[part].cpu().numpy(), wq, ws))
+    around = [i for i in range(9) if not first <= i < first + 4]
+    assert torch.all(q[around] == 5) and torch.all(sc[around] == 5) and torch.all(y[around] == 5)
+
+
+def test_matrices_that_share_rows_are_one_launch(device):
+    rng = np.random.default_rng(8)
+    mats = [matrix(rng, device, r, 160) for r in (64, 200, 1)]
+    x, sc = gpu(rng.integers(-127, 128, (5, 160)), torch.int8), torch.ones(5, device="cuda")
+    ys = [torch.zeros(5, r, device="cuda") for r in (64, 200, 1)]
+    before = device.counters().dispatches
+    S().project_many_i8(device, [w for w, _, _ in mats], x, sc, 5, ys)
+    assert device.counters().dispatches == before + 1
+
+
+def test_on_other_streams_and_handles():
+    """A handle on torch's streams, one after the other, and a second handle beside it: each call is in its stream's order."""
+    s, rng = S(), np.random.default_rng(9)
+    wq, ws = rng.integers(-127, 128, (700, 1040), dtype=np.int8), np.ones(700, np.float32)
+    handles = [s.Device(0, use_torch_stream=False) for _ in range(2)]
+    mats = [s.Matrix.from_i8(d, wq, ws) for d in handles]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    x = [gpu(rng.standard_normal((6, 1040))) for _ in range(2)]
+    q = [torch.zeros(6, 1040, dtype=torch.int8, device="cuda") for _ in range(2)]
+    sc, y = [torch.zeros(6, device="cuda") for _ in range(2)], [torch.zeros(6, 700, device="cuda") for _ in range(2)]
+    torch.cuda.synchronize()
+    for step in range(4):
+        for i in range(2):
+            stream = streams[(i + step) % 2]
+            with torch.cuda.stream(stream):
+                handles[i].set_stream(stream.cuda_stream)
+                x[i].mul_(-0.75)  # on the same stream, before and after
+                s.quantize_i8(handles[i], x[i], 6, q[i], sc[i])
+                s.project_i8(handles[i], mats[i], q[i], sc[i], 6, y[i])
+                result = y[i].clone()
+            stream.synchronize()
+            check_rows("quantize", x[i], None, None, q[i].cpu().numpy(), sc[i].cpu().numpy())
+            assert same(result, expect(q[i].cpu().numpy(), sc[i].cpu().numpy(), wq, ws))
+    for d, w in zip(handles, mats):
+        w.close()
+        d.close()
+
+
+def test_an_injected_failure_launches_nothing():
+    """A refused submission leaves the outputs as they were; after the recovery the same call gives the result."""
+    s, rng = S(), np.random.default_rng(10)
+    d = s.Device(0)
+    w, wq, ws = matrix(rng, d, 130, 64)
+    x, q, sc, y = gpu(rng.standard_normal((3, 64))), torch.zeros(3, 64, dtype=torch.int8, device="cuda"), torch.zeros(3, device="cuda"), torch.zeros(3, 130, device="cuda")
+    lp = torch.zeros(3, device="cuda")
+    ids = torch.zeros(3, dtype=torch.int32, device="cuda")
+    calls = (lambda: s.quantize_i8(d, x, 3, q, sc), lambda: s.project_i8(d, w, q, sc, 3, y), lambda: s.token_logprobs(d, y, 130, 3, ids, lp, None, None))
+    for call, out in zip(calls, (q, y, lp)):
+        d.fail_after(0)
+        with pytest.raises(s.SynchronizationError):
+            call()
+        d.recover()
+        d.synchronize()
+        assert not out.any()
+        call()
+        d.synchronize()
+        assert out.any()
+
+
 def test_a_layer_on_8_bits_captured_and_replayed():
     """norm -> gate | up -> gated unit -> down -> norm -> output head -> scores on the handle's own stream: eagerly, then as a
     graph that is replayed on other inputs, beside a second graph of the same handle."""
