@@ -380,9 +380,13 @@ k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids
     const uint32_t whole_from = skip ? 1 : 0, whole_to = min(end, (uint32_t)(((uint64_t)skip + n) / V)); // pieces that lie in the row
     const uint32_t id = ids ? __ldcg(ids + row) : n;
     constexpr uint32_t NONE = sizeof(T) == 2 ? 0xFF80FF80u : 0xFF800000u; // -infinity
+    // The next pieces are under way while these are added, where four blocks an SM read bf16 (8 of 1021 rows of 151936: 69 instead
+    // of 74 us).  F32 pieces take longer to arrive than to add and lose by the registers (k = 20: 128 / 132 us), and so do eight blocks an
+    // SM (20 of 2000 rows of 8192 bf16 19.6 / 20.6).
+    constexpr bool EARLY = sizeof(T) == 2 && NT == 256;
     uint4 now[UNROLL];
     // This thread's UNROLL pieces of the block's UNROLL * NT from j0 on.
-    auto fetch = [&](uint32_t j0) {
+    auto fetch = [&](uint32_t j0, uint4 (&now)[UNROLL]) {
         if (j0 >= whole_from && j0 + UNROLL * NT <= whole_to) {
 #pragma unroll
             for (int u = 0; u < UNROLL; u++) now[u] = __ldcg(aligned + j0 + u * NT + tid);
@@ -396,7 +400,7 @@ k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids
             }
         }
     };
-    fetch(begin);
+    fetch(begin, now);
     const float given = id < n ? load1(l, id) : __int_as_float(0x7fc00000);
 
     // The largest of what is read first is the pivot.
@@ -415,6 +419,8 @@ k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids
 
 #pragma unroll 1
     for (uint32_t j0 = begin; j0 < end; j0 += UNROLL * NT) {
+        [[maybe_unused]] uint4 next[UNROLL];
+        if (EARLY && j0 + UNROLL * NT < end) fetch(j0 + UNROLL * NT, next);
         const float highest = largest<T>(now);
         if constexpr (TOP) {
             float h = highest;
@@ -482,7 +488,12 @@ k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids
             }
         s2 = add2(s2, s_tile);
         t2 = add2(t2, t_tile);
-        if (j0 + UNROLL * NT < end) fetch(j0 + UNROLL * NT);
+        if constexpr (EARLY) {
+#pragma unroll
+            for (int u = 0; u < UNROLL; u++) now[u] = next[u];
+        } else if (j0 + UNROLL * NT < end) {
+            fetch(j0 + UNROLL * NT, now);
+        }
     }
     a.s = s2.x + s2.y;
     a.t = t2.x + t2.y;
@@ -602,14 +613,18 @@ cudaError_t launch_rows(fq_device *dev, const T *logits, uint32_t n, size_t stri
     uint32_t parts = 1;
     while (parts < MAX_CLUSTER && rows * (2 * parts) <= 4 * sms && n / (2 * parts) >= 4096) parts *= 2;
     // Blocks that leave half the SMs empty have 512 threads (with 20 alternatives, us with 256 / 512: one row of 151936 F32 10.1 /
-    // 9.0, 16 of 32000 8.2 / 7.7; but 18 of 151936 bf16, more clusters of eight such blocks than run at once, 12.6 / 17.4); those of
-    // short rows 128, which their joins cost less (128 / 256: 2000 rows of 8192 bf16 19.6 / 26.6, 512 of 4096 9.2 / 9.6).
+    // 9.0, 16 of 32000 8.2 / 7.7; but 18 of 151936 bf16, more clusters of eight such blocks than run at once, 12.6 / 17.4).
     const bool wide = rows * parts <= sms / 2 && n > 8192;
+    // Those of short rows 128, which the joins of a row cost less (128 / 256: 2000 rows of 8192 bf16 19.6 / 26.6, 512 of 4096 9.2 /
+    // 9.6), and so those of longer whole rows as long as the SMs are filled about as often: eight of them an SM run at once, and
+    // take a tenth less than four (2048 of 50257 bf16 62 / 72, 2048 of 32000 F32 65 / 69, 1500 of 65536 F32 104 / 88).
+    const uint32_t fills_128 = (rows + 8 * sms - 1) / (8 * sms), fills_256 = (rows + 4 * sms - 1) / (4 * sms);
+    const bool narrow = n <= 8192 || (n <= 65536 && parts == 1 && 18 * fills_128 <= 10 * fills_256);
     auto go = [&](auto top) {
         constexpr bool TOP = decltype(top)::value;
         if (wide) return launch_shape<T, 512, TOP>(dev, logits, n, stride, rows, ids, k, parts, out);
-        if (n > 8192) return launch_shape<T, 256, TOP>(dev, logits, n, stride, rows, ids, k, parts, out);
-        return launch_shape<T, 128, TOP>(dev, logits, n, stride, rows, ids, k, parts, out);
+        if (narrow) return launch_shape<T, 128, TOP>(dev, logits, n, stride, rows, ids, k, parts, out);
+        return launch_shape<T, 256, TOP>(dev, logits, n, stride, rows, ids, k, parts, out);
     };
     return k ? go(std::true_type{}) : go(std::false_type{});
 }
