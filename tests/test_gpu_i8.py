@@ -47,6 +47,7 @@ def run_op(d, op, x, r, w, rows, h=None):
     n = x.numel() // rows
     q, s = torch.full((rows + 1, n), 99, dtype=torch.int8, device="cuda"), torch.full((rows + 4,), -7.0, device="cuda")
     qq, ss = q[:rows], s[:rows]
+    torch.cuda.synchronize()
     if op == "quantize":
         S().quantize_i8(d, x, rows, qq, ss)
     elif op == "rmsnorm":
@@ -185,6 +186,7 @@ def project(d, mats, xq, xs, dtype, many):
     bufs = [torch.full((m * w.rows + 64,), 5.5, dtype=dtype, device="cuda") for w in mats]
     ys = [b[:m * w.rows] for b, w in zip(bufs, mats)]
     x, scales = torch.from_numpy(xq).cuda(), torch.from_numpy(xs).cuda()
+    torch.cuda.synchronize()
     if many:
         S().project_many_i8(d, mats, x, scales, m, ys)
     else:
@@ -238,6 +240,7 @@ def test_a_matrix_made_on_the_device_or_the_host(device):
     rng = np.random.default_rng(0)
     x = gpu(rng.standard_normal((300, 272)))
     q, s = torch.zeros(300, 272, dtype=torch.int8, device="cuda"), torch.zeros(300, device="cuda")
+    torch.cuda.synchronize()
     S().quantize_i8(device, x, 300, q, s)  # weights of floats, quantised where they are
     mats = [S().Matrix.from_i8(device, q, s), S().Matrix.from_i8(device, q.cpu(), s.cpu()), S().Matrix.from_i8(device, q.cpu().numpy(), s)]
     assert (mats[0].rows, mats[0].cols, mats[0].experts, mats[0].format, mats[0].byte_size()) == (300, 272, 1, S().I8, 300 * 276)
@@ -332,14 +335,14 @@ def test_rows_of_zeros_without_eps(device, op):
         x = torch.zeros(3, n, device="cuda")
         x[1] = 1
         q, s = torch.full((3, n), 9, dtype=torch.int8, device="cuda"), torch.full((3,), 9.0, device="cuda")
-        w = torch.ones(n, device="cuda")
+        w, zeros = torch.ones(n, device="cuda"), torch.zeros_like(x)
         torch.cuda.synchronize()
         if op == "quantize":
             S().quantize_i8(device, x, 3, q, s)
         elif op == "rmsnorm":
             S().rmsnorm_i8(device, x, w, 0.0, 3, q, s)
         elif op == "add":
-            S().add_rmsnorm_i8(device, x, torch.zeros_like(x), w, 0.0, 3, torch.empty_like(x), q, s)
+            S().add_rmsnorm_i8(device, x, zeros, w, 0.0, 3, torch.empty_like(x), q, s)
         else:
             S().glu_i8(device, x, x, 3, q, s)
         device.synchronize()
@@ -354,6 +357,7 @@ def test_later_rows_of_a_batch(device, first):
     x = gpu(rng.standard_normal((9, 272)))
     q, sc, y = torch.full((9, 272), 5, dtype=torch.int8, device="cuda"), torch.full((9,), 5.0, device="cuda"), torch.full((9, 200), 5.0, device="cuda")
     part = slice(first, first + 4)
+    torch.cuda.synchronize()
     S().quantize_i8(device, x[part], 4, q[part], sc[part])
     S().project_i8(device, w, q[part], sc[part], 4, y[part])
     device.synchronize()
@@ -368,6 +372,7 @@ def test_matrices_that_share_rows_are_one_launch(device):
     mats = [matrix(rng, device, r, 160) for r in (64, 200, 1)]
     x, sc = gpu(rng.integers(-127, 128, (5, 160)), torch.int8), torch.ones(5, device="cuda")
     ys = [torch.zeros(5, r, device="cuda") for r in (64, 200, 1)]
+    torch.cuda.synchronize()
     before = device.counters().dispatches
     S().project_many_i8(device, [w for w, _, _ in mats], x, sc, 5, ys)
     assert device.counters().dispatches == before + 1
@@ -409,6 +414,7 @@ def test_an_injected_failure_launches_nothing():
     x, q, sc, y = gpu(rng.standard_normal((3, 64))), torch.zeros(3, 64, dtype=torch.int8, device="cuda"), torch.zeros(3, device="cuda"), torch.zeros(3, 130, device="cuda")
     lp = torch.zeros(3, device="cuda")
     ids = torch.zeros(3, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
     calls = (lambda: s.quantize_i8(d, x, 3, q, sc), lambda: s.project_i8(d, w, q, sc, 3, y), lambda: s.token_logprobs(d, y, 130, 3, ids, lp, None, None))
     for call, out in zip(calls, (q, y, lp)):
         d.fail_after(0)
@@ -420,6 +426,45 @@ def test_an_injected_failure_launches_nothing():
         call()
         d.synchronize()
         assert out.any()
+
+
+def test_rows_whose_offsets_pass_32_bits(device):
+    """2^32 values and more: every row is one of 64 that a call of their own has given."""
+    n, rows = 4096, (1 << 20) + 64
+    x = torch.randn(64, n, generator=torch.Generator().manual_seed(1)).cuda().bfloat16()
+    w = torch.ones(n, device="cuda")
+    few = [torch.zeros(64, n, dtype=torch.int8, device="cuda"), torch.zeros(64, device="cuda")]
+    many = [torch.zeros(rows, n, dtype=torch.int8, device="cuda"), torch.zeros(rows, device="cuda")]
+    every = x.repeat(rows // 64, 1)
+    torch.cuda.synchronize()
+    for op in ("quantize", "rmsnorm", "glu"):
+        for t, m, out in ((x, 64, few), (every, rows, many)):
+            out[0].zero_()
+            torch.cuda.synchronize()
+            if op == "quantize":
+                S().quantize_i8(device, t, m, *out)
+            elif op == "rmsnorm":
+                S().rmsnorm_i8(device, t, w, EPS, m, *out)
+            else:
+                S().glu_i8(device, t, t, m, *out)
+            device.synchronize()
+        assert torch.equal(many[0].view(-1, 64, n), few[0].expand(rows // 64, 64, n)) and torch.equal(many[1].view(-1, 64), few[1].expand(rows // 64, 64))
+
+
+def test_products_whose_offsets_pass_32_bits(device):
+    """70000 tokens by 64000 rows, 4.48e9 outputs: as torch has them in fp32, where sums of 16 products are exact."""
+    rng = np.random.default_rng(2)
+    m, rows, cols = 70000, 64000, 16
+    w, wq, ws = matrix(rng, device, rows, cols)
+    x, sc = gpu(rng.integers(-127, 128, (m, cols)), torch.int8), gpu(rng.random(m).astype(np.float32))
+    y = torch.zeros(m, rows, dtype=BF16, device="cuda")
+    torch.cuda.synchronize()
+    S().project_i8(device, w, x, sc, m, y)
+    device.synchronize()
+    wt, ws = gpu(wq).t().contiguous(), gpu(ws)
+    for t in (0, 33333, 67106, m - 600):  # row 67108 begins beyond 2^32 values
+        part = slice(t, t + 600)
+        assert torch.equal(y[part], ((x[part].float() @ wt) * sc[part, None] * ws).to(BF16))
 
 
 def test_a_layer_on_8_bits_captured_and_replayed():

@@ -20,7 +20,9 @@ def run(d, l, n, ids, k, stride=None):
     new = lambda count, dtype, fill: torch.full((count + 4,), fill, dtype=dtype, device="cuda")
     lp, rk, en = new(rows, F32, 9.5), new(rows, torch.int32, -9), new(rows, F32, 9.5)
     tp, ti = new(rows * k, F32, 9.5), new(rows * k, torch.int32, -9)
-    S().token_logprobs(d, l, n, rows, torch.from_numpy(np.asarray(ids, np.int64).astype(np.uint32).view(np.int32)).cuda(), lp[:rows], rk[:rows], en[:rows], k,
+    dev_ids = torch.from_numpy(np.asarray(ids, np.int64).astype(np.uint32).view(np.int32)).cuda()
+    torch.cuda.synchronize()
+    S().token_logprobs(d, l, n, rows, dev_ids, lp[:rows], rk[:rows], en[:rows], k,
                        tp[:rows * k] if k else None, ti[:rows * k] if k else None, stride)
     d.synchronize()
     for t, count in ((lp, rows), (rk, rows), (en, rows), (tp, rows * k), (ti, rows * k)):
@@ -234,6 +236,28 @@ def test_more_best_tokens_than_are_kept(device, rows):
             check(l.double().numpy(), ids, k, run(device, l.cuda().view(-1), n, ids, k))
 
 
+def test_rows_whose_offsets_pass_32_bits(device):
+    """Rows 2^31 values apart, the third beyond 2^32 of them, and a row that is itself longer than 2^30."""
+    rng, n, stride = np.random.default_rng(3), 50000, (1 << 31) + 5
+    whole = torch.empty(2 * stride + n, dtype=BF16, device="cuda")
+    l = torch.from_numpy(logits(rng, 3, n)).to(BF16)
+    for r in range(3):
+        whole[r * stride:r * stride + n] = l[r].cuda()
+    ids = rng.integers(0, n, 3)
+    check(l.double().numpy(), ids, 20, run(device, whole, n, ids, 20, stride))
+    n = (1 << 31) - 9
+    row = whole[3:3 + n].fill_(-30)
+    at = np.sort(rng.choice(n, 6, replace=False))
+    values = torch.tensor([1.0, 2.0, 3.0, 0.5, 2.0, -1.0], dtype=BF16)
+    row[torch.from_numpy(at).cuda()] = values.cuda()
+    lp, rk, en, tp, ti = run(device, row, n, [at[3]], 6)
+    assert ti[0].tolist() == at[[2, 1, 4, 0, 3, 5]].tolist() and rk[0] == 5
+    z = np.log(np.exp(values.double().numpy()).sum() + (n - 6) * np.exp(-30.0))
+    # The six terms as in `check`, (2 * 100 + 28) * 2^-24 = 1.4e-5 of their sum, 39.6; the far ones are 2e-4 together, 5e-6 of it
+    # even if all of them were lost beside larger ones.
+    assert abs(lp[0] - (0.5 - z)) <= 1e-5 * 2 + 2.0 ** -18
+
+
 def test_padding_rows_and_unwanted_outputs(device):
     """Ids that name no token, the same id in every row, and each output alone with the same values."""
     s, rng, n = S(), np.random.default_rng(4), 5000
@@ -245,6 +269,7 @@ def test_padding_rows_and_unwanted_outputs(device):
     x, new = l.cuda(), lambda dtype, *shape: torch.zeros(shape, dtype=dtype, device="cuda")
     dev_ids = torch.from_numpy(ids.astype(np.uint32).view(np.int32)).cuda()
     lp, rk, en, tp, ti = new(F32, 6), new(torch.int32, 6), new(F32, 6), new(F32, 6, 3), new(torch.int32, 6, 3)
+    torch.cuda.synchronize()
     s.token_logprobs(device, x, n, 6, dev_ids, lp, None, None)
     s.token_logprobs(device, x, n, 6, dev_ids, None, rk, None)
     s.token_logprobs(device, x, n, 6, None, None, None, en)
