@@ -202,8 +202,8 @@ template <bool TOP> struct Best { // shared memory of best_of
 };
 template <> struct Best<false> {};
 
-// The first `total` keys of the pool in order, the best MAX_TOP of them in S.out.
-template <int NT> __device__ __forceinline__ void order_pool(Best<true> &S, uint32_t total) {
+// The first `total` keys of the pool in order, the best MAX_TOP of them in S.out; `meanwhile` is done before the last barrier.
+template <int NT, typename F> __device__ __forceinline__ void order_pool(Best<true> &S, uint32_t total, F meanwhile) {
     const uint32_t tid = threadIdx.x;
     if (tid < MAX_TOP) S.out[tid] = 0;
     if (tid == 0) S.keys[total] = 0; // they are read by twos
@@ -218,14 +218,15 @@ template <int NT> __device__ __forceinline__ void order_pool(Best<true> &S, uint
         }
         if (higher < MAX_TOP) S.out[higher] = mine;
     }
+    meanwhile();
     __syncthreads();
 }
 
 // The k best (value, index) keys of the block's pieces [begin, end), sorted, in the lanes of its first warp (0 where there are
-// fewer); all threads call it, after what they noted (`noted` times, the largest `most`).
-template <typename T, int NT>
+// fewer); all threads call it, after what they noted (`noted` times, the largest `most`).  `meanwhile`: before its last barrier.
+template <typename T, int NT, typename F>
 __device__ __forceinline__ uint64_t best_of(Best<true> &S, const float *notes, uint32_t noted, float most, uint32_t shared_by, const T *l, const uint4 *aligned, uint32_t n,
-                                            uint32_t skip, uint32_t begin, uint32_t end, uint32_t k) {
+                                            uint32_t skip, uint32_t begin, uint32_t end, uint32_t k, F meanwhile) {
     constexpr uint32_t W = NT / 32, V = PER_LOAD<T>, TILE = UNROLL * NT;
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     // This thread's first piece of a note; the threads that have one come first.
@@ -348,7 +349,7 @@ __device__ __forceinline__ uint64_t best_of(Best<true> &S, const float *notes, u
             total = min(total, max(k, 1u));
             __syncthreads();
         }
-    order_pool<NT>(S, total);
+    order_pool<NT>(S, total, meanwhile);
     return S.out[lane];
 }
 
@@ -362,6 +363,7 @@ k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids
     __shared__ Sums sums[W];
     __shared__ uint32_t counts[W], bads[W];
     __shared__ Best<TOP> top;
+    __shared__ double row_z; // log of the row's sum of exponentials
     // Of block 0: what the blocks of the cluster found.
     __shared__ Sums all_sums[MAX_CLUSTER];
     __shared__ uint32_t all_counts[MAX_CLUSTER], all_bads[MAX_CLUSTER];
@@ -507,34 +509,65 @@ k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids
         counts[warp] = count;
         bads[warp] = flags;
     }
-    uint64_t list = 0;
-    if constexpr (TOP) {
-        list = best_of<T, NT>(top, notes, at_note, most, shared_by, l, aligned, n, skip, begin, end, k);
-    } else {
-        __syncthreads();
-    }
-    if (warp == 0) {
+    // From here on the last warp has the numbers and the first one, beside it, the list.
+    const bool numbers = warp == W - 1;
+    auto join_block = [&] {
         a = join_warp(lane < W ? sums[lane] : Sums{sums[0].c, 0.f, 0.f});
         count = __reduce_add_sync(0xffffffffu, lane < W ? counts[lane] : 0u);
         flags = __reduce_or_sync(0xffffffffu, lane < W ? bads[lane] : 0u);
+    };
+    auto finish = [&] {
+        double z, entropy;
+        if ((flags & 1) || !(flags & 4)) z = entropy = NAN;
+        else if ((flags & 2) || a.c < -MOST * LOG2E) sum_64(l, n, lane, z, entropy); // (the pivot is the row's largest or near it)
+        else {
+            // log2 S from its exponent and, within 2^-24, its mantissa.
+            const uint32_t bits = __float_as_uint(a.s);
+            const double log2_s = (double)((int)(bits >> 23) - 127) + (double)log2f(__uint_as_float((bits & 0x7FFFFFu) | 0x3F800000u));
+            z = ((double)a.c + log2_s) * (1.0 / (double)LOG2E);
+            entropy = 0.69314718055994531 * (log2_s - (double)a.t / (double)a.s);
+        }
+        if (lane == 0) {
+            if (out.logprobs) out.logprobs[row] = (float)((double)given - z);
+            if (out.ranks) out.ranks[row] = id < n ? 1 + count : 0;
+            if (out.entropy) out.entropy[row] = (float)entropy;
+            row_z = z;
+        }
+    };
+    uint64_t list = 0;
+    if constexpr (TOP) {
+        list = best_of<T, NT>(top, notes, at_note, most, shared_by, l, aligned, n, skip, begin, end, k, [&] {
+            if (!numbers) return;
+            join_block();
+            if (parts == 1) finish();
+        });
+    } else {
+        __syncthreads();
+        if (numbers) {
+            join_block();
+            if (parts == 1) finish();
+        }
     }
     if (parts > 1) {
         asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
-        if (warp == 0) {
+        if (numbers) {
             if (lane < 3) store_cluster(cluster_address(&all_sums[rank], 0) + 4 * lane, __float_as_uint(lane == 0 ? a.c : lane == 1 ? a.s : a.t));
             if (lane == 3) store_cluster(cluster_address(&all_counts[rank], 0), count);
             if (lane == 4) store_cluster(cluster_address(&all_bads[rank], 0), flags);
-            if constexpr (TOP) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(cluster_address(&all_lists[rank][lane], 0)), "l"(list) : "memory");
         }
+        if constexpr (TOP)
+            if (warp == 0) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(cluster_address(&all_lists[rank][lane], 0)), "l"(list) : "memory");
         __syncwarp();
         asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
         if (rank != 0) return;
-        if (warp == 0) {
+        auto join_cluster = [&] {
+            if (!numbers) return;
             a = join_warp(lane < parts ? all_sums[lane] : Sums{all_sums[0].c, 0.f, 0.f}, MAX_CLUSTER);
             a = Sums{__shfl_sync(0xffffffffu, a.c, 0), __shfl_sync(0xffffffffu, a.s, 0), __shfl_sync(0xffffffffu, a.t, 0)};
             count = __reduce_add_sync(0xffffffffu, lane < parts ? all_counts[lane] : 0u);
             flags = __reduce_or_sync(0xffffffffu, lane < parts ? all_bads[lane] : 0u);
-        }
+            finish();
+        };
         if constexpr (TOP) { // what reaches the largest of the lists' k-th keys, put in order by counting
             uint64_t kth = lane < parts ? all_lists[lane][k - 1] : 0;
 #pragma unroll
@@ -551,30 +584,16 @@ k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids
                 if (reach >> lane & 1) top.keys[at + lane] = key;
             }
             __syncthreads();
-            order_pool<NT>(top, top.found);
+            order_pool<NT>(top, top.found, join_cluster);
             list = top.out[lane];
+        } else {
+            join_cluster();
         }
     }
-    if (warp != 0) return;
-    double z, entropy;
-    if ((flags & 1) || !(flags & 4)) z = entropy = NAN;
-    else if ((flags & 2) || a.c < -MOST * LOG2E) sum_64(l, n, lane, z, entropy); // (the pivot is the row's largest or near it)
-    else {
-        // log2 S from its exponent and, within 2^-24, its mantissa.
-        const uint32_t bits = __float_as_uint(a.s);
-        const double log2_s = (double)((int)(bits >> 23) - 127) + (double)log2f(__uint_as_float((bits & 0x7FFFFFu) | 0x3F800000u));
-        z = ((double)a.c + log2_s) * (1.0 / (double)LOG2E);
-        entropy = 0.69314718055994531 * (log2_s - (double)a.t / (double)a.s);
-    }
-    if (lane == 0) {
-        if (out.logprobs) out.logprobs[row] = (float)((double)given - z);
-        if (out.ranks) out.ranks[row] = id < n ? 1 + count : 0;
-        if (out.entropy) out.entropy[row] = (float)entropy;
-    }
     if constexpr (TOP)
-        if (lane < k) {
+        if (warp == 0 && lane < k) {
             out.top_ids[(size_t)row * k + lane] = ~(uint32_t)list;
-            out.top_logprobs[(size_t)row * k + lane] = (float)((double)value_of((uint32_t)(list >> 32)) - z);
+            out.top_logprobs[(size_t)row * k + lane] = (float)((double)value_of((uint32_t)(list >> 32)) - row_z);
         }
 }
 
