@@ -498,83 +498,75 @@ def topk_blocks(d: Device, x: torch.Tensor, n: int, rows: int, out: torch.Tensor
     d.check(d._L.fq_topk_blocks(d.handle, _ptr(x), n, rows, _ptr(out)))
 
 
-def _want(t: Optional[torch.Tensor], dtype: torch.dtype, count: int, name: str) -> None:
-    if t is None:
-        return
-    if t.dtype != dtype:
-        raise Unsupported(f"{name} of {t.dtype}")
-    if t.numel() != count:
-        raise ShapeError(f"{name} of {t.numel()} values for {count}")
-
-
 _MOST = 0x7fffffff  # rows, and values of a row: the C interface has 32 bits for them
 
 
-def _rows_i8(x: torch.Tensor, rows: int, q: torch.Tensor, scales: torch.Tensor) -> int:
-    """Checks the outputs of ``rows`` rows in 8 bits; the length of a row."""
-    n = x.numel() // rows if rows > 0 else 0
-    if not 0 < rows <= _MOST or n * rows != x.numel() or n > _MOST:
-        raise ShapeError(f"{x.numel()} values as {rows} rows")
-    _want(q, torch.int8, x.numel(), "q")
-    _want(scales, torch.float32, rows, "scales")
-    return n
+def _fit(d: Device, t: Optional[torch.Tensor], dtype: torch.dtype, count: int, name: str) -> int:
+    """Checks one array of a call; its address (0 for None, which the library takes or refuses)."""
+    if t is None:
+        return 0
+    if t.get_device() != d.ordinal or t.dtype is not dtype or t.numel() != count or not t.is_contiguous():
+        _need(d, t)
+        if t.dtype != dtype:
+            raise Unsupported(f"{name} of {t.dtype}")
+        raise ShapeError(f"{name} of {t.numel()} values for {count}")
+    return t.data_ptr()
+
+
+def _rows_i8(d: Device, x: torch.Tensor, rows: int, q: torch.Tensor, scales: torch.Tensor):
+    """Checks the input and the outputs of ``rows`` rows in 8 bits; the input's values and those of a row, the outputs' addresses."""
+    _need(d, x)
+    count = x.numel()
+    n = count // rows if rows > 0 else 0
+    if not 0 < rows <= _MOST or n * rows != count or n > _MOST:
+        raise ShapeError(f"{count} values as {rows} rows")
+    return count, n, _fit(d, q, torch.int8, count, "q"), _fit(d, scales, torch.float32, rows, "scales")
 
 
 def quantize_i8(d: Device, x: torch.Tensor, rows: int, q: torch.Tensor, scales: torch.Tensor) -> None:
     """``rows`` rows of F32 or BF16 values as 8-bit integers with a scale per row."""
-    _need(d, x, q, scales)
-    n = _rows_i8(x, rows, q, scales)
-    d.check(d._L.fq_quantize_i8(d.handle, _ptr(x), _dtype_id(x), n, rows, _ptr(q), _ptr(scales)))
+    _, n, pq, ps = _rows_i8(d, x, rows, q, scales)
+    d.check(d._L.fq_quantize_i8(d.handle, x.data_ptr(), _dtype_id(x), n, rows, pq, ps))
 
 
 def rmsnorm_i8(d: Device, x: torch.Tensor, w: torch.Tensor, eps: float, rows: int, q: torch.Tensor, scales: torch.Tensor) -> None:
     """``rmsnorm`` with its rows in 8 bits: q * scale = rmsnorm(x) * w."""
-    _need(d, x, w, q, scales)
-    n = _rows_i8(x, rows, q, scales)
-    _want(w, torch.float32, n, "w")
-    d.check(d._L.fq_rmsnorm_i8(d.handle, _ptr(x), _dtype_id(x), _ptr(w), n, eps, rows, _ptr(q), _ptr(scales)))
+    _, n, pq, ps = _rows_i8(d, x, rows, q, scales)
+    d.check(d._L.fq_rmsnorm_i8(d.handle, x.data_ptr(), _dtype_id(x), _fit(d, w, torch.float32, n, "w"), n, eps, rows, pq, ps))
 
 
 def add_rmsnorm_i8(d: Device, x: torch.Tensor, r: torch.Tensor, w: torch.Tensor, eps: float, rows: int, h: torch.Tensor, q: torch.Tensor,
                    scales: torch.Tensor) -> None:
     """``add_rmsnorm`` with its rows in 8 bits: h = x + r, q * scale = rmsnorm(h) * w."""
-    _need(d, x, r, w, h, q, scales)
-    n = _rows_i8(x, rows, q, scales)
-    _want(r, x.dtype, x.numel(), "r")
-    _want(h, x.dtype, x.numel(), "h")
-    _want(w, torch.float32, n, "w")
-    d.check(d._L.fq_add_rmsnorm_i8(d.handle, _ptr(x), _ptr(r), _dtype_id(x), _ptr(w), n, eps, rows, _ptr(h), _ptr(q), _ptr(scales)))
+    count, n, pq, ps = _rows_i8(d, x, rows, q, scales)
+    pr, ph = _fit(d, r, x.dtype, count, "r"), _fit(d, h, x.dtype, count, "h")
+    d.check(d._L.fq_add_rmsnorm_i8(d.handle, x.data_ptr(), pr, _dtype_id(x), _fit(d, w, torch.float32, n, "w"), n, eps, rows, ph, pq, ps))
 
 
 def glu_i8(d: Device, gate: torch.Tensor, up: torch.Tensor, rows: int, q: torch.Tensor, scales: torch.Tensor) -> None:
     """``glu`` with its rows in 8 bits: q * scale = silu(gate) * up."""
-    _need(d, gate, up, q, scales)
-    n = _rows_i8(gate, rows, q, scales)
-    _want(up, gate.dtype, gate.numel(), "up")
-    d.check(d._L.fq_glu_i8(d.handle, _ptr(gate), _ptr(up), _dtype_id(gate), n, rows, _ptr(q), _ptr(scales)))
+    count, n, pq, ps = _rows_i8(d, gate, rows, q, scales)
+    d.check(d._L.fq_glu_i8(d.handle, gate.data_ptr(), _fit(d, up, gate.dtype, count, "up"), _dtype_id(gate), n, rows, pq, ps))
 
 
 def project_i8(d: Device, w: Matrix, x: torch.Tensor, x_scales: torch.Tensor, m: int, y: torch.Tensor) -> None:
     """y[m, rows] = (x[m, cols] . W^T) * x_scales * the scales of W's rows, x and W in 8-bit integers (``Matrix.from_i8``)."""
-    _need(d, x, x_scales, y)
-    _want(x, torch.int8, x.numel(), "x")
-    _want(x_scales, torch.float32, m, "x_scales")
-    d.check(d._L.fq_project_i8(d.handle, w.handle, _ptr(x), x.numel(), _ptr(x_scales), m, _ptr(y), _dtype_id(y), y.numel()))
+    _need(d, y)
+    count = x.numel()
+    px, ps = _fit(d, x, torch.int8, count, "x"), _fit(d, x_scales, torch.float32, m, "x_scales")
+    d.check(d._L.fq_project_i8(d.handle, w.handle, px, count, ps, m, y.data_ptr(), _dtype_id(y), y.numel()))
 
 
 def project_many_i8(d: Device, ws: Sequence[Matrix], x: torch.Tensor, x_scales: torch.Tensor, m: int, ys: Sequence[torch.Tensor]) -> None:
     """``project_i8`` by up to eight matrices of one width that share x (q|k|v, gate|up), in one launch."""
-    _need(d, x, x_scales, *ys)
     n = len(ws)
     if n == 0 or len(ys) != n:
         raise ParameterError(f"{n} matrices for {len(ys)} outputs")
-    _want(x, torch.int8, x.numel(), "x")
-    _want(x_scales, torch.float32, m, "x_scales")
-    for w, y in zip(ws, ys):
-        _want(y, ys[0].dtype, m * w.rows, "output")
+    count = x.numel()
+    px, ps = _fit(d, x, torch.int8, count, "x"), _fit(d, x_scales, torch.float32, m, "x_scales")
     wa = (C.c_void_p * n)(*[w.handle.value for w in ws])
-    ya = (C.c_void_p * n)(*[y.data_ptr() for y in ys])
-    d.check(d._L.fq_project_many_i8(d.handle, wa, n, _ptr(x), x.numel(), _ptr(x_scales), m, ya, _dtype_id(ys[0])))
+    ya = (C.c_void_p * n)(*[_fit(d, y, ys[0].dtype, m * w.rows, "output") for w, y in zip(ws, ys)])
+    d.check(d._L.fq_project_many_i8(d.handle, wa, n, px, count, ps, m, ya, _dtype_id(ys[0])))
 
 
 def token_logprobs(d: Device, logits: torch.Tensor, n: int, rows: int, ids: Optional[torch.Tensor], logprobs: Optional[torch.Tensor],
@@ -582,18 +574,16 @@ def token_logprobs(d: Device, logits: torch.Tensor, n: int, rows: int, ids: Opti
                    top_ids: Optional[torch.Tensor] = None, stride: Optional[int] = None) -> None:
     """Log probability and rank of the token ``ids[r]`` under row r of ``rows`` rows of n logits (``stride`` values apart, n by
     default), the rows' entropy, and their k most likely tokens.  Outputs that are None are not computed."""
-    _need(d, logits, ids, logprobs, ranks, entropy, top_logprobs, top_ids)
+    _need(d, logits)
     stride = n if stride is None else stride
     if not 0 < n <= _MOST or not 0 < rows <= _MOST or stride < n or logits.numel() < (rows - 1) * stride + n:
         raise ShapeError(f"{logits.numel()} values as {rows} rows of {n} logits, {stride} apart")
     if not 0 <= k <= n:
         raise ParameterError(f"{k} alternatives")
-    for t, dtype, count, name in ((ids, torch.int32, rows, "ids"), (logprobs, torch.float32, rows, "logprobs"), (ranks, torch.int32, rows, "ranks"),
-                                  (entropy, torch.float32, rows, "entropy"), (top_logprobs, torch.float32, rows * k, "top_logprobs"),
-                                  (top_ids, torch.int32, rows * k, "top_ids")):
-        _want(t, dtype, count, name)
-    d.check(d._L.fq_token_logprobs(d.handle, _ptr(logits), _dtype_id(logits), n, stride, rows, _ptr(ids), k, _ptr(logprobs), _ptr(ranks),
-                                   _ptr(entropy), _ptr(top_logprobs), _ptr(top_ids)))
+    f32, i32 = torch.float32, torch.int32
+    d.check(d._L.fq_token_logprobs(d.handle, logits.data_ptr(), _dtype_id(logits), n, stride, rows, _fit(d, ids, i32, rows, "ids"), k,
+                                   _fit(d, logprobs, f32, rows, "logprobs"), _fit(d, ranks, i32, rows, "ranks"), _fit(d, entropy, f32, rows, "entropy"),
+                                   _fit(d, top_logprobs, f32, rows * k, "top_logprobs"), _fit(d, top_ids, i32, rows * k, "top_ids")))
 
 
 def project_id(d: Device, w: Matrix, x: torch.Tensor, ids: torch.Tensor, routes: int, x_div: int, y: torch.Tensor) -> None:

@@ -9,16 +9,19 @@ from ferrum_b200 import _lib, surface as s
 F32 = torch.float32
 
 
+class Library:
+    def __getattr__(self, name):
+        def call(*args):
+            raise AssertionError(name + " was called")
+        return call
+
+
 class Handle:
-    """A device handle whose library must not be reached; its tensors lie on the CPU (ordinal -1) or on the GPU that is not there."""
-    handle = None
+    """A device handle whose library must not be called; its tensors lie on the CPU (ordinal -1) or on the GPU that is not there."""
+    handle, _L = None, Library()
 
     def __init__(self, ordinal):
         self.ordinal, self.torch_device = ordinal, torch.device("cuda", max(ordinal, 0))
-
-    @property
-    def _L(self):
-        raise AssertionError("the library was called")
 
     def check(self, rc):
         raise AssertionError("the library was called")
@@ -67,6 +70,7 @@ def test_rows_refused():
 def test_more_rows_than_the_interface_counts():
     """Sizes that 32 bits would cut to others are refused, not cut."""
     d = Handle(-1)
+
     class Flat:  # a contiguous tensor of that many values, without their memory
         def __init__(self, dtype, count):
             self.dtype, self.count = dtype, count
