@@ -494,7 +494,7 @@ uint32_t stage_bytes(const Plan &p) { return TILE_BYTES + (p.pair ? p.bn / 2 : p
 //     SM streams weights at 57 bytes a clock, L2 feeds all of them 6500 a clock; the first ring of it comes at once;
 //   - HBM delivers 3440 bytes of weights a clock;
 //   - a cluster's exchange takes 1300 clocks and 55 a token; a pair's start 1000.
-// us, estimated best against the other (rows x cols, tokens): 5120 x 17408, 1: three slices 16.4, one 21.1; 8192 x 5120, 1: one
+// us, estimated best against the other (rows x cols, tokens): 5120 x 17408, 1: three slices 16.3, two 17.1, one 21.1; 8192 x 5120, 1: one
 // 9.1, two 9.9, 64: one 10.8, two 13.2; 34816 x 5120, 2048: pairs 224, single blocks 335.
 Plan plan(const fq_device *dev, const fq_matrix *const *w, uint32_t count, uint32_t k_blocks, uint32_t m) {
     const uint32_t sms = (uint32_t)dev->sm_count;
@@ -525,7 +525,7 @@ Plan plan(const fq_device *dev, const fq_matrix *const *w, uint32_t count, uint3
         const double feed = std::max(TILE_BYTES / 57.0 + (stage_bytes(c) - TILE_BYTES) / 300.0, stage_bytes(c) * active / 6500.0);
         const double rounds = (items + slots - 1) / slots, ring = std::min(c.per, 8u) * std::max(0.0, feed - mma);
         const double cost = std::max(hbm, rounds * c.per * std::max(mma, feed) - ring) + 6.0 * c.bn + (c.slices > 1 ? 1300.0 + 55.0 * c.bn : 0.0) + (pair ? 1000.0 : 0.0);
-        if (p.bn == 0 || cost < best) {
+        if (p.bn == 0 || cost <= best) { // (of equals the one with more blocks)
             best = cost;
             p = c;
         }

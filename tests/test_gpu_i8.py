@@ -211,6 +211,20 @@ def test_projections_of_every_shape(device, rows, cols, m, dtype):
     assert same(project(device, [w], xq, xs, dtype, False)[0], expect(xq, xs, wq, ws))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shapes,cols,m", [((20011,), 528, 16), ((20011,), 16, 1), ((19000, 5, 300), 1040, 70), ((40000,), 144, 130),  # more items than blocks
+                                           ((5000, 3001), 1040, 600), ((10007,), 272, 1100), ((5121, 1000), 2064, 2048), ((4000,), 2048, 1030),  # pairs, several items each
+                                           ((257,), 20000, 700), ((3000,), 4112, 700),  # pairs, one item
+                                           ((1000,), 8208, 300), ((2500,), 16400, 33), ((640,), 8208, 40), ((1500,), 4112, 17), ((700,), 65536, 250)])  # clusters
+def test_projections_of_every_cut(device, shapes, cols, m, dtype):
+    """Products large enough to be cut in each of the ways there are."""
+    rng = np.random.default_rng(cols + m)
+    mats = [matrix(rng, device, r, cols) for r in shapes]
+    xq, xs = rng.integers(-128, 128, (m, cols), dtype=np.int8), rng.random(m).astype(np.float32)
+    for y, (_, wq, ws) in zip(project(device, [w for w, _, _ in mats], xq, xs, dtype, True), mats):
+        assert same(y, expect(xq, xs, wq, ws))
+
+
 @pytest.mark.parametrize("m", [1, 16, 260])
 def test_the_largest_sums(device, m):
     """65536 products of 2^14: 2^30 fits, and so does its negative."""
