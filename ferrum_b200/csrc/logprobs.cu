@@ -21,7 +21,6 @@
 // by, against a bound that rose slowly, in the first version: 20 to 90 us more for 8 to 32 alternatives of 1021 rows).
 // Keys (value, index) are unique, of equal values the lower index is larger, so nothing depends on the order of threads.
 #include <algorithm>
-#include <atomic>
 #include <cmath>
 #include <type_traits>
 
@@ -33,7 +32,10 @@ using namespace fqk;
 
 constexpr uint32_t MAX_TOP = 32, MAX_CLUSTER = 8;
 constexpr int UNROLL = 4; // 16-byte loads of a thread in flight
-template <int NT> constexpr uint32_t NOTES = 40 * 256 / NT; // maxima that a thread notes (more tiles than these share one)
+// Maxima that a thread notes; tiles share one where they are more.  Eight KB a block: with 40 the blocks' shared memory left so little
+// of the L1 cache that loads waited for a place in it (20 alternatives of 1021 rows of 151936 F32: 128 us, with 20 / 12 / 8 / 6 / 4
+// 122 / 121 / 121 / 122 / 125; of 300 rows of 1000000 with 12 / 8 / 4 316 / 320 / 330).
+template <int NT> constexpr uint32_t NOTES = 8 * 256 / NT;
 constexpr uint32_t POOL = 512;   // pieces read again, and values kept of them
 constexpr float LOG2E = 1.44269502f; // b: log2(e) rounded to fp32
 constexpr float SLACK = 20.f;        // how far b l may be above the pivot
@@ -605,14 +607,6 @@ cudaError_t launch_shape(fq_device *dev, const T *logits, uint32_t n, size_t str
     const uint32_t pieces = (n + PER_LOAD<T> - 1) / PER_LOAD<T> + 1, tiles = (pieces + parts - 1) / parts / (UNROLL * NT) + 1;
     cfg.dynamicSmemBytes = TOP ? std::min(tiles, NOTES<NT>) * NT * sizeof(float) : 0;
     auto kernel = k_token_logprobs<T, NT, TOP>;
-    if (cfg.dynamicSmemBytes > (36 << 10)) { // with the kernel's own arrays beyond what it may use unasked: asked for once per device
-        static std::atomic<uint64_t> asked{0};
-        const uint64_t bit = 1ull << (dev->ordinal & 63);
-        if (!(asked.load(std::memory_order_relaxed) & bit) || dev->ordinal > 63) {
-            if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(NOTES<NT> * NT * sizeof(float)))) return e;
-            asked.fetch_or(bit, std::memory_order_relaxed);
-        }
-    }
     cfg.stream = dev->stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
