@@ -18,6 +18,9 @@
 // eight blocks cuts an item's K and adds the partial sums (whole numbers, so in any order) through distributed shared memory:
 // block r of the cluster collects and stores the tokens of its share, which the others send as one bulk copy each (value by
 // value, remote stores took 45 us for q|k|v of 128 rows where these took 24).  All waits are bounded (tcgen05.cuh).
+//
+// Up to about 128 tokens HBM bounds it (gate|up, 2 x 17408 x 5120: 16 tokens 27.7 us, 6.5 TB/s), from there the tensor pipe (2048
+// tokens 215 us, 3.4 POP/s, 95 % active); small matrices the launch and the filling of the ring (q|k|v of one token 9.1 us).
 #include <algorithm>
 #include <cmath>
 #include <cstring>

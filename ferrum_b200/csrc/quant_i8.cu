@@ -14,6 +14,9 @@
 // eights in 32 bits and from there in 64.
 // (Held in registers, unrolled over a row, the same took 105 registers and 63 instructions a value, a third of the time
 // waiting for instructions: 2048 x 5120 bf16 45 us.)
+//
+// What bounds it is a row's chain of dependent steps, of which the blocks of an SM cover a part: add_rmsnorm of 2048 x 5120 bf16
+// 20 us (3.7 TB/s) and F32 26 us (5.2 TB/s), the gated unit of 1021 x 17408 bf16 22 us (4.0 TB/s), one row of 5120 F32 3.5 us.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
