@@ -635,9 +635,10 @@ cudaError_t launch_rows(fq_device *dev, const T *logits, uint32_t n, size_t stri
     const bool wide = rows * parts <= sms / 2 && n > 8192;
     // Those of short rows 128, which the joins of a row cost less (128 / 256: 2000 rows of 8192 bf16 19.6 / 26.6, 512 of 4096 9.2 /
     // 9.6), and so those of longer whole rows as long as the SMs are filled about as often: eight of them an SM run at once, and
-    // take a tenth less than four (2048 of 50257 bf16 62 / 72, 2048 of 32000 F32 65 / 69, 1500 of 65536 F32 104 / 88).
+    // take up to a tenth less than four (2048 of 32000 F32 65 / 69, of 100000 163 / 169; 1500 of 65536 F32 104 / 88).  Long bf16
+    // rows are faster with their pieces fetched ahead (2048 of 50257 62 / 64, of 100000 98 / 96, 1021 of 151936 79 / 72).
     const uint32_t fills_128 = (rows + 8 * sms - 1) / (8 * sms), fills_256 = (rows + 4 * sms - 1) / (4 * sms);
-    const bool narrow = n <= 8192 || (n <= 65536 && parts == 1 && 18 * fills_128 <= 10 * fills_256);
+    const bool narrow = n <= 8192 || ((sizeof(T) == 4 || n <= 65536) && parts == 1 && 18 * fills_128 <= 10 * fills_256);
     auto go = [&](auto top) {
         constexpr bool TOP = decltype(top)::value;
         if (wide) return launch_shape<T, 512, TOP>(dev, logits, n, stride, rows, ids, k, parts, out);
