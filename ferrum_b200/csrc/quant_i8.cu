@@ -422,7 +422,10 @@ k_rows_i8(const T *x, const T *r, const float *w, uint32_t n, float eps, uint32_
     } else {
         for (uint32_t i = tid; i < groups; i += NT)
 #pragma unroll 1
-            for (uint32_t k = 0; k < VEC; k++) q[VEC * i + k] = !bad && a64 > 0.0 ? (int8_t)__double2int_rn(exact(VEC * i + k) * 127.0 / a64) : 0;
+            for (uint32_t k = 0; k < VEC; k++) {
+                const double v = bad ? 0.0 : exact(VEC * i + k); // (a quotient is rounded twice, and a tie falls to either side)
+                q[VEC * i + k] = a64 > 0.0 ? rounded(v, __double2int_rn(v * 127.0 / a64)) : 0;
+            }
     }
 }
 

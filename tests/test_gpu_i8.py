@@ -27,6 +27,10 @@ def rows_to_8_bits(v, factor):
     """The definition on 64-bit rows: whole numbers (ties to even) and scales."""
     a = np.abs(v).max(axis=1, keepdims=True)
     q = np.rint(v * 127 / np.where(a > 0, a, 1))
+    # The quotient is rounded twice, which takes a tie to either side of it; half of the largest value is one, and the two
+    # products of that comparison are one number rounded once: 127 (a / 2) = 63.5 a.
+    half = 127 * np.abs(v) == 63.5 * a
+    q[half & (a > 0)] = (64 * np.sign(v))[half & (a > 0)]
     return q, (a * factor / 127)[:, 0]
 
 
@@ -119,6 +123,28 @@ def test_ties_go_to_the_even_number(device, dtype):
         check_rows("quantize", x, None, None, *run_op(device, "quantize", x, None, None, 1))
         ones = torch.ones(v.shape[1], device="cuda")
         check_rows("rmsnorm", x, None, ones, *run_op(device, "rmsnorm", x, None, ones, 1))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("size", [1.0, 2.0 ** 60, 2.0 ** -90])
+@pytest.mark.parametrize("op", OPS)
+def test_half_of_the_largest_value_goes_to_64(device, op, size, dtype):
+    """63.5 is a tie, at sizes that are rounded in 32 bits and at those that are in 64, whatever the products' own roundings."""
+    rng, rows, n = np.random.default_rng(5), 400, 72
+    x, r, w = size * 0.1 * rng.standard_normal((rows, n)), np.zeros((rows, n)), 1 + 0.1 * rng.standard_normal(n)
+    w[1] = w[0]
+    x[:, 0] = size * (1 + rng.random(rows)) * rng.choice([-1, 1], rows)
+    if op == "glu":  # of one gate
+        x, r = rng.standard_normal((rows, n)), x
+        x[:, :2] = 1 + 4 * rng.random((rows, 1))
+    x, r, w = gpu(x, dtype), gpu(r, dtype), gpu(w)
+    t = r if op == "glu" else x
+    t[:, 1] = t[:, 0] / 2
+    q, s = run_op(device, op, x, r, w, rows, torch.zeros_like(x))
+    v = values_of(op, x, r, w)[0]
+    assert np.all(np.abs(v).argmax(1) == 0)
+    assert np.array_equal(q[:, 0], 127 * np.sign(v[:, 0])) and np.array_equal(q[:, 1], 64 * np.sign(v[:, 0]))
+    check_rows(op, x, r, w, q, s)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
