@@ -143,8 +143,10 @@ template <int OP> constexpr float OFF = OP == GLU ? 24 * 0x1p-24f : 4 * 0x1p-24f
 // gated unit is off by at most 10 steps, and so is the largest.
 template <int OP> constexpr uint32_t BELOW = OP == GLU ? 24 : 0;
 // Rows that leave these go through 64 bits throughout: the largest |v|, so that what 32 bits lose to underflow is nothing
-// beside it; and of the norms the largest sum of four squares, of the gated unit the largest |u|, for the same reason.
-constexpr float LEAST = 1e-20f, MOST = 1e37f;
+// beside it; and of the norms the largest sum of four squares, of the gated unit the largest |u|, for the same reason.  Of a
+// row as it is products of up to 127.5 and the largest |v| are taken in 32 bits (`settle`): fp32 ends at 127.5 * 2.66e36.
+constexpr float LEAST = 1e-20f;
+template <int OP> constexpr float MOST = OP == PLAIN ? 2.5e36f : 1e37f;
 template <int OP> constexpr float LEAST_2 = OP == NORM || OP == ADD_NORM ? 1e-20f : 0.f;
 template <int OP> constexpr float MOST_2 = OP == GLU ? 1048576.f : 1e37f;
 
@@ -290,7 +292,7 @@ k_rows_i8(const T *x, const T *r, const float *w, uint32_t n, float eps, uint32_
         if constexpr (OP != PLAIN) most_2 = __reduce_max_sync(0xffffffffu, part_2[lane % W]);
     }
 
-    const bool fast = __uint_as_float(most) >= LEAST && __uint_as_float(most) <= MOST &&
+    const bool fast = __uint_as_float(most) >= LEAST && __uint_as_float(most) <= MOST<OP> &&
                       (OP == PLAIN || (__uint_as_float(most_2) >= LEAST_2<OP> && __uint_as_float(most_2) <= MOST_2<OP>));
     double a64 = 0.0; // the row's largest |v|, exactly: of the thread's own values first
     bool bad = false;

@@ -587,3 +587,27 @@ def test_a_layer_on_8_bits_captured_and_replayed():
     for g in graphs:
         g.close()
     d.close()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("size", [9e35, 2.5e36, 5e36, 2e37])
+@pytest.mark.parametrize("n", [72, 4096])
+@pytest.mark.parametrize("op", OPS)
+def test_half_of_a_largest_value_whose_products_pass_the_end_of_fp32(device, op, n, size, dtype):
+    """127 times half of these, and 63.5 times their whole, are about fp32's largest number and beyond it."""
+    rng, rows = np.random.default_rng(6), 400
+    x, r, w = size * 0.1 * rng.standard_normal((rows, n)), np.zeros((rows, n)), 1 + 0.1 * rng.standard_normal(n)
+    x = np.clip(x, -0.4 * size, 0.4 * size)
+    w[:2] = w.max()
+    x[:, 0] = size * (1 + rng.random(rows)) * rng.choice([-1, 1], rows)
+    if op == "glu":  # of one gate, the largest of the row
+        x, r = rng.standard_normal((rows, n)), x
+        x[:, :2] = 4 + rng.random((rows, 1))
+    x, r, w = gpu(x, dtype), gpu(r, dtype), gpu(w)
+    t = r if op == "glu" else x
+    t[:, 1] = t[:, 0] / 2
+    q, s = run_op(device, op, x, r, w, rows, torch.zeros_like(x))
+    v = values_of(op, x, r, w)[0]
+    assert np.all(np.abs(v).argmax(1) == 0)
+    assert np.array_equal(q[:, 0], 127 * np.sign(v[:, 0])) and np.array_equal(q[:, 1], 64 * np.sign(v[:, 0]))
+    check_rows(op, x, r, w, q, s)
