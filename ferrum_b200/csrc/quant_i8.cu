@@ -124,13 +124,16 @@ __device__ __forceinline__ float rcp(float v) { // within 2^-23 of itself
     return r;
 }
 // silu(g) u for two values, e^-g = 2^t (1 + d ln 2) with t = -g log2 e rounded and d what the rounding took.  Relative error at
-// most 10 * 2^-24: 5 of the exponential, 1 of 1 + e^-g, 2 of its reciprocal and one of each product.  Beyond g = -87, where t is
-// held at 126, it is off by less than 2^-118 |u|.
+// most 10 * 2^-24: 5 of the exponential, 1 of 1 + e^-g, 2 of its reciprocal and one of each product.  Below g = -87.34, where the
+// reciprocal is below 2^-126 and flushed, it is 0 and off by less than 2^-119 |u|.  For that g is held at -127 ln 2 in t and in d
+// alike: of t alone, d of a g past 2^24 is the rounding of a t that is not used, and 1 + d ln 2 can be next to nothing.  The factor g
+// is as it is, so that an infinite one gives NaN.
 __device__ __forceinline__ float2 gated(const float2 &g, const float2 &u) {
-    constexpr float LOG2E = 1.44269502f, LOG2E_REST = 1.92596299e-8f, LN2 = 0.693147182f;
-    const float2 t = __fmul2_rn(g, both(-LOG2E));
-    const float2 d = __ffma2_rn(g, both(-LOG2E_REST), __ffma2_rn(g, both(-LOG2E), minus(t)));
-    const float2 e = make_float2(ex2(fminf(t.x, 126.f)), ex2(fminf(t.y, 126.f)));
+    constexpr float LOG2E = 1.44269502f, LOG2E_REST = 1.92596299e-8f, LN2 = 0.693147182f, LOWEST = -88.0296936f;
+    const float2 held = make_float2(fmaxf(g.x, LOWEST), fmaxf(g.y, LOWEST));
+    const float2 t = __fmul2_rn(held, both(-LOG2E));
+    const float2 d = __ffma2_rn(held, both(-LOG2E_REST), __ffma2_rn(held, both(-LOG2E), minus(t)));
+    const float2 e = make_float2(ex2(t.x), ex2(t.y));
     const float2 s = __fadd2_rn(__ffma2_rn(__fmul2_rn(d, both(LN2)), e, e), both(1.f));
     return __fmul2_rn(__fmul2_rn(g, make_float2(rcp(s.x), rcp(s.y))), u);
 }

@@ -611,3 +611,26 @@ def test_half_of_a_largest_value_whose_products_pass_the_end_of_fp32(device, op,
     assert np.all(np.abs(v).argmax(1) == 0)
     assert np.array_equal(q[:, 0], 127 * np.sign(v[:, 0])) and np.array_equal(q[:, 1], 64 * np.sign(v[:, 0]))
     check_rows(op, x, r, w, q, s)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("size", [4e-20, 1e-18, 1.0])
+@pytest.mark.parametrize("n", [1024, 5120, 20480, 70004])
+def test_gates_far_below_zero(device, n, size, dtype):
+    """silu of a gate below -88 is next to nothing: beside a large `up` it is still nothing to a row of small values."""
+    rng, rows = np.random.default_rng(n), 24
+    x, r = 1 + np.abs(rng.standard_normal((rows, n))), size * rng.standard_normal((rows, n))
+    # Where the rounding of g log2 e, a step or more of it, all but cancels a factor of the exponential.
+    worst = [-16770166.0, -23336016.0, -23386954.0, -68910152.0, -1175864200.0, -28420063232.0, -1024.0, -89.0, -88.03, -88.02, -87.34, -87.33, -3.3e38]
+    far = rng.random((rows, n)) < 0.3
+    far[:, 0] = False
+    x[far] = -np.exp(rng.uniform(np.log(80.0), np.log(3.3e38), far.sum()))
+    for row in range(rows):
+        at = 1 + rng.choice(n - 1, len(worst), replace=False)
+        x[row, at], far[row, at] = worst, True
+    r[far] = rng.choice([-1, 1], far.sum()) * 2.0 ** 20
+    if dtype == BF16:  # every bf16 gate there is below -80
+        every = (np.arange(0xC2A0, 0xFF80, dtype=np.uint32) << 16).view(np.float32)
+        x[far] = np.resize(rng.permutation(every), far.sum())
+    x, r = gpu(x, dtype), gpu(r, dtype)
+    check_rows("glu", x, r, None, *run_op(device, "glu", x, r, None, rows))
