@@ -11,6 +11,9 @@
 //
 //   S = sum 2^(b l - c)     T = sum 2^(b l - c) (b l - c)     z = (c + log2 S) / b     entropy = ln 2 (log2 S - T / S)
 //
+// Where one token has all of the probability, l_id - z and the entropy are what the roundings of c, S and T leave (less than 2^-21, of
+// either sign).  No log probability above 0 and no entropy below it is given out: such values are 0.
+//
 // b l - c is one FMA with one rounding; c is the largest b l of what the block reads first and moves only when a logit is more
 // than 20 / b above it (a term is 2^20 at most, far from fp32's end; a running maximum would rescale every few values).  Dividing by b as
 // it is keeps its own rounding out of z.
@@ -186,6 +189,8 @@ template <typename T> __device__ __noinline__ void sum_64(const T *l, uint32_t n
     z = mx + log(s);
     entropy = log(s) - t / s;
 }
+
+__device__ __forceinline__ float not_above_0(double v) { return v > 0.0 ? 0.f : (float)v; } // NaN stays NaN
 
 struct Outputs {
     float *logprobs;
@@ -535,9 +540,9 @@ k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids
             entropy = 0.69314718055994531 * (log2_s - (double)a.t / (double)a.s);
         }
         if (lane == 0) {
-            if (out.logprobs) out.logprobs[row] = (float)((double)given - z);
+            if (out.logprobs) out.logprobs[row] = not_above_0((double)given - z);
             if (out.ranks) out.ranks[row] = id < n ? 1 + count : 0;
-            if (out.entropy) out.entropy[row] = (float)entropy;
+            if (out.entropy) out.entropy[row] = entropy < 0.0 ? 0.f : (float)entropy;
             row_z = z;
         }
     };
@@ -600,7 +605,7 @@ k_token_logprobs(const T *logits, uint32_t n, size_t stride, const uint32_t *ids
     if constexpr (TOP)
         if (warp == 0 && lane < k) {
             out.top_ids[(size_t)row * k + lane] = ~(uint32_t)list;
-            out.top_logprobs[(size_t)row * k + lane] = (float)((double)value_of((uint32_t)(list >> 32)) - row_z);
+            out.top_logprobs[(size_t)row * k + lane] = not_above_0((double)value_of((uint32_t)(list >> 32)) - row_z);
         }
 }
 

@@ -289,6 +289,7 @@ int fq_project_many_i8(fq_device *dev, const fq_matrix *const *w, size_t count, 
  * Logits are F32 or BF16: `rows` rows of n, the first of each `stride` values (at least n) after the one before; what lies
  * between the rows is not read.  An output that is not wanted is NULL (top_ids and top_logprobs are when k = 0), and so is `ids`
  * when neither logprobs nor ranks are wanted.
+ * Log probabilities are never above 0 and entropies never below it.
  * A logit of -infinity is a token of probability 0: it adds nothing, and its own log probability is -infinity.  A row with a
  * NaN, with +infinity, or with nothing above -infinity has no distribution: its log probabilities and entropy are NaN; ranks
  * and top_ids still follow the order of the logits, a NaN below everything.  An id that is not below n names no token (a row

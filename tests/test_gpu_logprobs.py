@@ -332,3 +332,21 @@ def test_refused_calls(device):
         with pytest.raises(error):
             call()
     assert d.counters().dispatches == before, "a refused call enqueues nothing"
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,n", [(2000, 1), (2000, 64), (300, 5000), (20, 60000), (3, 151936), (600, 33000)])
+def test_one_token_with_all_of_the_probability(device, rows, n, dtype):
+    """Where a grammar allows one token, or one is far above the others: no log probability above 0, no entropy below it."""
+    rng = np.random.default_rng(n)
+    for below in (-np.inf, torch.finfo(dtype).min, -300.0):
+        l = np.full((rows, n), below)
+        keep = rng.integers(0, n, rows)
+        l[np.arange(rows), keep] = rng.uniform(-40, 40, rows)
+        t = torch.from_numpy(l).to(dtype)
+        ids = keep.copy()
+        ids[::5] = rng.integers(0, n, len(ids[::5]))
+        for k in (0, min(n, 3)):
+            got = run(device, t.cuda().view(-1), n, ids, k)
+            check(t.double().numpy(), ids, k, got)
+            assert (got[0] <= 0).all() and (got[2] >= 0).all() and (got[3] <= 0).all()
