@@ -215,11 +215,17 @@ int fq_check_binding(fq_device *dev, const void *p, size_t bytes, const char *na
     return FQ_OK;
 }
 
+int fq_check_apart(fq_device *dev, const void *a, size_t a_bytes, const void *b, size_t b_bytes, const char *name) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    if (a && b && x < y + b_bytes && y < x + a_bytes) return fq_fail(dev, FQ_ERR_ALIAS, "%s: output overlaps an input or another output", name);
+    return FQ_OK;
+}
+
 int fq_check_no_alias(fq_device *dev, const void *out, size_t out_bytes, const void *in, size_t in_bytes,
                       const char *name) {
-    const uintptr_t o = (uintptr_t)out, i = (uintptr_t)in;
+    const uintptr_t i = (uintptr_t)in;
     if (!out || !in) return FQ_OK;
-    if (o < i + in_bytes && i < o + out_bytes) return fq_fail(dev, FQ_ERR_ALIAS, "%s: output overlaps an input", name);
+    if (int rc = fq_check_apart(dev, out, out_bytes, in, in_bytes, name)) return rc;
     // What a failed submission wrote is not an input until it has been written again.  Only buffers the handle
     // allocated itself are tracked (`fq_buffer_alloc`, the counterpart of the reference's device buffers): memory the
     // caller owns is recycled and rewritten by the caller's allocator without the library seeing it.
@@ -797,7 +803,7 @@ extern "C" int fq_project_many(fq_device *dev, const fq_matrix *const *w, size_t
         if (int rc = fq_check_binding(dev, y[i], yb, "y")) return rc;
         if (int rc = fq_check_no_alias(dev, y[i], yb, x, xb, "y")) return rc;
         for (size_t j = 0; j < i; j++)
-            if (int rc = fq_check_no_alias(dev, y[i], yb, y[j], m * w[j]->rows * fq_dtype_size(y_dtype), "y")) return rc;
+            if (int rc = fq_check_apart(dev, y[i], yb, y[j], m * w[j]->rows * fq_dtype_size(y_dtype), "y")) return rc;
         args[i] = base_args(w[i], x, x_dtype, y[i], y_dtype);
         args[i].rows = (uint32_t)w[i]->rows;
         args[i].m = (uint32_t)m;

@@ -716,7 +716,7 @@ extern "C" int fq_project_many_i8(fq_device *dev, const fq_matrix *const *w, siz
         if (int rc = fq_check_no_alias(dev, y[i], yb, x, x_elems, "y")) return rc;
         if (int rc = fq_check_no_alias(dev, y[i], yb, x_scales, m * 4, "y")) return rc;
         for (size_t j = 0; j < i; j++)
-            if (int rc = fq_check_no_alias(dev, y[i], yb, y[j], m * w[j]->rows * fq_dtype_size(y_dtype), "y")) return rc;
+            if (int rc = fq_check_apart(dev, y[i], yb, y[j], m * w[j]->rows * fq_dtype_size(y_dtype), "y")) return rc;
     }
     if (int rc = launch(dev, w, (uint32_t)count, x, x_scales, (uint32_t)m, y, y_dtype)) return rc;
     return fq_end_enqueue(dev, "project_i8", 1);

@@ -679,7 +679,7 @@ extern "C" int fq_token_logprobs(fq_device *dev, const void *logits, int dtype, 
         if (int rc = fq_check_no_alias(dev, out[i].p, out[i].bytes, ids, (size_t)rows * 4, out[i].name)) return rc;
         for (int j = 0; j < i; j++)
             if (out[j].wanted)
-                if (int rc = fq_check_no_alias(dev, out[i].p, out[i].bytes, out[j].p, out[j].bytes, out[i].name)) return rc;
+                if (int rc = fq_check_apart(dev, out[i].p, out[i].bytes, out[j].p, out[j].bytes, out[i].name)) return rc;
     }
     if (!any) return fq_fail(dev, FQ_ERR_PARAM, "no output is asked for");
     const Outputs o{logprobs, ranks, entropy, top_logprobs, top_ids};

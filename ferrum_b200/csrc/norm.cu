@@ -324,7 +324,8 @@ extern "C" int fq_add_rmsnorm(fq_device *dev, const float *x, const float *r, co
     if (int rc = check_norm(dev, x, w, n, rows, y)) return rc;
     if (int rc = fq_check_binding(dev, r, (size_t)rows * n * 4, "r")) return rc;
     if (int rc = fq_check_binding(dev, h, (size_t)rows * n * 4, "h")) return rc;
-    if (int rc = fq_check_no_alias(dev, y, (size_t)rows * n * 4, h, (size_t)rows * n * 4, "y")) return rc;
+    if (int rc = fq_check_apart(dev, y, (size_t)rows * n * 4, h, (size_t)rows * n * 4, "y")) return rc;
+    for (const float *out : {h, y}) fq_note_write(dev, out, (size_t)rows * n * 4);
     if (int rc = fq_check_cuda(dev, launch_norm(dev, x, r, w, n, eps, rows, h, y), "add_rmsnorm launch")) return rc;
     return fq_end_enqueue(dev, "add_rmsnorm", 1);
 }

@@ -509,7 +509,7 @@ int check_rows(fq_device *dev, const void *x, const void *r, int dtype, const fl
         if (int rc = fq_check_no_alias(dev, q, count, i.p, i.bytes, "q")) return rc;
         if (int rc = fq_check_no_alias(dev, scales, (size_t)rows * 4, i.p, i.bytes, "scales")) return rc;
     }
-    return fq_check_no_alias(dev, scales, (size_t)rows * 4, q, count, "scales");
+    return fq_check_apart(dev, scales, (size_t)rows * 4, q, count, "scales");
 }
 
 } // namespace
@@ -540,8 +540,8 @@ extern "C" int fq_add_rmsnorm_i8(fq_device *dev, const void *x, const void *r, i
     if (h != r)
         if (int rc = fq_check_no_alias(dev, h, bytes, r, bytes, "h")) return rc;
     if (int rc = fq_check_no_alias(dev, h, bytes, w, (size_t)n * 4, "h")) return rc;
-    if (int rc = fq_check_no_alias(dev, q, count, h, bytes, "q")) return rc;
-    if (int rc = fq_check_no_alias(dev, scales, (size_t)rows * 4, h, bytes, "scales")) return rc;
+    if (int rc = fq_check_apart(dev, q, count, h, bytes, "q")) return rc;
+    if (int rc = fq_check_apart(dev, scales, (size_t)rows * 4, h, bytes, "scales")) return rc;
     return launch_rows<ADD_NORM>(dev, "add_rmsnorm_i8", x, r, x_dtype, w, n, eps, rows, h, q, scales);
 }
 

@@ -634,3 +634,128 @@ def test_gates_far_below_zero(device, n, size, dtype):
         x[far] = np.resize(rng.permutation(every), far.sum())
     x, r = gpu(x, dtype), gpu(r, dtype)
     check_rows("glu", x, r, None, *run_op(device, "glu", x, r, None, rows))
+
+
+class Owned:
+    """Buffers of a handle's own (`fq_buffer_alloc`) as tensors."""
+
+    def __init__(self, d):
+        self.d, self.held = d, []
+
+    def __call__(self, *shape, dtype=F32):
+        import ctypes as C
+        size, p = int(np.prod(shape)) * dtype.itemsize, C.c_void_p()
+        self.d.check(self.d._L.fq_buffer_alloc(self.d.handle, size, C.byref(p)))
+        self.__cuda_array_interface__ = {"shape": (size,), "typestr": "|u1", "data": (p.value, False), "version": 3}
+        self.held.append(p)
+        return torch.as_tensor(self, device="cuda").view(dtype).view(shape).zero_()
+
+    def free(self):
+        torch.cuda.synchronize()
+        for p in self.held:
+            self.d.check(self.d._L.fq_buffer_free(self.d.handle, p))
+
+
+@pytest.fixture
+def own():
+    """A handle of the test's own and its buffers."""
+    d = S().Device(0)
+    b = Owned(d)
+    yield d, b
+    b.free()
+    d.close()
+
+
+def fail(d):
+    """What is enqueued turns out to have failed, and the handle is taken into use again."""
+    d.fail_completion()
+    with pytest.raises(S().SynchronizationError):
+        d.synchronize()
+    d.recover()
+
+
+def calls_of_the_8_bit_path(d, rng, new):
+    """name -> (call, its outputs, made by `new`), on inputs of their own."""
+    s, m, n = S(), 3, 64
+    x, r, w = gpu(rng.standard_normal((m, n))), gpu(rng.standard_normal((m, n))), gpu(1 + 0.1 * rng.standard_normal(n))
+    mats = [matrix(rng, d, rows, n)[0] for rows in (40, 24)]
+    xq, xs = gpu(rng.integers(-127, 128, (m, n)), torch.int8), gpu(rng.random(m))
+    ids = torch.arange(m, dtype=torch.int32, device="cuda")
+    i8, i32 = torch.int8, torch.int32
+    out = {"quantize": (new(m, n, dtype=i8), new(m)), "rmsnorm": (new(m, n, dtype=i8), new(m)), "add": (new(m, n), new(m, n, dtype=i8), new(m)),
+           "glu": (new(m, n, dtype=i8), new(m)), "project": (new(m, 40),), "many": (new(m, 40), new(m, 24)),
+           "scores": (new(m), new(m, dtype=i32), new(m), new(m, 5), new(m, 5, dtype=i32))}
+    calls = {"quantize": lambda q, sc: s.quantize_i8(d, x, m, q, sc), "rmsnorm": lambda q, sc: s.rmsnorm_i8(d, x, w, EPS, m, q, sc),
+             "add": lambda h, q, sc: s.add_rmsnorm_i8(d, x, r, w, EPS, m, h, q, sc), "glu": lambda q, sc: s.glu_i8(d, x, r, m, q, sc),
+             "project": lambda y: s.project_i8(d, mats[0], xq, xs, m, y), "many": lambda a, b: s.project_many_i8(d, mats, xq, xs, m, [a, b]),
+             "scores": lambda lp, rk, en, tp, ti: s.token_logprobs(d, x, n, m, ids, lp, rk, en, 5, tp, ti)}
+    torch.cuda.synchronize()
+    return {name: (calls[name], out[name]) for name in calls}
+
+
+def test_outputs_of_a_failed_submission_are_written_again(own):
+    """They are refused as inputs until then, but not as what they are: outputs."""
+    d, new = own
+    rng = np.random.default_rng(20)
+    for name, (call, out) in calls_of_the_8_bit_path(d, rng, new).items():
+        call(*out)
+        d.synchronize()
+        first = [t.clone() for t in out]
+        torch.cuda.synchronize()
+        call(*out)
+        fail(d)
+        for t in out:
+            t.fill_(9)
+        torch.cuda.synchronize()
+        call(*out)
+        d.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, first)), name
+
+
+def test_every_output_of_a_failed_submission_is_refused_as_an_input(own):
+    d, new = own
+    s, rng = S(), np.random.default_rng(21)
+    y, ys = torch.zeros(1, 40, device="cuda"), torch.ones(1, device="cuda")
+    q, sc = torch.zeros(1, 64, dtype=torch.int8, device="cuda"), torch.zeros(1, device="cuda")
+    w = matrix(rng, d, 40, 64)[0]
+    for name, (call, out) in calls_of_the_8_bit_path(d, rng, new).items():
+        call(*out)
+        fail(d)
+        for t in out:
+            with pytest.raises(s.SynchronizationError):
+                if t.dtype == torch.int8:
+                    s.project_i8(d, w, t[:1], ys, 1, y)
+                elif t.dtype == torch.int32:
+                    s.token_logprobs(d, torch.zeros(t.numel(), 8, device="cuda"), 8, t.numel(), t.view(-1), torch.zeros(t.numel(), device="cuda"), None, None)
+                elif t.dim() == 1:
+                    s.project_i8(d, w, q, t[:1], 1, y)
+                else:
+                    s.token_logprobs(d, t, t.shape[1], t.shape[0], None, None, None, torch.zeros(t.shape[0], device="cuda"))
+        call(*out)
+        d.synchronize()
+
+
+def test_two_outputs_of_a_failed_submission_are_written_again(own):
+    """The same of the calls on floats that have more than one output."""
+    from oracle import ref
+    d, new = own
+    s = S()
+    x, w = torch.ones(2, 256, device="cuda"), torch.ones(256, device="cuda")
+    mat = s.Matrix.from_packed(d, 16, 256, 1, s.Q4_K, ref.random_matrix(s.Q4_K, 16, 256, 1))
+    h, y, a, b, c = new(2, 256), new(2, 256), new(2, 16), new(2, 16), torch.zeros(2, 16, device="cuda")
+    torch.cuda.synchronize()
+    for call, out in ((lambda: s.add_rmsnorm(d, x, x, w, EPS, 2, h, y), (h, y)), (lambda: s.project_many(d, [mat, mat], x, 2, [a, b]), (a, b))):
+        call()
+        d.synchronize()
+        first = [t.clone() for t in out]
+        torch.cuda.synchronize()
+        call()
+        fail(d)
+        for t in out:
+            t.fill_(9)
+        torch.cuda.synchronize()
+        call()
+        d.synchronize()
+        assert all(torch.equal(t, f) for t, f in zip(out, first))
+    s.project(d, mat, h, 2, c)  # written again, so an input again
+    d.synchronize()
