@@ -221,16 +221,21 @@ int fq_check_apart(fq_device *dev, const void *a, size_t a_bytes, const void *b,
     return FQ_OK;
 }
 
+// What a failed submission wrote is not an input until it has been written again.  Only buffers the handle
+// allocated itself are tracked (`fq_buffer_alloc`, the counterpart of the reference's device buffers): memory the
+// caller owns is recycled and rewritten by the caller's allocator without the library seeing it.
+int fq_check_input(fq_device *dev, const void *in, size_t bytes, const char *name) {
+    const uintptr_t i = (uintptr_t)in;
+    for (const auto &f : dev->failed_writes)
+        if (i < f.second && f.first < i + bytes) return fq_fail(dev, FQ_ERR_SYNC, "%s: input range belongs to a failed submission", name);
+    return FQ_OK;
+}
+
 int fq_check_no_alias(fq_device *dev, const void *out, size_t out_bytes, const void *in, size_t in_bytes,
                       const char *name) {
-    const uintptr_t i = (uintptr_t)in;
     if (!out || !in) return FQ_OK;
     if (int rc = fq_check_apart(dev, out, out_bytes, in, in_bytes, name)) return rc;
-    // What a failed submission wrote is not an input until it has been written again.  Only buffers the handle
-    // allocated itself are tracked (`fq_buffer_alloc`, the counterpart of the reference's device buffers): memory the
-    // caller owns is recycled and rewritten by the caller's allocator without the library seeing it.
-    for (const auto &f : dev->failed_writes)
-        if (i < f.second && f.first < i + in_bytes) return fq_fail(dev, FQ_ERR_SYNC, "%s: input range belongs to a failed submission", name);
+    if (int rc = fq_check_input(dev, in, in_bytes, name)) return rc;
     fq_note_write(dev, out, out_bytes);
     return FQ_OK;
 }

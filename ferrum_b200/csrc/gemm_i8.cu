@@ -713,12 +713,15 @@ extern "C" int fq_project_many_i8(fq_device *dev, const fq_matrix *const *w, siz
         if (int rc = fq_check_binding(dev, x, x_elems, "x")) return rc;
         if (int rc = fq_check_binding(dev, x_scales, m * 4, "x_scales", 4)) return rc;
         if (int rc = fq_check_binding(dev, y[i], yb, "y")) return rc;
-        if (int rc = fq_check_no_alias(dev, y[i], yb, x, x_elems, "y")) return rc;
-        if (int rc = fq_check_no_alias(dev, y[i], yb, x_scales, m * 4, "y")) return rc;
+        if (int rc = fq_check_apart(dev, y[i], yb, x, x_elems, "y")) return rc;
+        if (int rc = fq_check_apart(dev, y[i], yb, x_scales, m * 4, "y")) return rc;
         for (size_t j = 0; j < i; j++)
             if (int rc = fq_check_apart(dev, y[i], yb, y[j], m * w[j]->rows * fq_dtype_size(y_dtype), "y")) return rc;
     }
+    if (int rc = fq_check_input(dev, x, x_elems, "x")) return rc;
+    if (int rc = fq_check_input(dev, x_scales, m * 4, "x_scales")) return rc;
     if (int rc = launch(dev, w, (uint32_t)count, x, x_scales, (uint32_t)m, y, y_dtype)) return rc;
+    for (size_t i = 0; i < count; i++) fq_note_write(dev, y[i], m * w[i]->rows * fq_dtype_size(y_dtype));
     return fq_end_enqueue(dev, "project_i8", 1);
 }
 

@@ -675,16 +675,21 @@ extern "C" int fq_token_logprobs(fq_device *dev, const void *logits, int dtype, 
         if (!out[i].wanted) continue;
         any = true;
         if (int rc = fq_check_binding(dev, out[i].p, out[i].bytes, out[i].name, 4)) return rc;
-        if (int rc = fq_check_no_alias(dev, out[i].p, out[i].bytes, logits, bytes, out[i].name)) return rc;
-        if (int rc = fq_check_no_alias(dev, out[i].p, out[i].bytes, ids, (size_t)rows * 4, out[i].name)) return rc;
+        if (int rc = fq_check_apart(dev, out[i].p, out[i].bytes, logits, bytes, out[i].name)) return rc;
+        if (int rc = fq_check_apart(dev, out[i].p, out[i].bytes, ids, (size_t)rows * 4, out[i].name)) return rc;
         for (int j = 0; j < i; j++)
             if (out[j].wanted)
                 if (int rc = fq_check_apart(dev, out[i].p, out[i].bytes, out[j].p, out[j].bytes, out[i].name)) return rc;
     }
     if (!any) return fq_fail(dev, FQ_ERR_PARAM, "no output is asked for");
+    if (int rc = fq_check_input(dev, logits, bytes, "logits")) return rc;
+    if (ids)
+        if (int rc = fq_check_input(dev, ids, (size_t)rows * 4, "ids")) return rc;
     const Outputs o{logprobs, ranks, entropy, top_logprobs, top_ids};
     const cudaError_t e = dtype == FQ_BF16 ? launch_rows(dev, (const __nv_bfloat16 *)logits, n, stride, rows, ids, k, o)
                                            : launch_rows(dev, (const float *)logits, n, stride, rows, ids, k, o);
     if (int rc = fq_check_cuda(dev, e, "token_logprobs launch")) return rc;
+    for (const auto &t : out)
+        if (t.wanted) fq_note_write(dev, t.p, t.bytes);
     return fq_end_enqueue(dev, "token_logprobs", 1);
 }

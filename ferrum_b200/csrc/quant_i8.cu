@@ -487,6 +487,10 @@ int launch_rows(fq_device *dev, const char *what, const void *x, const void *r, 
                           : n % 8 == 0    ? launch_vec<OP, __nv_bfloat16, 8>(dev, x, r, w, n, eps, rows, h, q, scales)
                                           : launch_vec<OP, __nv_bfloat16, 4>(dev, x, r, w, n, eps, rows, h, q, scales);
     if (int rc = fq_check_cuda(dev, e, what)) return rc;
+    const size_t count = (size_t)rows * n;
+    if (h) fq_note_write(dev, h, count * fq_dtype_size(dtype));
+    fq_note_write(dev, q, count);
+    fq_note_write(dev, scales, (size_t)rows * 4);
     return fq_end_enqueue(dev, what, 1);
 }
 
@@ -504,10 +508,12 @@ int check_rows(fq_device *dev, const void *x, const void *r, int dtype, const fl
         if (int rc = fq_check_binding(dev, w, (size_t)n * 4, "w")) return rc;
     if (int rc = fq_check_binding(dev, q, count, "q")) return rc;
     if (int rc = fq_check_binding(dev, scales, (size_t)rows * 4, "scales", 4)) return rc;
-    const struct { const void *p; size_t bytes; } in[3] = {{x, bytes}, {r, bytes}, {w, (size_t)n * 4}};
+    const struct { const void *p; size_t bytes; const char *name; } in[3] = {{x, bytes, "x"}, {r, bytes, "r"}, {w, (size_t)n * 4, "w"}};
     for (const auto &i : in) {
-        if (int rc = fq_check_no_alias(dev, q, count, i.p, i.bytes, "q")) return rc;
-        if (int rc = fq_check_no_alias(dev, scales, (size_t)rows * 4, i.p, i.bytes, "scales")) return rc;
+        if (!i.p) continue;
+        if (int rc = fq_check_apart(dev, q, count, i.p, i.bytes, "q")) return rc;
+        if (int rc = fq_check_apart(dev, scales, (size_t)rows * 4, i.p, i.bytes, "scales")) return rc;
+        if (int rc = fq_check_input(dev, i.p, i.bytes, i.name)) return rc;
     }
     return fq_check_apart(dev, scales, (size_t)rows * 4, q, count, "scales");
 }
@@ -536,10 +542,10 @@ extern "C" int fq_add_rmsnorm_i8(fq_device *dev, const void *x, const void *r, i
     if (int rc = fq_check_binding(dev, h, bytes, "h")) return rc;
     // h may be x or r itself: a value of h is written by the thread that read it.
     if (h != x)
-        if (int rc = fq_check_no_alias(dev, h, bytes, x, bytes, "h")) return rc;
+        if (int rc = fq_check_apart(dev, h, bytes, x, bytes, "h")) return rc;
     if (h != r)
-        if (int rc = fq_check_no_alias(dev, h, bytes, r, bytes, "h")) return rc;
-    if (int rc = fq_check_no_alias(dev, h, bytes, w, (size_t)n * 4, "h")) return rc;
+        if (int rc = fq_check_apart(dev, h, bytes, r, bytes, "h")) return rc;
+    if (int rc = fq_check_apart(dev, h, bytes, w, (size_t)n * 4, "h")) return rc;
     if (int rc = fq_check_apart(dev, q, count, h, bytes, "q")) return rc;
     if (int rc = fq_check_apart(dev, scales, (size_t)rows * 4, h, bytes, "scales")) return rc;
     return launch_rows<ADD_NORM>(dev, "add_rmsnorm_i8", x, r, x_dtype, w, n, eps, rows, h, q, scales);

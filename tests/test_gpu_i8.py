@@ -759,3 +759,32 @@ def test_two_outputs_of_a_failed_submission_are_written_again(own):
         assert all(torch.equal(t, f) for t, f in zip(out, first))
     s.project(d, mat, h, 2, c)  # written again, so an input again
     d.synchronize()
+
+
+def test_a_refused_call_has_written_nothing(own):
+    """What a failed submission wrote stays refused after a call into it that was itself refused."""
+    d, new = own
+    s, rng = S(), np.random.default_rng(22)
+    x, w = gpu(rng.standard_normal((2, 64))), torch.ones(64, device="cuda")
+    mat = matrix(rng, d, 64, 64)[0]
+    q, sc, h, y, lp = new(2, 64, dtype=torch.int8), new(2), new(2, 64), new(2, 64), new(2)
+    spare, ids = torch.zeros(2, 64, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    s.add_rmsnorm_i8(d, x, x, w, EPS, 2, h, q, sc)
+    s.project_i8(d, mat, q, sc, 2, y)
+    s.token_logprobs(d, y, 64, 2, ids, lp, None, None)
+    fail(d)
+    part = x.view(-1)[:2]
+    for call in (lambda: s.quantize_i8(d, x, 2, q, part), lambda: s.rmsnorm_i8(d, x, w, EPS, 2, q, w[:2]), lambda: s.glu_i8(d, x, x, 2, q, part),
+                 lambda: s.add_rmsnorm_i8(d, x, x, w, EPS, 2, h, q, part), lambda: s.add_rmsnorm_i8(d, x, x, w, EPS, 2, h, q, h.view(-1)[:2]),
+                 lambda: s.project_many_i8(d, [mat, mat], torch.zeros_like(q), torch.ones(2, device="cuda"), 2, [y, y]),
+                 lambda: s.token_logprobs(d, spare, 64, 2, ids, lp, None, lp)):
+        with pytest.raises(s.AliasError):
+            call()
+    d.synchronize()
+    for call in (lambda: s.project_i8(d, mat, q, torch.ones(2, device="cuda"), 2, spare), lambda: s.project_i8(d, mat, torch.zeros_like(q), sc, 2, spare),
+                 lambda: s.quantize_i8(d, h, 2, torch.zeros_like(q), torch.zeros(2, device="cuda")),
+                 lambda: s.quantize_i8(d, y, 2, torch.zeros_like(q), torch.zeros(2, device="cuda")),
+                 lambda: s.project_i8(d, mat, torch.zeros_like(q), lp, 2, spare)):
+        with pytest.raises(s.SynchronizationError):
+            call()
