@@ -638,12 +638,17 @@ extern "C" int fq_matrix_create_i8(fq_device *dev, uint64_t rows, uint64_t cols,
     if (cols > FQ_MAX_COLS || rows > 0x7fffffffull / 128) return fq_fail(dev, FQ_ERR_SHAPE, "matrix geometry is out of range");
     if (dev->capturing) return fq_fail(dev, FQ_ERR_PARAM, "a matrix cannot be created inside a graph capture");
     if (int rc = fq_check_cuda(dev, cudaSetDevice(dev->ordinal), "cudaSetDevice")) return rc;
-    bool on_device = false;
-    for (const void *p : {(const void *)scales, (const void *)values}) {
+    bool on_device = false; // the values
+    const struct { const void *p; size_t bytes; const char *name; } payload[2] = {{scales, rows * 4, "scales"}, {values, rows * cols, "values"}};
+    for (const auto &t : payload) {
         cudaPointerAttributes attr{};
-        if (int rc = fq_check_cuda(dev, cudaPointerGetAttributes(&attr, p), "payload")) return rc;
-        if (attr.type == cudaMemoryTypeDevice && attr.device != dev->ordinal) return fq_fail(dev, FQ_ERR_DEVICE, "the payload is on device %d", attr.device);
+        if (int rc = fq_check_cuda(dev, cudaPointerGetAttributes(&attr, t.p), "payload")) return rc;
         on_device = attr.type == cudaMemoryTypeDevice;
+        if (!on_device) continue;
+        if (attr.device != dev->ordinal) return fq_fail(dev, FQ_ERR_DEVICE, "the payload is on device %d", attr.device);
+        // What makes the payload has to have ended well: no later call would see that a matrix was made of anything else.
+        if (int rc = fq_synchronize(dev)) return rc;
+        if (int rc = fq_check_input(dev, t.p, t.bytes, t.name)) return rc;
     }
     const std::unique_ptr<float[]> host(new (std::nothrow) float[rows]);
     if (!host) return fq_fail(dev, FQ_ERR_CUDA, "no host memory for %llu scales", (unsigned long long)rows);

@@ -267,8 +267,9 @@ int fq_add_rmsnorm_i8(fq_device *dev, const void *x, const void *r, int x_dtype,
                       int8_t *q, float *scales);
 int fq_glu_i8(fq_device *dev, const void *gate, const void *up, int dtype, uint32_t n, uint32_t rows, int8_t *q, float *scales);
 /* A matrix of 8-bit integers, [rows][cols], with a scale for each row; cols is a multiple of 16 and at most 65536.  `values`
- * and `scales` may be host memory or memory of the handle's device (read in the order of the handle's stream; the call waits
- * for the copy), e.g. what `fq_quantize_i8` makes of a matrix of floats.  Scales must be finite (FQ_ERR_WEIGHT).
+ * and `scales` may be host memory or memory of the handle's device, e.g. what `fq_quantize_i8` makes of a matrix of floats.  The
+ * call waits for the copy, and for memory of the device first for all that is enqueued, as `fq_synchronize` does and with its
+ * errors.  Scales must be finite (FQ_ERR_WEIGHT).
  * `fq_matrix_destroy` and `fq_matrix_get_info` as for the other formats (byte_size = rows * (cols + 4)). */
 int fq_matrix_create_i8(fq_device *dev, uint64_t rows, uint64_t cols, const int8_t *values, const float *scales, fq_matrix **out);
 /* y[t][o] = (sum_k x[t][k] w[o][k]) * x_scales[t] * w_scale[o] for m rows of 8-bit integers.  The sum is exact at every

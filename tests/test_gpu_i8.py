@@ -788,3 +788,25 @@ def test_a_refused_call_has_written_nothing(own):
                  lambda: s.project_i8(d, mat, torch.zeros_like(q), lp, 2, spare)):
         with pytest.raises(s.SynchronizationError):
             call()
+
+
+def test_no_matrix_is_made_of_what_a_failed_submission_wrote(own):
+    d, new = own
+    s, rng = S(), np.random.default_rng(23)
+    x = gpu(rng.standard_normal((32, 64)))
+    q, sc = new(32, 64, dtype=torch.int8), new(32)
+    good = torch.ones(32, 64, dtype=torch.int8, device="cuda"), torch.ones(32, device="cuda")
+    torch.cuda.synchronize()
+    s.quantize_i8(d, x, 32, q, sc)
+    d.fail_completion()
+    with pytest.raises(s.SynchronizationError):  # the submission that makes the integers: this call waits for it
+        s.Matrix.from_i8(d, q, sc)
+    d.recover()
+    for values, scales in ((q, good[1]), (good[0], sc), (q, sc.cpu())):
+        with pytest.raises(s.SynchronizationError):
+            s.Matrix.from_i8(d, values, scales)
+    s.Matrix.from_i8(d, *good)
+    s.quantize_i8(d, x, 32, q, sc)
+    w = s.Matrix.from_i8(d, q, sc)
+    xq, xs = rng.integers(-127, 128, (3, 64), dtype=np.int8), np.ones(3, np.float32)
+    assert same(project(d, [w], xq, xs, F32, False)[0], expect(xq, xs, q.cpu().numpy(), sc.cpu().numpy()))
