@@ -646,6 +646,7 @@ extern "C" int fq_matrix_create_i8(fq_device *dev, uint64_t rows, uint64_t cols,
         on_device = attr.type == cudaMemoryTypeDevice;
         if (!on_device) continue;
         if (attr.device != dev->ordinal) return fq_fail(dev, FQ_ERR_DEVICE, "the payload is on device %d", attr.device);
+        if (int rc = fq_check_binding(dev, t.p, t.bytes, t.name, 1)) return rc;
         // What makes the payload has to have ended well: no later call would see that a matrix was made of anything else.
         if (int rc = fq_synchronize(dev)) return rc;
         if (int rc = fq_check_input(dev, t.p, t.bytes, t.name)) return rc;

@@ -810,3 +810,16 @@ def test_no_matrix_is_made_of_what_a_failed_submission_wrote(own):
     w = s.Matrix.from_i8(d, q, sc)
     xq, xs = rng.integers(-127, 128, (3, 64), dtype=np.int8), np.ones(3, np.float32)
     assert same(project(d, [w], xq, xs, F32, False)[0], expect(xq, xs, q.cpu().numpy(), sc.cpu().numpy()))
+
+
+def test_no_matrix_is_made_of_memory_past_an_allocation(own):
+    d, new = own
+    import ctypes as C
+    s = S()
+    q, sc = new(32, 64, dtype=torch.int8), new(32)
+    torch.cuda.synchronize()
+    for values, scales in ((q.data_ptr() + 16, sc.data_ptr()), (q.data_ptr(), sc.data_ptr() + 4)):
+        out = C.c_void_p()
+        with pytest.raises(s.RangeError):
+            d.check(d._L.fq_matrix_create_i8(d.handle, 32, 64, values, scales, C.byref(out)))
+        assert not out.value
