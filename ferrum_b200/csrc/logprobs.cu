@@ -659,7 +659,9 @@ extern "C" int fq_token_logprobs(fq_device *dev, const void *logits, int dtype, 
                                  uint32_t k, float *logprobs, uint32_t *ranks, float *entropy, float *top_logprobs, uint32_t *top_ids) {
     if (int rc = fq_begin_enqueue(dev)) return rc;
     if (dtype != FQ_F32 && dtype != FQ_BF16) return fq_fail(dev, FQ_ERR_UNSUPPORTED, "element type %d", dtype);
-    if (n == 0 || n > 0x7fffffffu || rows == 0 || rows > 0x7fffffffu / MAX_CLUSTER || stride < n) return fq_fail(dev, FQ_ERR_SHAPE, "%u rows of %u logits, %zu apart", rows, n, stride);
+    // (A stride whose bytes pass 64 bits would pass the check of the binding too.)
+    if (n == 0 || n > 0x7fffffffu || rows == 0 || rows > 0x7fffffffu / MAX_CLUSTER || stride < n || (rows > 1 && stride > (SIZE_MAX >> 4) / (rows - 1)))
+        return fq_fail(dev, FQ_ERR_SHAPE, "%u rows of %u logits, %zu apart", rows, n, stride);
     if (k > MAX_TOP || k > n) return fq_fail(dev, FQ_ERR_PARAM, "%u alternatives of %u tokens (at most %u)", k, n, MAX_TOP);
     const size_t bytes = ((size_t)(rows - 1) * stride + n) * fq_dtype_size(dtype);
     if (int rc = fq_check_binding(dev, logits, bytes, "logits", (uint32_t)fq_dtype_size(dtype))) return rc;

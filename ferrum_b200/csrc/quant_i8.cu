@@ -499,8 +499,9 @@ int check_rows(fq_device *dev, const void *x, const void *r, int dtype, const fl
                const float *scales) {
     if (dtype != FQ_F32 && dtype != FQ_BF16) return fq_fail(dev, FQ_ERR_UNSUPPORTED, "element type %d", dtype);
     if (n == 0 || n % 4 || rows == 0) return fq_fail(dev, FQ_ERR_SHAPE, "%u rows of %u values in 8 bits (a multiple of 4)", rows, n);
-    if (rows > 0x7fffffffu) return fq_fail(dev, FQ_ERR_SHAPE, "too many rows");
-    const size_t count = (size_t)rows * n, bytes = count * fq_dtype_size(dtype);
+    const size_t count = (size_t)rows * n;
+    if (rows > 0x7fffffffu || count > SIZE_MAX >> 4) return fq_fail(dev, FQ_ERR_SHAPE, "too many rows"); // (bytes that pass 64 bits would pass the checks)
+    const size_t bytes = count * fq_dtype_size(dtype);
     if (int rc = fq_check_binding(dev, x, bytes, "x")) return rc;
     if (r)
         if (int rc = fq_check_binding(dev, r, bytes, "r")) return rc;

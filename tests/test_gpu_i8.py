@@ -823,3 +823,26 @@ def test_no_matrix_is_made_of_memory_past_an_allocation(own):
         with pytest.raises(s.RangeError):
             d.check(d._L.fq_matrix_create_i8(d.handle, 32, 64, values, scales, C.byref(out)))
         assert not out.value
+
+
+def test_sizes_whose_bytes_pass_64_bits(own):
+    """They are refused as shapes, not cut to what a buffer holds."""
+    from ferrum_b200 import _lib
+    d, new = own
+    s = S()
+    x, q, sc, ids = new(8, 64), new(8, 64, dtype=torch.int8), new(8), new(8, dtype=torch.int32)
+    torch.cuda.synchronize()
+    lib, h, before = d._L, d.handle, d.counters().dispatches
+    n, rows = 2 ** 32 - 4, 2 ** 31 - 1
+    for rc in (lib.fq_token_logprobs(h, x.data_ptr(), _lib.F32, 4, 2 ** 62, 5, ids.data_ptr(), 0, sc.data_ptr(), None, None, None, None),
+               lib.fq_token_logprobs(h, x.data_ptr(), _lib.BF16, 4, 2 ** 63, 3, ids.data_ptr(), 0, sc.data_ptr(), None, None, None, None),
+               lib.fq_token_logprobs(h, x.data_ptr(), _lib.F32, 4, 2 ** 64 - 4, 2, ids.data_ptr(), 0, sc.data_ptr(), None, None, None, None),
+               lib.fq_quantize_i8(h, x.data_ptr(), _lib.F32, n, rows, q.data_ptr(), sc.data_ptr()),
+               lib.fq_rmsnorm_i8(h, x.data_ptr(), _lib.BF16, x.data_ptr(), n, EPS, rows, q.data_ptr(), sc.data_ptr())):
+        with pytest.raises(s.ShapeError):
+            d.check(rc)
+    with pytest.raises(s.RangeError):  # rows that a buffer does not hold
+        d.check(lib.fq_token_logprobs(h, x.data_ptr(), _lib.F32, 4, 128, 5, ids.data_ptr(), 0, sc.data_ptr(), None, None, None, None))
+    assert d.counters().dispatches == before
+    s.token_logprobs(d, x.view(-1), 4, 1, ids[:1], sc[:1], None, None, stride=2 ** 62)  # one row has no next one
+    d.synchronize()
