@@ -434,7 +434,9 @@ k_rows_i8(const T *x, const T *r, const float *w, uint32_t n, float eps, uint32_
     }
 }
 
-constexpr size_t STAGE_MOST = 200 << 10;
+constexpr size_t STAGE_MOST = 200 << 10, BULK_MOST = 74 << 10; // bytes of v of a row: what fits, and three blocks an SM
+constexpr uint32_t NARROW_GROUPS = 1600;                       // of a row, for blocks of fewer than 512 threads
+static_assert(NARROW_GROUPS * 8 * 4 <= BULK_MOST && 8 * 1024 * 4 <= BULK_MOST, "only blocks of 512 threads get longer rows");
 
 // What a kernel may use of an SM's shared memory beyond what it may unasked (48 KB with its own arrays): asked for once per device.
 template <typename K> cudaError_t allow(fq_device *dev, K kernel, size_t bytes, std::atomic<uint64_t> &asked) {
@@ -451,19 +453,27 @@ cudaError_t launch_nt(fq_device *dev, const T *x, const T *r, const float *w, ui
     const size_t bytes = (size_t)n * 4 * (NT == 32 ? 8 : 1);
     const dim3 grid(NT == 32 ? (rows + 7) / 8 : rows), block(NT == 32 ? 256 : NT);
     const double inv_n = 1.0 / n;
-    if constexpr (NT != 32 && VEC == 8)
-        if (bytes <= (74 << 10)) { // three blocks an SM
+    auto go = [&](auto kernel, size_t smem, std::atomic<uint64_t> &asked) {
+        if (const cudaError_t e = allow(dev, kernel, smem, asked)) return e;
+        return launch_pdl(kernel, grid, block, smem, dev->stream, x, r, w, n, eps, rows, h, q, scales, inv_n, dev->status_dev);
+    };
+    // Each mode for the rows that it gets: bulk copies bring in eight bf16 values a thread at a time, and only 512 threads get rows
+    // past BULK_MOST.
+    constexpr bool BULKS = NT != 32 && VEC == 8;
+    if constexpr (BULKS)
+        if (NT != 512 || bytes <= BULK_MOST) {
             static std::atomic<uint64_t> asked{0};
-            auto kernel = k_rows_i8<OP, T, VEC, NT, BULK>;
-            if (const cudaError_t e = allow(dev, kernel, bytes, asked)) return e;
-            return launch_pdl(kernel, grid, block, bytes, dev->stream, x, r, w, n, eps, rows, h, q, scales, inv_n, dev->status_dev);
+            return go(k_rows_i8<OP, T, VEC, NT, BULK>, bytes, asked);
         }
-    if (bytes > STAGE_MOST)
-        return launch_pdl(k_rows_i8<OP, T, VEC, NT, DIRECT>, grid, block, 0, dev->stream, x, r, w, n, eps, rows, h, q, scales, inv_n, dev->status_dev);
-    static std::atomic<uint64_t> asked{0};
-    auto kernel = k_rows_i8<OP, T, VEC, NT, KEPT>;
-    if (const cudaError_t e = allow(dev, kernel, bytes, asked)) return e;
-    return launch_pdl(kernel, grid, block, bytes, dev->stream, x, r, w, n, eps, rows, h, q, scales, inv_n, dev->status_dev);
+    if constexpr (NT == 512)
+        if (bytes > STAGE_MOST) {
+            static std::atomic<uint64_t> asked{0};
+            return go(k_rows_i8<OP, T, VEC, NT, DIRECT>, 0, asked);
+        }
+    if constexpr (!BULKS || NT == 512) {
+        static std::atomic<uint64_t> asked{0};
+        return go(k_rows_i8<OP, T, VEC, NT, KEPT>, bytes, asked);
+    }
 }
 
 template <int OP, typename T, int VEC>
@@ -475,7 +485,7 @@ cudaError_t launch_vec(fq_device *dev, const void *x, const void *r, const float
     // With many rows the threads that a row's sums are joined over cost more than the time a row waits for itself; a few rows wait.
     // us with 128 / 256 / 512 threads: add_rmsnorm bf16 2048 x 5120 21.1 / 19.5 / -, gated unit 14.8 / 16.4 / -, 1021 x 17408 - /
     // 24.5 / 22.2; add_rmsnorm F32 of one row of 5120 - / 4.1 / 3.5, of 200 - / 6.5 / 5.3.
-    if (groups > (few ? 512 : 1600)) return launch_nt<OP, T, VEC, 512>(dev, tx, tr, w, n, eps, rows, (T *)h, q, scales);
+    if (groups > (few ? 512 : NARROW_GROUPS)) return launch_nt<OP, T, VEC, 512>(dev, tx, tr, w, n, eps, rows, (T *)h, q, scales);
     if (groups > (few ? 256 : OP == ADD_NORM ? 400 : 800)) return launch_nt<OP, T, VEC, 256>(dev, tx, tr, w, n, eps, rows, (T *)h, q, scales);
     return launch_nt<OP, T, VEC, 128>(dev, tx, tr, w, n, eps, rows, (T *)h, q, scales);
 }

@@ -846,3 +846,22 @@ def test_sizes_whose_bytes_pass_64_bits(own):
     assert d.counters().dispatches == before
     s.token_logprobs(d, x.view(-1), 4, 1, ids[:1], sc[:1], None, None, stride=2 ** 62)  # one row has no next one
     d.synchronize()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows", [3, 150])
+@pytest.mark.parametrize("n", [18944, 18952, 28672, 51200, 51208, 65536])
+@pytest.mark.parametrize("op", OPS)
+def test_rows_around_the_ends_of_shared_memory(device, op, n, rows, dtype):
+    """The longest rows that bulk copies bring in (18944) and that are kept (51200), the next ones, and widths between."""
+    rng = np.random.default_rng(n + rows)
+    x = gpu(rng.standard_normal((rows, n)) * (1 + 30 * (rng.random(n) < 0.01)), dtype)
+    r, w = gpu(rng.standard_normal((rows, n)), dtype), gpu(1 + 0.1 * rng.standard_normal(n))
+    h = torch.zeros_like(x)
+    q, s = run_op(device, op, x, r, w, rows, h)
+    check_rows(op, x, r, w, q, s)
+    if op == "add":
+        assert torch.equal(h.cpu(), values_of(op, x, r, w)[2])
+        for first, second, place in ((x.clone(), r, 0), (x, r.clone(), 1)):  # the sum in place of either input
+            place = (first, second)[place]
+            assert np.array_equal(run_op(device, op, first, second, w, rows, place)[0], q) and torch.equal(place, h)
