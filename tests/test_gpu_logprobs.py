@@ -350,3 +350,16 @@ def test_one_token_with_all_of_the_probability(device, rows, n, dtype):
             got = run(device, t.cuda().view(-1), n, ids, k)
             check(t.double().numpy(), ids, k, got)
             assert (got[0] <= 0).all() and (got[2] >= 0).all() and (got[3] <= 0).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows", [1, 74, 75, 296, 400])
+@pytest.mark.parametrize("n", [8191, 8192, 8193, 16384, 65536])
+def test_lengths_at_which_rows_are_cut_otherwise(device, n, rows, dtype):
+    """8192 logits are the fewest that two blocks share, and the longest rows of the smallest blocks; 65536 the longest bf16 ones.
+    A block notes 8 (of 256 threads; of 512: 4, of 128: 16) maxima a thread."""
+    rng = np.random.default_rng(n + rows)
+    l = torch.from_numpy(logits(rng, rows, n)).to(dtype)
+    ids = rng.integers(0, n, rows)
+    for k in (0, 7, 32):
+        check(l.double().numpy(), ids, k, run(device, l.cuda().view(-1), n, ids, k))
