@@ -4,7 +4,7 @@
 //   z = log sum_j exp(l_j)     logprob = l_id - z     rank = 1 + |{j: l_j > l_id}|     entropy = z - sum_j exp(l_j - z) l_j
 //
 // A logit of -infinity is a token of probability 0 and adds nothing anywhere.  A row with a NaN, with +infinity or with nothing
-// above -infinity has no distribution: its numbers are NaN.
+// above -infinity has no distribution: its numbers are NaN, and its rank counts what compares above l_id.
 //
 // A row is read once, by a block or by a cluster of blocks (each a contiguous part; block 0 collects through distributed shared
 // memory).  In powers of two, with b = log2(e) as fp32 has it and a pivot c:
@@ -175,7 +175,7 @@ __device__ __forceinline__ Sums join_warp(Sums a, int lanes = 32) {
     }
     return a;
 }
-// A row of logits around numbers beyond MOST: by one warp, in 64 bits about its largest.
+// A row of logits around numbers beyond MOST: by one warp, in 64 bits about its largest (151936 of them 1.7 ms; no model has such).
 template <typename T> __device__ __noinline__ void sum_64(const T *l, uint32_t n, uint32_t lane, double &z, double &entropy) {
     double mx = -INFINITY, s = 0.0, t = 0.0;
     for (uint32_t i = lane; i < n; i += 32) mx = fmax(mx, (double)load1(l, i));

@@ -15,8 +15,10 @@
 // (Held in registers, unrolled over a row, the same took 105 registers and 63 instructions a value, a third of the time
 // waiting for instructions: 2048 x 5120 bf16 45 us.)
 //
-// What bounds it is a row's chain of dependent steps, of which the blocks of an SM cover a part: add_rmsnorm of 2048 x 5120 bf16
-// 20 us (3.7 TB/s) and F32 26 us (5.2 TB/s), the gated unit of 1021 x 17408 bf16 22 us (4.0 TB/s), one row of 5120 F32 3.5 us.
+// What bounds it is a row's chain of dependent steps, of which the blocks of an SM cover a part.  2048 x 5120, bf16 / F32: quantize
+// 11.5 / 14.8 us (2.7 / 3.6 TB/s), rmsnorm 13.1 / 16.1 (2.4 / 3.3), add_rmsnorm 20.0 / 28.1 (3.7 / 4.8); the gated unit of 1021 x
+// 17408 22.3 / 39.1 (4.0 / 4.1), of 28672 values a row, of which an SM holds one or two, 49 / 63 (3.0 / 4.1), of 53248, computed
+// twice, 111 / 195 (2.5 / 2.5); one row of 5120 F32 2.2, 2.5 and 3.4.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>

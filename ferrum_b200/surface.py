@@ -573,7 +573,8 @@ def token_logprobs(d: Device, logits: torch.Tensor, n: int, rows: int, ids: Opti
                    ranks: Optional[torch.Tensor], entropy: Optional[torch.Tensor], k: int = 0, top_logprobs: Optional[torch.Tensor] = None,
                    top_ids: Optional[torch.Tensor] = None, stride: Optional[int] = None) -> None:
     """Log probability and rank of the token ``ids[r]`` under row r of ``rows`` rows of n logits (``stride`` values apart, n by
-    default), the rows' entropy, and their k most likely tokens.  Outputs that are None are not computed."""
+    default), the rows' entropy, and their k most likely tokens.  Outputs that are None are not computed.  ``logits`` is contiguous:
+    of a head with more columns than tokens it is the whole output, with ``stride`` its columns.  Ids are int32."""
     _need(d, logits)
     stride = n if stride is None else stride
     if not 0 < n <= _MOST or not 0 < rows <= _MOST or stride < n or logits.numel() < (rows - 1) * stride + n:

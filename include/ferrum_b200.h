@@ -260,7 +260,10 @@ int fq_topk_blocks(fq_device *dev, const float *x, uint32_t n, uint32_t rows, fl
  *   fq_glu_i8           v = silu(gate) * up
  * The row inputs are F32 or BF16, `rows` rows of n values (a multiple of 4); w is F32.  A row of zeros has scale 0.  A row
  * with an infinity or a NaN among its inputs or its v (for the norms: among h * w) has scale NaN and q = 0, which makes NaN of
- * everything projected from it and of nothing else.  Scales may start at any 4 bytes (those of later rows of a batch do). */
+ * everything projected from it and of nothing else.  Scales may start at any 4 bytes (those of later rows of a batch do).
+ * A row is worked out in 64 bits value by value, three to eight times as slowly (2048 rows of 5120 values 49 to 63 us, a gated unit
+ * of 1021 x 17408 170 us), where the largest |v| is not within 1e-20 .. 1e37 (of fq_quantize_i8 .. 2.5e36), a norm's largest
+ * sum of four squares (eight, of bf16) is not either, or a gated unit's largest |up| is above 2^20. */
 int fq_quantize_i8(fq_device *dev, const void *x, int x_dtype, uint32_t n, uint32_t rows, int8_t *q, float *scales);
 int fq_rmsnorm_i8(fq_device *dev, const void *x, int x_dtype, const float *w, uint32_t n, float eps, uint32_t rows, int8_t *q, float *scales);
 int fq_add_rmsnorm_i8(fq_device *dev, const void *x, const void *r, int x_dtype, const float *w, uint32_t n, float eps, uint32_t rows, void *h,
@@ -293,8 +296,10 @@ int fq_project_many_i8(fq_device *dev, const fq_matrix *const *w, size_t count, 
  * Log probabilities are never above 0 and entropies never below it.
  * A logit of -infinity is a token of probability 0: it adds nothing, and its own log probability is -infinity.  A row with a
  * NaN, with +infinity, or with nothing above -infinity has no distribution: its log probabilities and entropy are NaN; ranks
- * and top_ids still follow the order of the logits, a NaN below everything.  An id that is not below n names no token (a row
- * of padding): log probability NaN, rank 0.  Logits may start at any element and the other arrays at any 4 bytes. */
+ * and top_ids still follow the order of the logits: a NaN is the last of the alternatives, it is above no given logit, and nothing is
+ * above a given NaN, whose rank is 1.  An id that is not below n names no token (a row of padding): log probability NaN, rank 0.
+ * Logits may start at any element and the other arrays at any 4 bytes.
+ * A row whose largest logit is beyond 2^20 or below -2^20 is summed in 64 bits by one warp: 1.7 ms for 151936 logits instead of 9 us. */
 int fq_token_logprobs(fq_device *dev, const void *logits, int dtype, uint32_t n, size_t stride, uint32_t rows, const uint32_t *ids, uint32_t k,
                       float *logprobs, uint32_t *ranks, float *entropy, float *top_logprobs, uint32_t *top_ids);
 
