@@ -111,10 +111,11 @@ int fq_end_enqueue(fq_device *dev, const char *what, int kernels);
 // Binding checks shared by the op surface (null, alignment, ownership range, overlap).
 void fq_note_write(fq_device *dev, const void *out, size_t bytes); // an enqueue writes [out, out + bytes)
 int fq_check_binding(fq_device *dev, const void *p, size_t bytes, const char *name, uint32_t align = 16);
+// An output that is apart from an input, which no failed submission has written; the output is noted as written.
 int fq_check_no_alias(fq_device *dev, const void *out, size_t out_bytes, const void *in,
-                      size_t in_bytes, const char *name); // of calls that check one output and write it: the three below
-// The parts of it.  Two outputs are only apart: either may be what a failed submission has written.  A call with checks
-// after the first one notes its outputs when it has launched: a refused one has written nothing.
+                      size_t in_bytes, const char *name);
+// The same in parts.  Two outputs have to be apart only: either may be what a failed submission has written.  A call that
+// checks more after this notes its outputs (fq_note_write) when it has launched: a refused one has written nothing.
 int fq_check_input(fq_device *dev, const void *in, size_t bytes, const char *name);
 int fq_check_apart(fq_device *dev, const void *a, size_t a_bytes, const void *b, size_t b_bytes, const char *name);
 
